@@ -222,6 +222,92 @@ typedef struct {
 } zkfp_gated_norm_args;
 int zkfp_gated_norm(const zkfp_gated_norm_args* a, void* stream);
 
+/* ---- a pool of pages ---------------------------------------------------------------------------------------------
+ * Keys and values of many sequences live in pages of `page` positions (a power of two from 8 to 1024), in no order.
+ * Position j of sequence b is line j % page of page table[b * table_ld + j / page]; a sequence may hold up to
+ * table_cols * page positions.  Rows rows[b] .. rows[b + 1] - 1 of a batch are the newest tokens of sequence b, which
+ * holds lengths[b] positions with them: row rows[b] + t sits at position lengths[b] - (rows[b + 1] - rows[b]) + t.
+ * All three are device data and are checked there: what lies outside the tensors is not read or written, and
+ * zkfp_device_status() reports it.  Rows behind rows[batch] are left as they were. */
+
+/* Softmax attention of new tokens over pages: a row sees the positions up to its own (window > 0: the last `window` of
+ * them); a row at a negative position sees none and gives zeros.  Keys and values that a row does not see have no part in
+ * it, whatever they hold. */
+typedef struct {
+    const void* q;         /* [tokens][heads][d] */
+    const void* k;         /* [pages][page][kv_heads][d] */
+    const void* v;         /* [pages][page][kv_heads][dv] */
+    void* out;             /* [tokens][heads][dv] */
+    const void* gate;      /* may be null: out is multiplied by sigmoid(gate[row][head][c]) * out_scale */
+    const int* table;
+    const int* rows;       /* [batch + 1] */
+    const int* lengths;    /* [batch] */
+    float* scratch;        /* zkfp_paged_scratch() floats, this call's alone */
+    long long q_tok, q_head, k_page, k_pos, k_head, v_page, v_pos, v_head, o_tok, o_head, gate_tok, gate_head;   /* elements */
+    long long tokens, pages, table_cols, table_ld, batch;
+    long long max_tokens;  /* most rows a sequence brings; chooses the kernel, no result depends on it */
+    int heads, kv_heads, d, dv, page, window, dtype;
+    float scale, out_scale;
+} zkfp_paged_attention_args;
+int zkfp_paged_attention(const zkfp_paged_attention_args* a, void* stream);
+long long zkfp_paged_scratch(const zkfp_paged_attention_args* a);
+int zkfp_paged_path(const zkfp_paged_attention_args* a);   /* 0 plain CUDA cores, 1 tcgen05 tiles, 2 warp-level products */
+
+/* New keys and values to their pages, keys and (if given) queries turned on the way: element pairs (2i, 2i + 1), or with
+ * half = 1 (i, i + pairs), of the first 2 * pairs elements of a head, by cos_sin[position][i].  Rows at positions that
+ * the table of angles does not hold keep their angles; rows without a place in the pages are not written. */
+typedef struct {
+    const void* q;         /* may be null; [tokens][heads][d] */
+    const void* k;         /* [tokens][kv_heads][d] */
+    const void* v;         /* [tokens][kv_heads][dv] */
+    void* q_out;           /* like q, may be q itself */
+    void* k_pages;         /* [pages][page][kv_heads][d] */
+    void* v_pages;         /* [pages][page][kv_heads][dv] */
+    const float* cos_sin;  /* may be null (nothing turns); [positions][pairs][2] */
+    const int* table;
+    const int* rows;
+    const int* lengths;
+    long long q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head;
+    long long k_page, k_pos, kp_head, v_page, v_pos, vp_head;
+    long long tokens, pages, table_cols, table_ld, batch, positions;
+    int heads, kv_heads, d, dv, page, pairs, half, dtype;
+} zkfp_write_pages_args;
+int zkfp_write_pages(const zkfp_write_pages_args* a, void* stream);
+
+/* Copies the first `bytes` of page source[i] over those of page target[i] in every buffer, all of them at once: no page
+ * may be a target twice, or a source and a target.  source and target are host memory and are read before the call
+ * returns. */
+typedef struct {
+    void* base;
+    long long stride, bytes;   /* both multiples of 16 */
+    long long pages;
+} zkfp_page_buffer;
+int zkfp_copy_pages(const zkfp_page_buffer* buffers, int n_buffers, const int* source, const int* target, long long moves,
+                    void* stream);
+
+/* One token per row of logits, from given random numbers in [0, 1).  With w_v = exp((l_v - max) / temperature) a row keeps
+ *   the top_k largest (0: all; of equal logits the lower indices),
+ *   of those, in falling order, every token with less than top_p of their weight in front of it (1: all),
+ *   of those, the tokens with w_v >= min_p,
+ * but always the largest; the token is the first, by index, up to which the kept weights sum to more than random times their
+ * total.  temperature <= 0 takes the largest logit's first index.  NaN counts as -infinity; a row without any logit
+ * above -infinity gives -1.  Sums are exact to 2^-44 of the largest weight. */
+typedef struct {
+    const void* logits;        /* [rows][ld] */
+    const float* random;       /* [rows] */
+    long long* out;            /* [rows] */
+    const float* temperature;  /* [rows] or null: value_temperature for all; likewise the others */
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    long long ld, rows, vocab;
+    int dtype;
+    float value_temperature;
+    int value_top_k;
+    float value_top_p, value_min_p;
+} zkfp_sample_args;
+int zkfp_sample(const zkfp_sample_args* a, void* stream);
+
 /* which kernel a call takes: 0 plain CUDA cores, 1 tensor cores, 2 weight streaming, 3 weight streaming through
  * warp-level tensor-core products; for tests and reports */
 int zkfp_linear_path(const zkfp_linear_args* a);

@@ -226,3 +226,72 @@ def forward(cfg, W, tokens, layers_out=None, rnd=exact):
         if layers_out is not None:
             layers_out.append(x.copy())
     return rnd(rms_norm(x, W["final.norm"], eps)) @ W["embed"].T
+
+
+# ---- a pool of pages ---------------------------------------------------------------------------------------------
+def gather_pages(pages, table, length):
+    """positions 0 .. length - 1 of a sequence, from pages [pages, page, heads, size]"""
+    page = pages.shape[1]
+    return np.stack([pages[table[j // page], j % page] for j in range(length)]) if length else pages[:0, 0]
+
+
+def paged_attention(q, k_pages, v_pages, table, rows, lengths, scale, window=0, gate=None, out_scale=1.0):
+    """(outputs [tokens, heads, dv], how large what they are made of is: sum of weight times |value|, largest sum |q k| scale)"""
+    heads, group = q.shape[1], q.shape[1] // k_pages.shape[2]
+    out = np.full((q.shape[0], heads, v_pages.shape[3]), np.nan)
+    size, score = np.zeros_like(out), np.zeros(q.shape[:2])
+    for b, length in enumerate(lengths):
+        k, v = gather_pages(k_pages, table[b], length), gather_pages(v_pages, table[b], length)
+        n = rows[b + 1] - rows[b]
+        for t in range(n):
+            i, r = length - n + t, rows[b] + t
+            lo = max(0, i - window + 1) if window else 0
+            for h in range(heads):
+                if i < 0:
+                    out[r, h] = 0
+                    continue
+                kk, vv = k[lo:i + 1, h // group], v[lo:i + 1, h // group]
+                s = kk @ q[r, h] * scale
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                out[r, h], size[r, h] = p @ vv, p @ np.abs(vv)
+                score[r, h] = (np.abs(kk) @ np.abs(q[r, h])).max() * scale
+    if gate is not None:
+        f = out_scale / (1 + np.exp(-gate))
+        out, size = out * f, size * f
+    return out, size, score
+
+
+def turned(x, cos_sin, layout):
+    """one head x turned by cos_sin [pairs, 2]"""
+    y, p = np.array(x, dtype=np.float64), len(cos_sin)
+    for i, (c, s) in enumerate(np.asarray(cos_sin, dtype=np.float64)):
+        a, b = (2 * i, 2 * i + 1) if layout == "pairs" else (i, i + p)
+        y[a], y[b] = x[a] * c - x[b] * s, x[b] * c + x[a] * s
+    return y
+
+
+def kept_tokens(logits, temperature, top_k, top_p, min_p):
+    """(indices that a row keeps, their weights), indices rising"""
+    l = np.where(np.isnan(logits), -np.inf, np.asarray(logits, dtype=np.float64))
+    top = l.max()
+    if top == -np.inf:
+        return np.zeros(0, dtype=int), np.zeros(0)
+    order = np.lexsort((np.arange(len(l)), -l))
+    if not temperature > 0:
+        return order[:1], np.ones(1)
+    w = np.where(l == top, 1.0, 0.0) if top == np.inf else np.exp((l - top) / temperature)
+    order = order[:top_k] if top_k > 0 else order
+    if top_p < 1:
+        front = np.concatenate(([0.0], np.cumsum(w[order])))
+        order = order[(front[:-1] < top_p * front[-1]) | (np.arange(len(order)) == 0)]
+    order = np.sort(order[w[order] >= min(min_p, 1.0)])
+    return order, w[order]
+
+
+def sample(logits, random, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    index, w = kept_tokens(logits, temperature, top_k, top_p, min_p)
+    if not len(index):
+        return -1
+    run = np.cumsum(w)
+    return int(index[min(np.searchsorted(run, random * run[-1], side="right"), len(index) - 1)])

@@ -1,0 +1,287 @@
+"""Attention over pages, heads into pages, copies of pages and sampling against plain float64 loops: sizes and masks where they can
+go wrong, what masked places hold, refusals, and a run of them together."""
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import PKG
+from oracle import float_oracle as fo
+
+pytestmark = pytest.mark.gpu
+DTYPES = ["float32", "bfloat16"]
+HALF = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8}           # a rounding's most, relative
+
+
+@pytest.fixture(scope="module")
+def K(float_libpath):
+    torch.backends.cuda.matmul.allow_tf32 = False
+    return importlib.import_module(PKG + ".float_kernel")
+
+
+def rnd(shape, dtype, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(getattr(torch, dtype)).cuda()
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def np64(t):
+    return t.double().cpu().numpy()
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------
+def pool(dtype, new, lengths, page, heads, kv_heads, d, dv, seed=0, spare=3, fill=float("nan"), pad=0):
+    """a batch over a pool: pages in no order, everything that no sequence holds is `fill`"""
+    g = np.random.default_rng(seed)
+    need = [-(-n // page) for n in lengths]
+    pages = sum(need) + spare
+    order = g.permutation(pages)
+    cols = max(need + [1]) + 1
+    table = np.full((len(lengths), cols), -7, dtype=np.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    width = kv_heads * (d + dv) + pad
+    both = torch.full((pages, page, width), fill, dtype=getattr(torch, dtype), device="cuda")
+    for b, n in enumerate(lengths):
+        for p in range(need[b]):
+            lines = min(page, n - p * page)
+            both[table[b, p], :lines] = rnd((lines, width), dtype, seed + 100 + 37 * b + p)
+    rows = np.concatenate(([0], np.cumsum(new))).astype(np.int32)
+    return dict(k=both[:, :, :kv_heads * d].unflatten(2, (kv_heads, d)),
+                v=both[:, :, kv_heads * d:kv_heads * (d + dv)].unflatten(2, (kv_heads, dv)),
+                table=torch.from_numpy(table).cuda(), rows=torch.from_numpy(rows).cuda(), lengths=i32(*lengths),
+                q=rnd((int(rows[-1]), heads, d), dtype, seed + 1), host=(table, rows, lengths), new=new)
+
+
+def attend(K, s, dtype, scale, window=0, gate=None, out_scale=1.0, behind=2, **kw):
+    q, dv = s["q"], s["v"].shape[3]
+    out = torch.full((q.shape[0] + behind, q.shape[1], dv), 5.0, dtype=q.dtype, device="cuda")
+    qx = torch.cat([q, torch.full((behind,) + q.shape[1:], float("nan"), dtype=q.dtype, device="cuda")])
+    gx = None if gate is None else torch.cat([gate, gate[:1].expand(behind, -1, -1)])
+    K.paged_attention(qx, s["k"], s["v"], s["table"], s["rows"], s["lengths"], out, scale, window=window, gate=gx, out_scale=out_scale, **kw)
+    assert (out[q.shape[0]:] == 5.0).all()              # rows behind the last sequence
+    return out[:q.shape[0]]
+
+
+def limit(dtype, size, score, d, keys):
+    """Half steps that a result can be off by.  A weight: its score's sum of d products in 32 bits, both of score and maximum,
+    the exponential's few ulps, its sum of `keys` weights; the weighted sum as many additions.  In bfloat16 also the weight's own
+    rounding; the result's rounding is added by the caller."""
+    e = 2.0 ** -24 * (2 * (d + 4) * score[..., None] + 3 * keys + 32)
+    return size * (e + (HALF[dtype] if dtype == "bfloat16" else 0.0)) * 1.05
+
+
+def check(K, s, dtype, scale=None, window=0, gate=None, out_scale=1.0, **kw):
+    d = s["q"].shape[2]
+    scale = d ** -0.5 if scale is None else scale
+    got = np64(attend(K, s, dtype, scale, window, gate, out_scale, **kw))
+    K.device_status(sync=True)
+    table, rows, lengths = s["host"]
+    want, size, score = fo.paged_attention(np64(s["q"]), np64(s["k"]), np64(s["v"]), table, rows, lengths, scale, window,
+                                           None if gate is None else np64(gate), out_scale)
+    off = np.abs(got - want) - limit(dtype, size, score, d, max(list(lengths) + [1])) - HALF[dtype] * np.abs(want)
+    if gate is not None:
+        off -= 2.0 ** -22 * np.abs(want)
+    assert np.isfinite(got).all() and (off <= 1e-30).all(), float(off.max())
+    return got
+
+
+SHAPES = [  # new, lengths, page, heads, kv heads, d, dv, window
+    ([1], [1], 8, 1, 1, 8, 8, 0), ([1], [4095], 64, 8, 2, 128, 128, 0), ([1, 1, 1], [17, 600, 64], 16, 8, 2, 64, 64, 0),
+    ([2, 0, 1], [130, 40, 9], 32, 6, 2, 24, 40, 0), ([1, 3], [65, 64], 64, 7, 1, 40, 24, 5), ([16], [16], 16, 4, 4, 128, 128, 0),
+    ([5, 1, 2], [300, 1, 77], 128, 12, 4, 96, 128, 64), ([100], [100], 16, 4, 2, 80, 80, 0), ([129, 1], [400, 33], 8, 3, 3, 16, 16, 33),
+    ([33, 64], [512, 64], 1024, 16, 2, 128, 64, 1), ([70], [1000], 64, 9, 3, 72, 72, 129), ([300], [300], 32, 2, 1, 128, 128, 0),
+    ([1] * 40, list(range(1, 400, 10)), 16, 4, 1, 64, 64, 0), ([3], [50], 16, 2, 2, 256, 200, 0), ([257, 1, 31], [700, 700, 31], 64, 8, 1, 128, 128, 200),
+    ([1, 1], [9000, 3], 256, 16, 1, 128, 128, 0), ([40], [6000], 128, 32, 8, 64, 128, 0)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_attention(K, dtype, shape):
+    new, lengths, page, heads, kv, d, dv, window = shape
+    s = pool(dtype, new, lengths, page, heads, kv, d, dv, pad=8 * (page == 16))
+    check(K, s, dtype, window=window)
+    # sharper scores, a gate, and the bound on the rows of a sequence given
+    check(K, s, dtype, scale=2.0 * d ** -0.5, window=window, gate=rnd((sum(new), heads, dv), dtype, 9), out_scale=0.7, max_tokens=max(new))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,length", [([1], [0]), ([5], [3]), ([40, 2], [7, 0]), ([200], [130])])
+def test_rows_that_see_nothing_are_zero(K, dtype, new, length):
+    s = pool(dtype, new, length, 16, 4, 2, 64, 64, fill=0.0)
+    got = check(K, s, dtype)
+    for b, (n, m) in enumerate(zip(new, length)):
+        assert (got[sum(new[:b]):sum(new[:b]) + max(0, n - m)] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("new,window", [(1, 20), (4, 20), (90, 33), (300, 0)])
+def test_what_masked_places_hold_has_no_part(K, dtype, bad, new, window):
+    """keys and values that are infinite or NaN at a position that some rows see and others do not"""
+    length = 310
+    s = pool(dtype, [new], [length], 16, 4, 2, 64, 64)
+    want = check(K, s, dtype, window=window)
+    at = length - new // 2 - 1 if new > 1 else length - window - 1          # seen by the rows from there on, or by none
+    page, line = s["host"][0][0][at // 16], at % 16
+    for what in ("k", "v"):
+        kept = s[what][page, line].clone()
+        s[what][page, line] = bad
+        got = np64(attend(K, s, dtype, 64 ** -0.5, window))
+        s[what][page, line] = kept
+        i = np.arange(length - new, length)
+        blind = (i < at) | ((i - at >= window) if window else np.zeros(new, bool))
+        assert blind.any() and np.isfinite(got[blind]).all()
+        # the rows that do not see it, within the rounding of either run
+        assert np.abs(got - want)[blind].max() <= 4 * HALF[dtype] * (np.abs(want).max() + 4.0) + (2e-5 if dtype == "float32" else 0)
+        if what == "v" and not blind.all():
+            assert not np.isfinite(got[~blind]).any()
+    K.device_status(sync=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_without_a_finite_maximum(K, dtype):
+    """every visible score -infinity gives NaN, as the formula does; one finite score among them takes all the weight"""
+    s = pool(dtype, [1], [40], 16, 2, 1, 64, 64)
+    s["q"][:] = 1.0
+    s["k"].copy_(torch.full_like(s["k"], -1.0))
+    s["k"][..., 0] = -float("inf")
+    assert torch.isnan(attend(K, s, dtype, 0.125)).all()
+    table = s["host"][0]
+    s["k"][table[0][1], 3] = 0.0
+    out = attend(K, s, dtype, 0.125)
+    assert torch.equal(out, s["v"][table[0][1], 3, 0].expand_as(out))
+
+
+# ---- heads into pages --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["pairs", "half"])
+@pytest.mark.parametrize("new,lengths,page,heads,kv,d,dv,pairs", [
+    ([1], [1], 8, 1, 1, 8, 8, 4), ([1, 1], [30, 7], 16, 5, 1, 64, 64, 16), ([3, 0, 9], [40, 5, 9], 8, 4, 2, 48, 24, 7),
+    ([200], [333], 64, 8, 4, 128, 128, 64), ([2], [9], 32, 3, 3, 256, 8, 40), ([33, 1], [33, 65], 1024, 16, 2, 24, 40, 0)])
+def test_heads_into_pages(K, dtype, layout, new, lengths, page, heads, kv, d, dv, pairs):
+    s = pool(dtype, new, lengths, page, heads, kv, d, dv, fill=3.0, pad=16)
+    n = sum(new)
+    k, v = rnd((n, kv, d), dtype, 5), rnd((n, kv, dv), dtype, 6)
+    angles = torch.outer(torch.arange(max(lengths) - 1).double(), 0.37 ** torch.arange(pairs).double())
+    cos_sin = torch.stack((angles.cos(), angles.sin()), -1).float().cuda()      # one position fewer than the longest holds
+    before, q_out = np64(s["k"]), torch.empty_like(s["q"])
+    beforev = np64(s["v"])
+    K.write_pages(k, v, s["k"], s["v"], s["table"], s["rows"], s["lengths"], q=s["q"], q_out=q_out, cos_sin=cos_sin, layout=layout)
+    K.device_status(sync=True)
+    wk, wv, wq = before, beforev, np64(s["q"])
+    table, rows, _ = s["host"]
+    cs = np64(cos_sin)
+    for b, length in enumerate(lengths):
+        for t in range(new[b]):
+            i, r = length - new[b] + t, rows[b] + t
+            turn = (lambda x: fo.turned(x, cs[i], layout)) if i < len(cs) else (lambda x: x)
+            for g in range(kv):
+                wk[table[b, i // page], i % page, g] = turn(np64(k)[r, g])
+                wv[table[b, i // page], i % page, g] = np64(v)[r, g]
+            for h in range(heads):
+                wq[r, h] = turn(wq[r, h])
+    # two products and their sum in 32 bits, one rounding
+    for got, want, x in ((s["k"], wk, k), (q_out, wq, s["q"])):
+        assert (np.abs(np64(got) - want) <= HALF[dtype] * np.abs(want) + 3 * 2.0 ** -24 * 2 * float(x.abs().max())).all()
+    assert np.array_equal(np64(s["v"]), wv)
+    # in place, and without queries or angles
+    q2 = s["q"].clone()
+    K.write_pages(k, v, s["k"], s["v"], s["table"], s["rows"], s["lengths"], q=q2, q_out=q2, cos_sin=cos_sin, layout=layout)
+    assert torch.equal(q2, q_out)
+    K.write_pages(k, v, s["k"], s["v"], s["table"], s["rows"], s["lengths"])
+    for b, length in enumerate(lengths):
+        if new[b]:
+            i = length - 1
+            assert torch.equal(s["k"][table[b, i // page], i % page], k[rows[b + 1] - 1])
+
+
+# ---- copies ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("layers,pages,page,width,moves,positions", [
+    (1, 2, 8, 8, 1, None), (3, 40, 16, 24, 20, 5), (40, 9, 8, 8, 3, 8), (1, 900, 8, 16, 450, 7), (2, 7, 64, 4104, 3, 63), (2, 5, 16, 8, 2, 0)])
+def test_copies_of_pages(K, layers, pages, page, width, moves, positions):
+    g = np.random.default_rng(pages)
+    # buffers of two formats, the second a part of a larger one
+    bufs = [rnd((pages, page, width), DTYPES[i % 2], i) for i in range(layers - 1)] + [rnd((pages, 2, page, width), "bfloat16", 99)[:, 1]]
+    order = g.permutation(pages).tolist()
+    source, target = order[:moves], order[moves:2 * moves]
+    if moves > 2:
+        source[1] = source[0]                            # a page copied twice
+    want = [b.clone() for b in bufs]
+    n = page if positions is None else positions
+    for w, b in zip(want, bufs):
+        for s, t in zip(source, target):
+            w[t, :n] = b[s, :n]
+    K.copy_pages(bufs, source, target, positions=positions)
+    for w, b in zip(want, bufs):
+        assert torch.equal(w, b)
+
+
+# ---- sampling ----------------------------------------------------------------------------------------------------
+def sample_both(K, logits, u, **kw):
+    got = K.sample(logits, u, **kw).cpu().tolist()
+    l, r = np64(logits), np64(u)
+    at = lambda x, i: float(x[i]) if isinstance(x, torch.Tensor) else x
+    full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+    full.update(kw)
+    full = {k: (v.cpu().to(torch.float64) if isinstance(v, torch.Tensor) else float(np.float32(v)) if k != "top_k" else v) for k, v in full.items()}
+    want = [fo.sample(l[i], r[i], at(full["temperature"], i), int(at(full["top_k"], i)), at(full["top_p"], i), at(full["min_p"], i))
+            for i in range(len(l))]
+    return got, want
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (5, 31), (40, 1000), (7, 32768), (2, 129280), (160, 513), (3, 262144), (300, 40)])
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.0), dict(temperature=0.6, top_k=20), dict(top_p=0.9), dict(min_p=0.05, temperature=1.7),
+                                dict(temperature=0.8, top_k=50, top_p=0.7, min_p=0.02), dict(top_k=1), dict(top_p=0.0), dict(temperature=30.0, top_p=0.5)],
+                         ids=str)
+def test_sampling(K, dtype, rows, vocab, kw):
+    logits = rnd((rows, vocab), dtype, vocab, 2.0)
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(rows)).cuda()
+    got, want = sample_both(K, logits, u, **kw)
+    assert got == want
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sampling_by_row(K, dtype):
+    """settings of their own for every row, rows of a wider tensor, many equal logits"""
+    R, V = 200, 2500
+    logits = rnd((R, V + 24), dtype, 3, 1.5)[:, 8:8 + V]
+    logits[::3] = (logits[::3] * 2).round() / 2
+    g = torch.Generator().manual_seed(1)
+    f = lambda lo, hi: (torch.rand(R, generator=g) * (hi - lo) + lo).cuda()
+    u, t, p, m = f(0, 1), f(0.3, 2.0), f(0.2, 1.1), f(-0.02, 0.1).clamp(min=0)
+    k = torch.randint(0, 60, (R,), generator=g, dtype=torch.int32).cuda()
+    t[5], k[6], p[7], m[8] = 0.0, V, 1.0, 1.0
+    got, want = sample_both(K, logits, u, temperature=t, top_k=k, top_p=p, min_p=m)
+    assert got == want
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=3), dict(top_p=0.5), dict(min_p=0.5), dict(temperature=0.0)], ids=str)
+def test_sampling_of_odd_logits(K, dtype, kw):
+    inf, nan, low = float("inf"), float("nan"), torch.finfo(getattr(torch, dtype)).min
+    rows = [[-inf] * 6, [nan] * 6, [nan, -inf, 1.0, 1.0, -inf, 0.5], [low] * 6, [low, low, 0.0, low, low, low], [inf, 1.0, inf, 2.0, nan, inf],
+            [0.0, -0.0, 0.0, -0.0, 0.0, 0.0], [3e38, -3e38, 0.0, 3e38, 1.0, 2.0], [1.0] * 6]
+    logits = torch.tensor(rows).to(getattr(torch, dtype)).cuda()
+    for x in (0.0, 0.3, 0.5, 0.75, 1.0 - 2.0 ** -24):
+        got, want = sample_both(K, logits, torch.full((len(rows),), x, device="cuda"), **kw)
+        assert got == want and got[:2] == [-1, -1]
+
+
+def test_every_kept_token_is_met_as_often_as_it_is_likely(K):
+    """random numbers over the whole interval: each kept token's stretch of them, to the step of the numbers"""
+    V, R = 37, 4096
+    l = rnd((1, V), "float32", 8, 2.0)
+    u = ((torch.arange(R) + 0.5) / R).cuda()
+    got = K.sample(l.expand(R, V).contiguous(), u, temperature=0.9, top_k=12, top_p=0.95).cpu()
+    index, w = fo.kept_tokens(np64(l)[0], float(np.float32(0.9)), 12, float(np.float32(0.95)), 0.0)
+    share = np.bincount(got, minlength=V) / R
+    assert set(got.tolist()) <= set(index.tolist())
+    assert np.abs(share[index] - w / w.sum()).max() <= 1.0 / R and (np.diff(got.numpy()) >= 0).all()

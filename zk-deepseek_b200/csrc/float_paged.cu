@@ -1,0 +1,294 @@
+// Attention of new tokens over pages: the kernel of CUDA cores (float32, and sizes that the tensor cores do not take) and
+// the one that merges what the CTAs of a cut item leave.  How the work is shared is in float_paged.cuh.
+#include "float_paged.cuh"
+
+namespace zkds {
+
+namespace {
+
+// ---- CUDA cores --------------------------------------------------------------------------------------------------
+// Tiles of 16 rows over blocks of 64 keys, all in shared memory, sums of a row in registers: a thread holds eight columns of
+// up to four rows.
+constexpr int kPlainRows = 16, kPlainKeys = 64, kPlainThreads = 128, kPlainMost = 256;
+
+template <typename T>
+struct PlainShape {
+    int kpitch;
+    size_t smem;
+    PlainShape(const zkfp_paged_attention_args& a)
+    {
+        kpitch = a.d + 16 / (int)sizeof(T);            // rows shifted by one 16-byte piece: no bank conflicts
+        smem = plan_bytes(a.batch) + (size_t)kPlainKeys * (kpitch + a.dv) * sizeof(T) +
+               sizeof(float) * ((size_t)kPlainRows * (a.d + a.dv) + kPlainRows * kPlainKeys + 3 * kPlainRows);
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kPlainThreads)
+paged_plain_kernel(const Paged p, int kpitch)
+{
+    chain_enter();
+    extern __shared__ __align__(16) uint8_t sm[];
+    const zkfp_paged_attention_args& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 31, d = a.d, dv = a.dv, vd = d / 8, vv = dv / 8, batch = (int)a.batch;
+    const Plan plan(sm, batch);
+    T* Ks = (T*)(sm + (((size_t)(batch + 1) * 8 + (size_t)batch * 12 + 15) & ~(size_t)15));
+    T* Vs = Ks + kPlainKeys * kpitch;
+    float* Q = (float*)(Vs + kPlainKeys * dv);
+    float* O = Q + kPlainRows * d;
+    float* P = O + kPlainRows * dv;
+    float* M = P + kPlainRows * kPlainKeys;
+    float *L = M + kPlainRows, *F = L + kPlainRows;
+    make_plan(p, plan);
+    const long long units = plan.before[batch], u1 = range_begin(units, blockIdx.x + 1, p.grid);
+    long long u = range_begin(units, blockIdx.x, p.grid);
+    if (u >= u1) return;
+    Walk w;
+    for (w.locate(p, plan, u); u < u1; w.next(p, plan)) {
+        const int j_end = (int)min((long long)w.count, w.j + (u1 - u));
+        const bool whole = w.j == 0 && j_end == w.count;
+        const int slot = 2 * blockIdx.x + (w.j == 0 ? 1 : 0), row0 = w.t * kPlainRows, rows = min(kPlainRows, w.n * p.group - row0);
+        __syncthreads();
+        for (int i = tid; i < kPlainRows * vd; i += kPlainThreads) {
+            const int r = i / vd, c = (i - r * vd) * 8;
+            float x[8] = {};
+            if (r < rows) {
+                const int t = (row0 + r) / p.group, h = w.kv * p.group + (row0 + r) % p.group;
+                load8((const T*)a.q + (long long)(w.row0 + t) * a.q_tok + h * a.q_head + c, x);
+            }
+            store8(Q + r * d + c, x);
+        }
+        if (tid < kPlainRows) { M[tid] = -INFINITY; L[tid] = 0.f; }
+        float acc[4][8] = {};
+        for (int j = w.j; j < j_end; ++j) {
+            const int k0 = (w.first + j) * kPlainKeys, nk = min(kPlainKeys, w.len - k0);
+            __syncthreads();                           // the block in front is done with keys, values and weights
+            for (int i = tid; i < kPlainKeys * (vd + vv); i += kPlainThreads) {
+                const int r = i / (vd + vv), c = i - r * (vd + vv);
+                const long long page = r < nk ? page_of(p, w.b, k0 + r) : -1;
+                if (r < nk && page < 0) *(volatile int*)p.error_flag = 1;
+                const long long line = (k0 + r) & (a.page - 1);
+                const T* src = c < vd ? (const T*)a.k + page * a.k_page + line * a.k_pos + w.kv * a.k_head + c * 8
+                                      : (const T*)a.v + page * a.v_page + line * a.v_pos + w.kv * a.v_head + (c - vd) * 8;
+                T* dst = c < vd ? Ks + r * kpitch + c * 8 : Vs + r * dv + (c - vd) * 8;
+#pragma unroll
+                for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+                    reinterpret_cast<uint4*>(dst)[q] = page >= 0 ? reinterpret_cast<const uint4*>(src)[q] : make_uint4(0, 0, 0, 0);
+            }
+            __syncthreads();
+            // scores: a thread takes one key and four rows
+            for (int i = tid; i < kPlainKeys * (kPlainRows / 4); i += kPlainThreads) {
+                const int key = i % kPlainKeys, r = i / kPlainKeys * 4;
+                if (r >= rows) continue;
+                float s[4] = {};
+                for (int c = 0; c < d; c += 8) {
+                    float k8[8];
+                    load8(Ks + key * kpitch + c, k8);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float q8[8];
+                        load8(Q + (r + q) * d + c, q8);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s[q] = fmaf(q8[e], k8[e], s[q]);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) P[(r + q) * kPlainKeys + key] = s[q];
+            }
+            __syncthreads();
+            // softmax of the block, a warp per row
+            for (int r = tid >> 5; r < rows; r += kPlainThreads / 32) {
+                const int pos = w.len - w.n + (row0 + r) / p.group;
+                float s[kPlainKeys / 32], m = M[r];
+                const float m_old = m;
+#pragma unroll
+                for (int i = 0; i < kPlainKeys / 32; ++i) {
+                    const int key = k0 + i * 32 + lane;
+                    const bool seen = key <= pos && (a.window <= 0 || pos - key < a.window);
+                    s[i] = seen ? P[r * kPlainKeys + i * 32 + lane] * a.scale : -INFINITY;
+                    m = fmaxf(m, s[i]);
+                }
+                m = warp_max(m);
+                float l = 0.f;
+#pragma unroll
+                for (int i = 0; i < kPlainKeys / 32; ++i) {
+                    const float e = s[i] == -INFINITY ? 0.f : expf(s[i] - m);
+                    P[r * kPlainKeys + i * 32 + lane] = e;
+                    l += e;
+                }
+                l = warp_sum(l);
+                if (lane == 0) {
+                    const float f = m_old == -INFINITY ? 0.f : expf(m_old - m);
+                    M[r] = m;
+                    L[r] = L[r] * f + l;
+                    F[r] = f;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = tid + k * kPlainThreads, r = i / vv, c = (i - r * vv) * 8;
+                if (r >= rows) break;
+                const float f = F[r];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[k][e] *= f;
+#pragma unroll 4
+                for (int key = 0; key < kPlainKeys; ++key) {
+                    float v8[8];
+                    load8(Vs + key * dv + c, v8);
+                    const float e = P[r * kPlainKeys + key];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) acc[k][q] = fmaf(e, v8[q], acc[k][q]);
+                }
+            }
+        }
+        float* to = whole ? O : p.part + (long long)slot * p.tile * dv;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = tid + k * kPlainThreads, r = i / vv, c = (i - r * vv) * 8;
+            if (r < rows) store8(to + r * dv + c, acc[k]);
+        }
+        if (whole) {
+            __syncthreads();
+            for (int r = tid >> 5; r < rows; r += kPlainThreads / 32) {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = lane + 32 * k < dv ? O[r * dv + lane + 32 * k] : 0.f;
+                finish_row<T>(p, w, row0 + r, x, L[r]);
+            }
+        } else if (tid < rows) {
+            p.ml[((long long)slot * p.tile + tid) * 2] = M[tid];
+            p.ml[((long long)slot * p.tile + tid) * 2 + 1] = L[tid];
+        }
+        u += j_end - w.j;
+    }
+}
+
+// ---- cut items ---------------------------------------------------------------------------------------------------
+// CTA x looks at the item that its namesake's range ends in: if that began there and goes on behind it, its parts are merged, a
+// warp per row, gridDim.y warps' rows side by side.  Maxima are in units of log2 where base2.
+template <typename T>
+__global__ void __launch_bounds__(128)
+paged_combine_kernel(const Paged p, int base2)
+{
+    chain_enter();
+    extern __shared__ __align__(16) uint8_t sm[];
+    const Plan plan(sm, (int)p.a.batch);
+    make_plan(p, plan);
+    const int c = blockIdx.x, lane = threadIdx.x & 31, dv = p.a.dv;
+    const long long units = plan.before[p.a.batch], u0 = range_begin(units, c, p.grid), u1 = range_begin(units, c + 1, p.grid);
+    if (u0 >= u1) return;
+    Walk w;
+    w.locate(p, plan, u1 - 1);
+    const long long begin = u1 - 1 - w.j, end = begin + w.count;
+    if (end <= u1 || begin < u0) return;
+    const int row0 = w.t * p.tile, rows = min(p.tile, w.n * p.group - row0);
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += 4 * gridDim.y) {
+        float x[8] = {}, m = -INFINITY, l = 0.f;
+        for (int i = c; i < p.grid; ++i) {
+            if (i > c && range_begin(units, i, p.grid) >= end) break;
+            if (range_begin(units, i, p.grid) >= range_begin(units, i + 1, p.grid)) continue;
+            m = fmaxf(m, p.ml[((2ll * i + (i == c)) * p.tile + r) * 2]);
+        }
+        for (int i = c; i < p.grid; ++i) {
+            if (i > c && range_begin(units, i, p.grid) >= end) break;
+            if (range_begin(units, i, p.grid) >= range_begin(units, i + 1, p.grid)) continue;
+            const long long at = (2ll * i + (i == c)) * p.tile + r;
+            const float mi = p.ml[at * 2], f = mi == -INFINITY ? 0.f : base2 ? exp2f(mi - m) : expf(mi - m);
+            l = fmaf(f, p.ml[at * 2 + 1], l);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (lane + 32 * k < dv) x[k] = fmaf(f, p.part[at * dv + lane + 32 * k], x[k]);
+        }
+        finish_row<T>(p, w, row0 + r, x, l);
+    }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------
+template <typename T>
+int plain_grid(const zkfp_paged_attention_args& a)
+{
+    const size_t smem = PlainShape<T>(a).smem;
+    const int per_sm = (int)(220 * 1024 / smem);
+    return fp_sm_count() * (per_sm < 1 ? 1 : per_sm > 6 ? 6 : per_sm);
+}
+
+template <typename T>
+int launch_combine(const Paged& p, int base2, cudaStream_t st)
+{
+    fp_launch(paged_combine_kernel<T>, dim3((unsigned)p.grid, (unsigned)(p.tile + 15) / 16), dim3(128), plan_bytes(p.a.batch), st, p, base2);
+    return fp_launched();
+}
+
+template <typename T>
+int launch_plain(Paged& p, cudaStream_t st)
+{
+    const PlainShape<T> s(p.a);
+    if (s.smem > (size_t)kSharedMax) return ZKDS_ERR_UNSUPPORTED;
+    ZKDS_CUDA(cudaFuncSetAttribute(paged_plain_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax));
+    fp_launch(paged_plain_kernel<T>, dim3((unsigned)p.grid), dim3(kPlainThreads), s.smem, st, p, s.kpitch);
+    const int rc = fp_launched();
+    return rc != ZKDS_OK ? rc : launch_combine<T>(p, 0, st);
+}
+
+// grid and tile of the kernel that a call takes
+void choose(Paged& p)
+{
+    p.shift = page_shift(p.a.page);
+    p.group = p.a.heads / p.a.kv_heads;
+    p.tile = kPlainRows;
+    p.block = kPlainKeys;
+    p.grid = p.a.dtype == ZKFP_BF16 ? plain_grid<bf16>(p.a) : plain_grid<float>(p.a);
+}
+
+bool paged_ok(const zkfp_paged_attention_args* a)
+{
+    return a && a->q && a->k && a->v && a->out && a->table && a->rows && a->lengths && a->tokens >= 0 && a->pages > 0 && a->table_cols > 0 &&
+           a->table_ld >= a->table_cols && a->batch > 0 && a->max_tokens >= 0 && a->kv_heads > 0 && a->heads > 0 &&
+           a->heads % a->kv_heads == 0 && a->d > 0 && a->dv > 0 && !(a->d & 7) && !(a->dv & 7) && page_shift(a->page) >= 0 && (unsigned)a->dtype <= 1 &&
+           !((a->q_tok | a->q_head | a->k_page | a->k_pos | a->k_head | a->v_page | a->v_pos | a->v_head | a->o_tok | a->o_head | a->gate_tok |
+              a->gate_head) & 7) &&
+           !(((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out | (uintptr_t)a->gate) & 15);
+}
+
+bool paged_takes(const zkfp_paged_attention_args* a)
+{
+    return a->batch <= kPagedBatch && a->d <= kPlainMost && a->dv <= kPlainMost && a->tokens < 0x40000000ll / a->heads && a->pages <= 0x7fffffffll;
+}
+
+}  // namespace
+
+}  // namespace zkds
+
+using namespace zkds;
+
+extern "C" {
+
+int zkfp_paged_path(const zkfp_paged_attention_args* a) { return 0; }
+
+long long zkfp_paged_scratch(const zkfp_paged_attention_args* a)
+{
+    if (!paged_ok(a) || !paged_takes(a)) return 0;
+    Paged p;
+    p.a = *a;
+    choose(p);
+    return 2ll * p.grid * p.tile * (a->dv + 2);
+}
+
+int zkfp_paged_attention(const zkfp_paged_attention_args* a, void* stream)
+{
+    if (!paged_ok(a)) return ZKDS_ERR_ARG;
+    if (!paged_takes(a)) return ZKDS_ERR_UNSUPPORTED;
+    if (a->tokens == 0) return ZKDS_OK;
+    if (!a->scratch) return ZKDS_ERR_ARG;
+    Paged p;
+    p.a = *a;
+    choose(p);
+    p.part = a->scratch;
+    p.ml = a->scratch + 2ll * p.grid * p.tile * a->dv;
+    p.error_flag = fp_error_flag();
+    if (!p.error_flag) return ZKDS_ERR_WORKSPACE;
+    return a->dtype == ZKFP_BF16 ? launch_plain<bf16>(p, (cudaStream_t)stream) : launch_plain<float>(p, (cudaStream_t)stream);
+}
+
+}  // extern "C"

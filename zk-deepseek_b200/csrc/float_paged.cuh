@@ -1,0 +1,293 @@
+// What the kernels of a pool of pages share: page arithmetic and the place of a row in its batch.
+#pragma once
+#include "float_common.cuh"
+
+namespace zkds {
+
+// log2 of a page size; -1 where it is none (a power of two from 8 to 1024)
+inline int page_shift(int page)
+{
+    for (int s = 3; s <= 10; ++s)
+        if (page == 1 << s) return s;
+    return -1;
+}
+
+// the sequence that row r belongs to, the same in every thread of the block, or -1 (all threads call it)
+__device__ __forceinline__ int sequence_of_row(const int* rows, int batch, long long r)
+{
+    int b = 0;
+    for (int base = 0; base < batch; base += blockDim.x) {
+        const int i = base + (int)threadIdx.x;
+        b += __syncthreads_count(i < batch && rows[i + 1] <= r);
+    }
+    return b < batch && rows[b] >= 0 && rows[b] <= r ? b : -1;
+}
+
+// ---- attention over pages: how the work is shared ----------------------------------------------------------------
+// An item is a tile of query rows (token, head of a group, in this order) of one sequence and one key head; it takes a
+// number of units, blocks of keys from the first that any of its rows sees to the last.  All units in the order
+// sequence, key head, tile, block are cut into equal ranges, one per CTA, so that one long sequence among short ones,
+// a prompt among decoding sequences or a single sequence all keep every SM busy, and neither grid nor scratch depends on
+// lengths that only the device knows.  An item that one CTA takes whole goes straight to `out`; of one that is cut, every CTA
+// leaves its sums, and paged_combine_kernel merges them in the order of the keys.  Results depend on lengths alone, not on timing.
+constexpr int kPagedBatch = 1024;
+
+struct Paged {
+    zkfp_paged_attention_args a;
+    int shift, group, tile, block, grid;
+    float* part;                     // [2 * grid][tile][dv] weighted sums; first the item that began in front of a CTA's
+    float* ml;                       // [2 * grid][tile][2] maximum, sum        range, then the one that ends behind it
+    int* error_flag;
+};
+
+// in dynamic shared memory: (batch + 1) units in front of each sequence, then its first row, rows and positions
+struct Plan {
+    long long* before;
+    int *row0, *n, *len;
+    __device__ __forceinline__ Plan(uint8_t* at, int batch)
+    {
+        before = (long long*)at;
+        row0 = (int*)(before + batch + 1);
+        n = row0 + batch;
+        len = n + batch;
+    }
+};
+inline size_t plan_bytes(long long batch) { return ((size_t)(batch + 1) * 8 + (size_t)batch * 12 + 15) & ~(size_t)15; }
+
+// blocks of keys that tile t of a sequence with n rows and len positions visits: first .. first + count - 1, one at least
+__device__ __forceinline__ void tile_blocks(const Paged& p, int n, int len, int t, int& first, int& count)
+{
+    const int last_row = min((t + 1) * p.tile, n * p.group) - 1;
+    const int i0 = len - n + t * p.tile / p.group, i1 = len - n + last_row / p.group;
+    if (i1 < 0) { first = 0; count = 1; return; }
+    const int lo = p.a.window > 0 ? max(i0 - p.a.window + 1, 0) : 0;
+    first = lo / p.block;
+    count = i1 / p.block - first + 1;
+}
+
+__device__ __forceinline__ int tiles_of(const Paged& p, int n) { return (n * p.group + p.tile - 1) / p.tile; }
+
+__device__ __forceinline__ long long warp_sum64(long long v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// every thread of the block takes part; ends with a barrier
+__device__ __forceinline__ void make_plan(const Paged& p, const Plan& s)
+{
+    const int batch = (int)p.a.batch, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const long long capacity = min(p.a.table_cols << p.shift, 0x7fffffffll);
+    for (int base = warp * 32; base < batch; base += warps * 32) {
+        const int b = base + lane;
+        int n = 0, len = 0, row0 = 0;
+        if (b < batch) {
+            row0 = p.a.rows[b];
+            const int row1 = p.a.rows[b + 1];
+            len = p.a.lengths[b];
+            n = row1 - row0;
+            bool bad = len < 0 || len > capacity;
+            len = len < 0 ? 0 : len > capacity ? (int)capacity : len;
+            if (row0 < 0 || row1 < row0 || row1 > p.a.tokens) { n = 0; bad = true; }
+            if (bad) *(volatile int*)p.error_flag = 1;
+        }
+        const int tiles = tiles_of(p, n);
+        long long units = 0;
+        if (tiles <= 8)
+            for (int t = 0; t < tiles; ++t) {
+                int first, count;
+                tile_blocks(p, n, len, t, first, count);
+                units += count;
+            }
+        for (unsigned left = __ballot_sync(0xffffffffu, tiles > 8); left; left &= left - 1) {
+            const int who = __ffs(left) - 1, nn = __shfl_sync(0xffffffffu, n, who), ll = __shfl_sync(0xffffffffu, len, who);
+            long long sum = 0;
+            for (int t = lane; t < tiles_of(p, nn); t += 32) {
+                int first, count;
+                tile_blocks(p, nn, ll, t, first, count);
+                sum += count;
+            }
+            sum = warp_sum64(sum);
+            if (lane == who) units = sum;
+        }
+        if (b < batch) {
+            s.row0[b] = row0;
+            s.n[b] = n;
+            s.len[b] = len;
+            s.before[b + 1] = units * p.a.kv_heads;
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        long long total = 0;
+        for (int base = 0; base < batch; base += 32) {
+            const int b = base + lane;
+            long long v = b < batch ? s.before[b + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long w = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += w;
+            }
+            if (b < batch) s.before[b + 1] = total + v;
+            total += __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (lane == 0) s.before[0] = 0;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ long long range_begin(long long units, int cta, int grid) { return units * cta / grid; }
+
+// one item and the part of it that starts at unit u; whole warps walk, every warp by itself
+struct Walk {
+    int b, kv, t, tiles;             // sequence, key head, tile
+    int first, count, j;             // blocks of the item, and the one that u is
+    int row0, n, len;
+
+    __device__ __forceinline__ void item(const Paged& p) { tile_blocks(p, n, len, t, first, count); }
+    __device__ __forceinline__ void sequence(const Paged& p, const Plan& s)
+    {
+        row0 = s.row0[b]; n = s.n[b]; len = s.len[b];
+        tiles = tiles_of(p, n);
+    }
+    __device__ __forceinline__ void locate(const Paged& p, const Plan& s, long long u)
+    {
+        int lo = 0, hi = (int)p.a.batch;               // before[lo] <= u < before[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s.before[mid] <= u) lo = mid;
+            else hi = mid;
+        }
+        b = lo;
+        sequence(p, s);
+        const long long per = (s.before[b + 1] - s.before[b]) / p.a.kv_heads;
+        long long rest = u - s.before[b];
+        kv = (int)(rest / per);
+        rest -= kv * per;
+        const int lane = threadIdx.x & 31;
+        for (int t0 = 0;; t0 += 32) {                  // ends: rest < per, the sum of all tiles
+            int f = 0, c = 0;
+            if (t0 + lane < tiles) tile_blocks(p, n, len, t0 + lane, f, c);
+            int sum = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int w = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += w;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, sum > rest);
+            if (past || t0 + 32 >= tiles) {
+                const int who = past ? __ffs(past) - 1 : 31;
+                t = t0 + who;
+                j = (int)rest - __shfl_sync(0xffffffffu, sum - c, who);
+                first = __shfl_sync(0xffffffffu, f, who);
+                count = __shfl_sync(0xffffffffu, c, who);
+                return;
+            }
+            rest -= __shfl_sync(0xffffffffu, sum, 31);
+        }
+    }
+    __device__ __forceinline__ void next(const Paged& p, const Plan& s)
+    {
+        j = 0;
+        if (++t == tiles) {
+            t = 0;
+            if (++kv == p.a.kv_heads) {
+                kv = 0;
+                do ++b;
+                while (b < p.a.batch && s.before[b + 1] == s.before[b]);
+                if (b == p.a.batch) return;
+                sequence(p, s);
+            }
+        }
+        item(p);
+    }
+};
+
+// page of position j, or -1
+__device__ __forceinline__ long long page_of(const Paged& p, int b, int j)
+{
+    const long long page = p.a.table[b * p.a.table_ld + (j >> p.shift)];
+    return page >= 0 && page < p.a.pages ? page : -1;
+}
+
+// ---- a row by itself ---------------------------------------------------------------------------------------------
+// The tiles multiply weights of zero with whatever values stand at positions that a row does not see.  Where that
+// is an infinity or a NaN (another row's, or what an earlier owner left in a page), the row's sums are not finite, and the row is
+// taken once more from the definition, visible positions alone.  A warp takes 32 keys at a time, a lane one key, then a lane every
+// 32nd column.  o[k]: column lane + 32 k.
+template <typename T>
+__device__ __noinline__ void attend_row(const Paged& p, int b, int kv, int token, int head, int pos, float (&o)[8])
+{
+    const int lane = threadIdx.x & 31;
+    const T* q = (const T*)p.a.q + (long long)token * p.a.q_tok + head * p.a.q_head;
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = 0.f;
+    for (int j0 = p.a.window > 0 ? max(pos - p.a.window + 1, 0) : 0; j0 <= pos; j0 += 32) {
+        const int j = j0 + lane;
+        const long long page = j <= pos ? page_of(p, b, j) : -1;
+        float s = 0.f;
+        if (page >= 0) {
+            const T* key = (const T*)p.a.k + page * p.a.k_page + (j & (p.a.page - 1)) * p.a.k_pos + kv * p.a.k_head;
+            for (int c = 0; c < p.a.d; c += 8) {
+                float x[8], y[8];
+                load8(q + c, x);
+                load8(key + c, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
+            }
+            s *= p.a.scale;
+        }
+        const float m_new = fmaxf(m, warp_max(page >= 0 ? s : -INFINITY));
+        const float f = m == m_new ? 1.f : expf(m - m_new);
+        const float e = page < 0 || (s == -INFINITY && m_new == -INFINITY) ? 0.f : expf(s - m_new);
+        l = l * f + warp_sum(e);
+        m = m_new;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] *= f;
+        for (int i = 0; i < 32 && j0 + i <= pos; ++i) {
+            const float w = __shfl_sync(0xffffffffu, e, i);
+            const long long at = __shfl_sync(0xffffffffu, page, i);
+            if (at < 0) continue;
+            const T* value = (const T*)p.a.v + at * p.a.v_page + ((j0 + i) & (p.a.page - 1)) * p.a.v_pos + kv * p.a.v_head;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (lane + 32 * k < p.a.dv) o[k] = fmaf(w, to_f32(value[lane + 32 * k]), o[k]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] /= l;
+}
+
+// A warp finishes a row: x[k] is the weighted sum of column lane + 32 k, l the sum of the weights.
+template <typename T>
+__device__ __forceinline__ void finish_row(const Paged& p, const Walk& w, int row, float (&x)[8], float l)
+{
+    const int lane = threadIdx.x & 31, in_seq = row / p.group, head = w.kv * p.group + row - in_seq * p.group;
+    const int token = w.row0 + in_seq, pos = w.len - w.n + in_seq;
+    if (pos < 0) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = 0.f;
+    } else {
+        bool finite = true;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (lane + 32 * k < p.a.dv) x[k] /= l;
+            else x[k] = 0.f;
+            finite = finite && isfinite(x[k]);
+        }
+        if (!__all_sync(0xffffffffu, finite)) attend_row<T>(p, w.b, w.kv, token, head, pos, x);
+    }
+    T* out = (T*)p.a.out + (long long)token * p.a.o_tok + head * p.a.o_head;
+    const T* gate = p.a.gate ? (const T*)p.a.gate + (long long)token * p.a.gate_tok + head * p.a.gate_head : nullptr;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int c = lane + 32 * k;
+        if (c >= p.a.dv) continue;
+        if (gate) x[k] *= sigmoid_f(to_f32(gate[c])) * p.a.out_scale;
+        out[c] = from_f32<T>(x[k]);
+    }
+}
+
+}  // namespace zkds

@@ -88,6 +88,33 @@ class GatedNormArgs(ctypes.Structure):
                 ("heads", _i), ("vdim", _i), ("p", _i), ("part", _i), ("dtype", _i), ("scale", _f), ("eps", _d)]
 
 
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("gate", _vp), ("table", _vp), ("rows", _vp), ("lengths", _vp),
+                ("scratch", _vp), ("q_tok", _ll), ("q_head", _ll), ("k_page", _ll), ("k_pos", _ll), ("k_head", _ll), ("v_page", _ll),
+                ("v_pos", _ll), ("v_head", _ll), ("o_tok", _ll), ("o_head", _ll), ("gate_tok", _ll), ("gate_head", _ll), ("tokens", _ll),
+                ("pages", _ll), ("table_cols", _ll), ("table_ld", _ll), ("batch", _ll), ("max_tokens", _ll), ("heads", _i),
+                ("kv_heads", _i), ("d", _i), ("dv", _i), ("page", _i), ("window", _i), ("dtype", _i), ("scale", _f), ("out_scale", _f)]
+
+
+class WritePagesArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_out", _vp), ("k_pages", _vp), ("v_pages", _vp), ("cos_sin", _vp),
+                ("table", _vp), ("rows", _vp), ("lengths", _vp), ("q_tok", _ll), ("q_head", _ll), ("k_tok", _ll), ("k_head", _ll),
+                ("v_tok", _ll), ("v_head", _ll), ("qo_tok", _ll), ("qo_head", _ll), ("k_page", _ll), ("k_pos", _ll), ("kp_head", _ll),
+                ("v_page", _ll), ("v_pos", _ll), ("vp_head", _ll), ("tokens", _ll), ("pages", _ll), ("table_cols", _ll),
+                ("table_ld", _ll), ("batch", _ll), ("positions", _ll), ("heads", _i), ("kv_heads", _i), ("d", _i), ("dv", _i),
+                ("page", _i), ("pairs", _i), ("half", _i), ("dtype", _i)]
+
+
+class PageBuffer(ctypes.Structure):
+    _fields_ = [("base", _vp), ("stride", _ll), ("bytes", _ll), ("pages", _ll)]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("logits", _vp), ("random", _vp), ("out", _vp), ("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp),
+                ("ld", _ll), ("rows", _ll), ("vocab", _ll), ("dtype", _i), ("value_temperature", _f), ("value_top_k", _i),
+                ("value_top_p", _f), ("value_min_p", _f)]
+
+
 def _sig(name, argtypes, restype=_i):
     fn = getattr(lib, name)
     fn.argtypes, fn.restype = argtypes, restype
@@ -109,6 +136,12 @@ _scan = _sig("zkfp_scan", [ctypes.POINTER(ScanArgs), _vp])
 _scan_scratch = _sig("zkfp_scan_scratch", [ctypes.POINTER(ScanArgs)], _ll)
 scan_path = _sig("zkfp_scan_path", [ctypes.POINTER(ScanArgs)])
 _gated_norm = _sig("zkfp_gated_norm", [ctypes.POINTER(GatedNormArgs), _vp])
+_paged = _sig("zkfp_paged_attention", [ctypes.POINTER(PagedAttentionArgs), _vp])
+_paged_scratch = _sig("zkfp_paged_scratch", [ctypes.POINTER(PagedAttentionArgs)], _ll)
+paged_path = _sig("zkfp_paged_path", [ctypes.POINTER(PagedAttentionArgs)])
+_write_pages = _sig("zkfp_write_pages", [ctypes.POINTER(WritePagesArgs), _vp])
+_copy_pages = _sig("zkfp_copy_pages", [ctypes.POINTER(PageBuffer), _i, ctypes.POINTER(_i), ctypes.POINTER(_i), _ll, _vp])
+_sample = _sig("zkfp_sample", [ctypes.POINTER(SampleArgs), _vp])
 _embed = _sig("zkfp_embed", [_vp, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _f, _i, _vp])
 _add_norm = _sig("zkfp_add_norm", [_vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _ll, _d, _i, _vp])
 _norm_rows = _sig("zkfp_norm_rows", [_vp, _ll, _vp, _vp, _vp, _ll, _ll, _ll, _d, _i, _vp])
@@ -277,3 +310,207 @@ def scan(args, device, *tensors):
 
 def gated_norm(args, *tensors):
     _call(_gated_norm, (ctypes.byref(args),), "gated_norm", *tensors)
+
+
+# ---- a pool of pages ---------------------------------------------------------------------------------------------
+# Shared by the calls below: k_pages and v_pages [pages, page, kv_heads, size] (views with contiguous heads, the page size a
+# power of two from 8 to 1024), table [batch, columns] int32 (page numbers), rows [batch + 1] int32 (sequence b owns the
+# rows rows[b] .. rows[b + 1] - 1 of the batch), lengths [batch] int32 (positions that a sequence holds, its new rows
+# among them).  The device checks what they hold; `device_status` raises for what did not fit.
+
+def _refuse(what, why):
+    raise ValueError("%s: %s" % (what, why))
+
+
+def _tensor(what, name, t, dtype, dims, device=None, shape=None):
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        _refuse(what, "%s is no tensor of %d dimensions" % (name, dims))
+    if t.dtype != dtype:
+        _refuse(what, "%s is %s, not %s" % (name, t.dtype, dtype))
+    if t.device.type != "cuda":
+        _refuse(what, "%s is on %s" % (name, t.device))
+    device = torch.cuda.current_device() if device is None else device
+    if t.device.index != device:
+        _refuse(what, "%s is on %s, the call goes to cuda:%d" % (name, t.device, device))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        _refuse(what, "%s is %s, not %s" % (name, list(t.shape), list(shape)))
+    return t
+
+
+def _heads(what, name, t, dtype, device, shape):
+    """a tensor of heads: the elements of a head adjacent, everything on 16-byte pieces"""
+    _tensor(what, name, t, dtype, len(shape), device, shape)
+    strides = t.stride()
+    if (t.shape[-1] > 1 and strides[-1] != 1) or any(s & 7 and n > 1 for s, n in zip(strides[:-1], t.shape)) or t.data_ptr() & 15:
+        _refuse(what, "%s has strides %s: heads must be contiguous, all else multiples of 8 elements" % (name, list(strides)))
+    # a dimension of one element has no stride of its own
+    return [s if n > 1 else 0 for s, n in zip(strides[:-1], t.shape)]
+
+
+def _pool(what, k, v, table, rows, lengths):
+    dev = k.device.index if isinstance(k, torch.Tensor) else None
+    if not isinstance(k, torch.Tensor) or k.dtype not in (torch.float32, torch.bfloat16):
+        _refuse(what, "pages hold float32 or bfloat16")
+    _tensor(what, "k_pages", k, k.dtype, 4)
+    _tensor(what, "v_pages", v, k.dtype, 4, dev)
+    ks, vs = _heads(what, "k_pages", k, k.dtype, dev, k.shape), _heads(what, "v_pages", v, k.dtype, dev, tuple(k.shape[:3]) + (v.shape[3],))
+    if k.shape[1] not in (8, 16, 32, 64, 128, 256, 512, 1024):
+        _refuse(what, "pages of %d positions" % k.shape[1])
+    _tensor(what, "table", table, torch.int32, 2, dev)
+    batch = table.shape[0]
+    _tensor(what, "rows", rows, torch.int32, 1, dev, (batch + 1,))
+    _tensor(what, "lengths", lengths, torch.int32, 1, dev, (batch,))
+    if not batch or not table.shape[1] or not k.shape[0]:
+        _refuse(what, "no sequences, no pages or no columns")
+    if (table.shape[1] > 1 and table.stride(1) != 1) or rows.stride(0) != 1 or (batch > 1 and lengths.stride(0) != 1):
+        _refuse(what, "table, rows and lengths must be contiguous along their last dimension")
+    ld = table.stride(0) if batch > 1 else table.shape[1]
+    if ld < table.shape[1]:
+        _refuse(what, "rows of the table overlap")
+    return dev, ks, vs, ld
+
+
+def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, window=0, max_tokens=None, gate=None, out_scale=1.0):
+    """Softmax attention of new tokens over pages.
+
+    q [tokens, heads, d], out [tokens, heads, dv] (strided views): the rows of every sequence behind one another, a row sees
+    the positions up to its own, with window > 0 the last `window` of them.  A row at a negative position (a sequence
+    with more rows than positions) sees none and gives zeros; rows behind the last sequence are left as they were.
+    max_tokens: most rows that a sequence brings (default: all), which chooses the kernel.  gate [tokens, heads, dv]: out is
+    multiplied by sigmoid(gate) * out_scale."""
+    what = "paged_attention"
+    dev, ks, vs, ld = _pool(what, k_pages, v_pages, table, rows, lengths)
+    dt = k_pages.dtype
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        _refuse(what, "q is no tensor of 3 dimensions")
+    tokens, heads, d = q.shape
+    kv, dv = k_pages.shape[2], v_pages.shape[3]
+    if not kv or not heads or heads % kv or d != k_pages.shape[3]:
+        _refuse(what, "%d query heads of %d over %d key heads of %d" % (heads, d, kv, k_pages.shape[3]))
+    if d & 7 or dv & 7 or not d or not dv:
+        _refuse(what, "head sizes %d and %d are no multiples of 8" % (d, dv))
+    qs, os = _heads(what, "q", q, dt, dev, (tokens, heads, d)), _heads(what, "out", out, dt, dev, (tokens, heads, dv))
+    gs = _heads(what, "gate", gate, dt, dev, (tokens, heads, dv)) if gate is not None else (0, 0)
+    if window < 0 or (max_tokens is not None and max_tokens < 0):
+        _refuse(what, "a negative window or bound")
+    a = PagedAttentionArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ptr(gate), table.data_ptr(),
+                           rows.data_ptr(), lengths.data_ptr(), None, *qs, *ks, *vs, *os, *gs, tokens, k_pages.shape[0], table.shape[1],
+                           ld, table.shape[0], tokens if max_tokens is None else max_tokens, heads, kv, d, dv, k_pages.shape[1],
+                           min(window, 0x7fffffff), code(dt), scale, out_scale)
+    if tokens:
+        _with_scratch(_paged, _paged_scratch, a, what, q.device, (q, k_pages, v_pages, table, rows, lengths, out, gate))
+    return out
+
+
+def write_pages(k, v, k_pages, v_pages, table, rows, lengths, q=None, q_out=None, cos_sin=None, layout="pairs"):
+    """New keys and values k, v [tokens, kv_heads, size] to their places in the pages; keys, and queries q [tokens, heads, size]
+    on their way to q_out (which may be q), turned by the angles of their positions.
+
+    cos_sin [positions, pairs, 2] float32 (`float_model.rotary_table`): the first 2 * pairs elements of a head turn, (2i, 2i + 1)
+    with layout "pairs", (i, i + pairs) with "half"; None: nothing does.  A row at a position without angles keeps its own, a row
+    without a place in the pages is not written."""
+    what = "write_pages"
+    dev, ks, vs, ld = _pool(what, k_pages, v_pages, table, rows, lengths)
+    dt, (kv, d), dv = k_pages.dtype, k_pages.shape[2:], v_pages.shape[3]
+    if not isinstance(k, torch.Tensor) or k.dim() != 3 or layout not in ("pairs", "half") or (q is None) != (q_out is None):
+        _refuse(what, "k has three dimensions, layout is 'pairs' or 'half', q and q_out come together")
+    tokens = k.shape[0]
+    if d & 7 or dv & 7 or not d or not dv:
+        _refuse(what, "head sizes %d and %d are no multiples of 8" % (d, dv))
+    kt, vt = _heads(what, "k", k, dt, dev, (tokens, kv, d)), _heads(what, "v", v, dt, dev, (tokens, kv, dv))
+    heads, qs, os = 0, (0, 0), (0, 0)
+    if q is not None:
+        if not isinstance(q, torch.Tensor) or q.dim() != 3 or not q.shape[1]:
+            _refuse(what, "q is no tensor of 3 dimensions")
+        heads = q.shape[1]
+        qs, os = _heads(what, "q", q, dt, dev, (tokens, heads, d)), _heads(what, "q_out", q_out, dt, dev, (tokens, heads, d))
+    positions = pairs = 0
+    if cos_sin is not None:
+        _tensor(what, "cos_sin", cos_sin, torch.float32, 3, dev)
+        positions, pairs = cos_sin.shape[:2]
+        if cos_sin.shape[2] != 2 or not cos_sin.is_contiguous() or 2 * pairs > d:
+            _refuse(what, "cos_sin %s is no contiguous [positions, pairs, 2] for heads of %d" % (list(cos_sin.shape), d))
+    a = WritePagesArgs(ptr(q), k.data_ptr(), v.data_ptr(), ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(), ptr(cos_sin), table.data_ptr(),
+                       rows.data_ptr(), lengths.data_ptr(), *qs, *kt, *vt, *os, *ks, *vs, tokens, k_pages.shape[0], table.shape[1], ld,
+                       table.shape[0], positions, heads, kv, d, dv, k_pages.shape[1], pairs, int(layout == "half"), code(dt))
+    if tokens:
+        _call(_write_pages, (ctypes.byref(a),), what, q, k, v, q_out, k_pages, v_pages, cos_sin, table, rows, lengths)
+
+
+def copy_pages(buffers, source, target, positions=None):
+    """Copies page source[i] over page target[i] in every buffer [pages, page, ...], or the first `positions` positions of it.  All
+    copies happen at once: no page may be a target twice, or both a source and a target.  source and target: page numbers on the
+    host."""
+    what = "copy_pages"
+    if len(source) != len(target):
+        _refuse(what, "%d sources, %d targets" % (len(source), len(target)))
+    if not buffers or not len(source):
+        return
+    dev = None
+    list_ = (PageBuffer * len(buffers))()
+    for p, t in zip(list_, buffers):
+        if not isinstance(t, torch.Tensor) or t.dim() < 2 or t.device.type != "cuda":
+            _refuse(what, "a buffer is no [pages, page, ...] tensor on a GPU")
+        dev = torch.cuda.current_device() if dev is None else dev
+        if t.device.index != dev:
+            _refuse(what, "a buffer is on %s, the call goes to cuda:%d" % (t.device, dev))
+        if t.numel() and not t[0].is_contiguous():
+            _refuse(what, "pages are not contiguous: strides %s" % (list(t.stride()),))
+        n = t.shape[1] if positions is None else positions
+        if not 0 <= n <= t.shape[1]:
+            _refuse(what, "%d positions of pages of %d" % (n, t.shape[1]))
+        size = t.element_size()
+        page = t[0].numel() * size if t.shape[0] else 0
+        p.base, p.pages, p.bytes = t.data_ptr(), t.shape[0], page // t.shape[1] * n if t.shape[1] else 0
+        p.stride = t.stride(0) * size if t.shape[0] > 1 else page
+        if (p.base | p.stride | p.bytes) & 15:
+            _refuse(what, "pages, or the part of them that is copied, do not lie on 16-byte pieces")
+    n = len(source)
+    src, dst = (_i * n)(*source), (_i * n)(*target)
+    _call(_copy_pages, (list_, len(buffers), src, dst, n), what, *buffers)
+
+
+def sample(logits, random, out=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token per row of logits [rows, vocab] from random [rows] float32 in [0, 1): out [rows] int64.
+
+    A row keeps its top_k largest logits (0: all), of those the likeliest tokens until top_p of their weight lies in front
+    (1: all), of those the tokens at least min_p as likely as the likeliest; of equal logits the lower indices.  Kept tokens lie in
+    the order of their indices on [0, 1), as wide as they are likely, and random names the one.  temperature 0 takes the first of
+    the largest.  Each of the four is a number or a tensor [rows] (float32; top_k int32).  A row of nothing but -infinity and
+    NaN gives -1."""
+    what = "sample"
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16):
+        _refuse(what, "logits are float32 or bfloat16")
+    _tensor(what, "logits", logits, logits.dtype, 2)
+    rows, vocab = logits.shape
+    dev = logits.device.index
+    if not vocab or (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        _refuse(what, "logits %s with strides %s" % (list(logits.shape), list(logits.stride())))
+
+    def per_row(name, t, dtype):
+        _tensor(what, name, t, dtype, 1, dev, (rows,))
+        if rows > 1 and t.stride(0) != 1:
+            _refuse(what, "%s is not contiguous" % name)
+        return t.data_ptr()
+
+    out = torch.empty(rows, dtype=torch.int64, device=logits.device) if out is None else out
+    pointers, values, held = [], [], []
+    for name, x, dtype, least in (("temperature", temperature, torch.float32, 0), ("top_k", top_k, torch.int32, 0), ("top_p", top_p, torch.float32, 0),
+                                  ("min_p", min_p, torch.float32, 0)):
+        if isinstance(x, torch.Tensor):
+            pointers.append(per_row(name, x, dtype))
+            held.append(x)
+            x = 0
+        else:
+            pointers.append(None)
+            if not x >= least:
+                _refuse(what, "%s is %r" % (name, x))
+        values.append(x)
+    if values[1] != int(values[1]):
+        _refuse(what, "top_k is %r" % (top_k,))
+    a = SampleArgs(logits.data_ptr(), per_row("random", random, torch.float32), per_row("out", out, torch.int64), *pointers,
+                   logits.stride(0) if rows > 1 else vocab, rows, vocab, code(logits.dtype), values[0], min(int(values[1]), 0x7fffffff), values[2],
+                   values[3])
+    if rows:
+        _call(_sample, (ctypes.byref(a),), what, logits, random, out, *held)
+    return out
