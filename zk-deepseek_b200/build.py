@@ -26,7 +26,7 @@ LIBRARIES = {
     "libint64gemm.so": (["capi.cu", "fixedpoint.cu", "gemm_exact.cu", "limb_gemm.cu", "converters.cu"],
                         ["common.cuh", "kernels.h", "range_answer.h", "tcgen05.cuh", "zkds_int64.h"]),
     "libfloatops.so": (["float_capi.cu", "float_ops.cu", "float_gemm.cu", "float_gemm_f32.cu", "float_gemm_tc.cu", "float_attention.cu",
-                        "float_grouped.cu", "float_paged.cu", "float_pages.cu", "float_recurrent.cu", "float_sample.cu", "float_scan_tc.cu"],
+                        "float_grouped.cu", "float_paged.cu", "float_paged_tc.cu", "float_pages.cu", "float_recurrent.cu", "float_sample.cu", "float_scan_tc.cu"],
                        ["common.cuh", "float_common.cuh", "float_paged.cuh", "tcgen05.cuh", "zkds_float.h"]),
 }
 INT_LIBRARY, FLOAT_LIBRARY = "libint64gemm.so", "libfloatops.so"

@@ -25,7 +25,7 @@ struct PlainShape {
 
 template <typename T>
 __global__ void __launch_bounds__(kPlainThreads)
-paged_plain_kernel(const Paged p, int kpitch)
+paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
 {
     chain_enter();
     extern __shared__ __align__(16) uint8_t sm[];
@@ -169,7 +169,7 @@ paged_plain_kernel(const Paged p, int kpitch)
 // warp per row, gridDim.y warps' rows side by side.  Maxima are in units of log2 where base2.
 template <typename T>
 __global__ void __launch_bounds__(128)
-paged_combine_kernel(const Paged p, int base2)
+paged_combine_kernel(const __grid_constant__ Paged p, int base2)
 {
     chain_enter();
     extern __shared__ __align__(16) uint8_t sm[];
@@ -194,7 +194,9 @@ paged_combine_kernel(const Paged p, int base2)
             if (i > c && range_begin(units, i, p.grid) >= end) break;
             if (range_begin(units, i, p.grid) >= range_begin(units, i + 1, p.grid)) continue;
             const long long at = (2ll * i + (i == c)) * p.tile + r;
-            const float mi = p.ml[at * 2], f = mi == -INFINITY ? 0.f : base2 ? exp2f(mi - m) : expf(mi - m);
+            const float mi = p.ml[at * 2];
+            if (mi == -INFINITY) continue;             // no key that the row sees
+            const float f = base2 ? exp2f(mi - m) : expf(mi - m);
             l = fmaf(f, p.ml[at * 2 + 1], l);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
@@ -236,6 +238,9 @@ void choose(Paged& p)
 {
     p.shift = page_shift(p.a.page);
     p.group = p.a.heads / p.a.kv_heads;
+    const int path = zkfp_paged_path(&p.a);
+    if (path == 2) return paged_stream_shape(p);
+    if (path == 1) return paged_tile_shape(p);
     p.tile = kPlainRows;
     p.block = kPlainKeys;
     p.grid = p.a.dtype == ZKFP_BF16 ? plain_grid<bf16>(p.a) : plain_grid<float>(p.a);
@@ -264,7 +269,11 @@ using namespace zkds;
 
 extern "C" {
 
-int zkfp_paged_path(const zkfp_paged_attention_args* a) { return 0; }
+int zkfp_paged_path(const zkfp_paged_attention_args* a)
+{
+    if (paged_stream_takes(*a)) return 2;
+    return paged_tile_takes(*a) ? 1 : 0;
+}
 
 long long zkfp_paged_scratch(const zkfp_paged_attention_args* a)
 {
@@ -288,7 +297,13 @@ int zkfp_paged_attention(const zkfp_paged_attention_args* a, void* stream)
     p.ml = a->scratch + 2ll * p.grid * p.tile * a->dv;
     p.error_flag = fp_error_flag();
     if (!p.error_flag) return ZKDS_ERR_WORKSPACE;
-    return a->dtype == ZKFP_BF16 ? launch_plain<bf16>(p, (cudaStream_t)stream) : launch_plain<float>(p, (cudaStream_t)stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    const int path = zkfp_paged_path(a);
+    if (path) {
+        const int rc = path == 2 ? launch_paged_stream(p, st) : launch_paged_tile(p, st);
+        return rc != ZKDS_OK ? rc : launch_combine<bf16>(p, 1, st);
+    }
+    return a->dtype == ZKFP_BF16 ? launch_plain<bf16>(p, st) : launch_plain<float>(p, st);
 }
 
 }  // extern "C"

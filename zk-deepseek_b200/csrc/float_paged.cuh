@@ -290,4 +290,12 @@ __device__ __forceinline__ void finish_row(const Paged& p, const Walk& w, int ro
     }
 }
 
+// ---- kernels on the tensor cores (float_paged_tc.cu): whether they take a call, their tile and grid, and the launch -----
+bool paged_stream_takes(const zkfp_paged_attention_args& a);
+void paged_stream_shape(Paged& p);
+int launch_paged_stream(const Paged& p, cudaStream_t st);
+bool paged_tile_takes(const zkfp_paged_attention_args& a);
+void paged_tile_shape(Paged& p);
+int launch_paged_tile(const Paged& p, cudaStream_t st);
+
 }  // namespace zkds

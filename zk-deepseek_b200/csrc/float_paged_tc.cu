@@ -1,0 +1,826 @@
+// Attention of new tokens over pages on the tensor cores, bfloat16 operands, 32-bit scores, weights and sums.  How the work is
+// shared, and what becomes of an item that several CTAs take parts of, is in float_paged.cuh.
+//
+// paged_stream_kernel: up to 16 query rows (tokens of the step times heads of a group) per key head, so that keys and values are read once
+// and their bytes are the bound.  A warp works by itself: it owns every fourth stretch of 16 keys, loads it by TMA into a ring of its
+// own and keeps maxima, sums and the weighted values of all 16 rows in registers (m16n8k16 products: queries are the
+// A operand and stay in registers, keys and values are read from the swizzled tiles by ldmatrix).  No warp waits for
+// another one before the item ends.
+//
+// paged_tile_kernel: more rows.  An item is two tiles of up to 128 rows over tiles of 128 keys: scores and outputs of both in tensor
+// memory, bfloat16 weights overwrite their scores and are the tensor-memory operand of the second product; while one tile is
+// in its softmax the tensor core works for the other.  The rows of a tile are (token, head) pairs, so that all heads of a
+// group share the keys that they read.
+//   warp 0      TMA loads          warp 1      MMA issue
+//   warps 2-9   softmax, tile 0    warps 10-17 softmax, tile 1: two threads share a query row, half of the columns each
+// The running maximum only replaces the one in use when it has grown by more than 2^8; the output tile is then rescaled in
+// place.  CTAs stay and take one part of an item after the other.
+#include <cuda.h>
+
+#include "float_paged.cuh"
+#include "tcgen05.cuh"
+
+namespace zkds {
+
+bool fp_tensor_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                   const uint32_t* box);
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- few rows ----------------------------------------------------------------------------------------------------
+constexpr int kStreamWarps = 4, kStretch = 16, kStreamRows = 16, kStreamKeys = kStreamWarps * kStretch, kStreamMost = 128;
+constexpr int kStretchSeg = kStretch * 128;            // bytes of 16 keys x 64 columns
+constexpr int kStreamStages = 4;
+
+struct StreamShape {
+    int segk, segv, box, stages;
+    size_t smem;
+    StreamShape(const zkfp_paged_attention_args& a)
+    {
+        segk = (a.d + 63) / 64;
+        segv = (a.dv + 63) / 64;
+        box = a.page < kStretch ? a.page : kStretch;
+        const size_t fixed = 1024 + plan_bytes(a.batch) + (size_t)kStreamRows * (a.dv + 4) * 4 + 2 * kStreamRows * 4 + 256;
+        const size_t stage = (size_t)kStreamWarps * (segk + segv) * kStretchSeg, room = 112 * 1024 - fixed;
+        stages = (int)(room / stage < kStreamStages ? room / stage : kStreamStages);
+        smem = fixed + stages * stage;
+    }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// the stretch of keys that a warp takes of a unit, and whether any row of the item sees some of it
+struct Stretch {
+    int k0;
+    bool seen;
+    __device__ __forceinline__ Stretch(const Paged& p, const Walk& w, int j, int warp)
+    {
+        const int rows = min(p.tile, w.n * p.group - w.t * p.tile), base = w.len - w.n;
+        const int i0 = base + w.t * p.tile / p.group, i1 = base + (w.t * p.tile + rows - 1) / p.group;
+        k0 = (w.first + j) * kStreamKeys + warp * kStretch;
+        seen = k0 <= i1 && (p.a.window <= 0 || k0 + kStretch > i0 - p.a.window + 1);
+    }
+};
+
+template <int SEGK, int SEGV>
+__global__ void __launch_bounds__(kStreamWarps * 32, 2)
+paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ Paged p, int box, int stages)
+{
+    extern __shared__ uint8_t raw[];
+    chain_enter();
+    const zkfp_paged_attention_args& a = p.a;
+    uint8_t* ring = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = (int)a.batch, dv = a.dv, pitch = dv + 4;
+    constexpr uint32_t kStage = (SEGK + SEGV) * kStretchSeg;
+    uint8_t* behind = ring + kStreamWarps * stages * kStage;
+    uint64_t* bars = (uint64_t*)behind;                        // [warp][stage]
+    float* M = (float*)(bars + kStreamWarps * kStreamStages);
+    float *L = M + kStreamRows, *O = L + kStreamRows;
+    int* gave_up = (int*)(O + kStreamRows * pitch);
+    const Plan plan((uint8_t*)(gave_up + 4), batch);
+    volatile int* abort_flag = gave_up;
+    if (threadIdx.x == 0) {
+        *gave_up = 0;
+        for (int i = 0; i < kStreamWarps * stages; ++i) mbar_init(smem_u32(bars + i), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    make_plan(p, plan);
+    const long long units = plan.before[batch], u1 = range_begin(units, blockIdx.x + 1, p.grid);
+    long long u = range_begin(units, blockIdx.x, p.grid), ui = u;
+    if (u >= u1) return;
+    const uint32_t one = elect_one(), my_ring = smem_u32(ring) + warp * stages * kStage, my_bars = smem_u32(bars + warp * stages);
+    Walk w, wi;
+    w.locate(p, plan, u);
+    wi = w;
+    int ji = wi.j, slot_i = 0, slot = 0;
+    uint32_t phase = 0;
+    // pages of the next 32 stretches of the item that is being loaded: lane i holds that of unit base + i
+    int page_base = -1, page_id = 0, page_id2 = 0;
+    auto issue = [&] {
+        if (ui >= u1) return;
+        const Stretch st(p, wi, ji, warp);
+        if (page_base < 0 || ji >= page_base + 32) {
+            page_base = ji;
+            const int j = ji + lane;
+            page_id = page_id2 = (int)a.pages;                 // beyond the tensor: the tile is filled with zeros
+            if (j < wi.count) {
+                const int k = (wi.first + j) * kStreamKeys + warp * kStretch;
+                bool bad = false;
+                if (k < wi.len) {
+                    const long long page = page_of(p, wi.b, k);
+                    if (page >= 0) page_id = (int)page;
+                    else bad = true;
+                }
+                if (box < kStretch && k + 8 < wi.len) {
+                    const long long page = page_of(p, wi.b, k + 8);
+                    if (page >= 0) page_id2 = (int)page;
+                    else bad = true;
+                }
+                if (bad) *(volatile int*)p.error_flag = 1;
+            }
+        }
+        if (st.seen) {
+            const int page = __shfl_sync(0xffffffffu, page_id, ji - page_base), page2 = __shfl_sync(0xffffffffu, page_id2, ji - page_base);
+            const uint32_t bar = my_bars + slot_i * 8, dst = my_ring + slot_i * kStage;
+            const int line = st.k0 & (a.page - 1);
+            mbar_expect_tx(bar, kStage, one);
+#pragma unroll
+            for (int c = 0; c < SEGK + SEGV; ++c) {
+                const CUtensorMap* map = c < SEGK ? &tmK : &tmV;
+                const int x = (c < SEGK ? c : c - SEGK) * 64;
+                tma_load_4d(dst + c * kStretchSeg, map, x, wi.kv, line, page, bar, one);
+                if (box < kStretch) tma_load_4d(dst + c * kStretchSeg + 1024, map, x, wi.kv, 0, page2, bar, one);
+            }
+            if (++slot_i == stages) slot_i = 0;
+        }
+        ++ui;
+        if (++ji == wi.count && ui < u1) {
+            wi.next(p, plan);
+            ji = 0;
+            page_base = -1;
+        }
+    };
+    // a stretch that no row sees takes no place in the ring: as many are on their way as the ring holds
+    auto loads = [&](const Walk& at, int j) { return Stretch(p, at, j, warp).seen; };
+    int ahead = 0;
+    auto fill = [&] {
+        while (ui < u1 && ahead < stages) {
+            ahead += loads(wi, ji) ? 1 : 0;
+            issue();
+        }
+    };
+    fill();
+    bool ok = true;
+    for (; u < u1;) {
+        const int j_end = (int)min((long long)w.count, w.j + (u1 - u));
+        const bool whole = w.j == 0 && j_end == w.count;
+        const int row0 = w.t * p.tile, rows = min(p.tile, w.n * p.group - row0), r = lane >> 2, cq = (lane & 3) * 2;
+        // queries: rows r and r + 8, elements cq, cq + 1 and eight further on of every 16
+        uint32_t q[SEGK * 4][4];
+        int pos[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int rr = row0 + r + 8 * h, t = rr / p.group, head = w.kv * p.group + rr - t * p.group;
+            const bool in = r + 8 * h < rows;
+            pos[h] = in ? w.len - w.n + t : -1;
+            const bf16* src = (const bf16*)a.q + (long long)(w.row0 + t) * a.q_tok + head * a.q_head;
+#pragma unroll
+            for (int k = 0; k < SEGK * 4; ++k) {
+                const int c = k * 16 + cq;
+                q[k][h] = in && c < a.d ? *(const uint32_t*)(src + c) : 0u;
+                q[k][h + 2] = in && c + 8 < a.d ? *(const uint32_t*)(src + c + 8) : 0u;
+            }
+        }
+        float o[SEGV * 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+        const float scale = a.scale * kLog2e;
+        for (int j = w.j; j < j_end; ++j, ++u) {
+            const Stretch st(p, w, j, warp);
+            if (!st.seen) continue;
+            const uint32_t tile = my_ring + slot * kStage;
+            if (ok) ok = mbar_wait_warp(my_bars + slot * 8, phase, abort_flag);
+            float s[2][4] = {};
+#pragma unroll
+            for (int k = 0; k < SEGK * 2; ++k) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    uint32_t b[4];
+                    const int key = t * 8 + (lane & 7), chunk = k * 4 + (lane >> 3);
+                    ldmatrix4(b, tile + (chunk >> 3) * kStretchSeg + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+                    mma16816(s[t], q[2 * k], b[0], b[1]);
+                    mma16816(s[t], q[2 * k + 1], b[2], b[3]);
+                }
+            }
+            // s[t][2 h + e]: row r + 8 h, key k0 + 8 t + cq + e
+            float f[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = -INFINITY;
+                const int lo = a.window > 0 ? pos[h] - a.window : -1;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = st.k0 + 8 * t + cq + e;
+                        float& x = s[t][2 * h + e];
+                        x = key <= pos[h] && key > lo ? x * scale : -INFINITY;
+                        top = fmaxf(top, x);
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float m_new = fmaxf(m[h], top), m_sub = m_new == -INFINITY ? 0.f : m_new;
+                f[h] = exp2_approx(m[h] - m_sub);
+                m[h] = m_new;
+                float sum = 0.f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& x = s[t][2 * h + e];
+                        x = exp2_approx(x - m_sub);
+                        sum += x;
+                    }
+                l[h] = l[h] * f[h] + sum;
+            }
+            if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < SEGV * 8; ++c) {
+                    o[c][0] *= f[0]; o[c][1] *= f[0];
+                    o[c][2] *= f[1]; o[c][3] *= f[1];
+                }
+            }
+            if (st.k0 + kStretch > w.len) {                    // lines that the sequence does not hold: no value, whatever is there
+                for (int i = lane; i < SEGV * 128; i += 32) {
+                    const int c = i >> 7, line = (i >> 3) & 15;
+                    if (st.k0 + line >= w.len)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (SEGK + c) * kStretchSeg + (i & 127) * 16), "r"(0) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
+            const uint32_t pa[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
+#pragma unroll
+            for (int c = 0; c < SEGV * 4; ++c) {
+                uint32_t b[4];
+                const int key = (lane & 15), chunk = c * 2 + (lane >> 4);
+                ldmatrix4_trans(b, tile + (SEGK + (chunk >> 3)) * kStretchSeg + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+                mma16816(o[2 * c], pa, b[0], b[1]);
+                mma16816(o[2 * c + 1], pa, b[2], b[3]);
+            }
+            __syncwarp();                                      // every lane has read the tile
+            --ahead;
+            if (++slot == stages) { slot = 0; phase ^= 1u; }
+            fill();
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        }
+        // the warps' sums, one after the other
+        for (int i = 0; i < kStreamWarps; ++i) {
+            __syncthreads();
+            if (warp != i) continue;
+            float mine[2] = {1.f, 1.f}, theirs[2] = {};
+            if (i) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float mo = M[r + 8 * h], top = fmaxf(mo, m[h]);
+                    mine[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - top);
+                    theirs[h] = mo == -INFINITY ? 0.f : exp2_approx(mo - top);
+                    l[h] = l[h] * mine[h] + L[r + 8 * h] * theirs[h];
+                    m[h] = top;
+                }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int rr = r + 8 * h;
+                if ((lane & 3) == 0) { M[rr] = m[h]; L[rr] = l[h]; }
+                if (rr >= rows) continue;
+#pragma unroll
+                for (int c = 0; c < SEGV * 8; ++c) {
+                    if (c * 8 + cq >= dv) continue;
+                    float2* at = (float2*)(O + rr * pitch + c * 8 + cq);
+                    float2 x = make_float2(o[c][2 * h] * mine[h], o[c][2 * h + 1] * mine[h]);
+                    if (theirs[h] != 0.f) {
+                        const float2 y = *at;
+                        x.x = fmaf(y.x, theirs[h], x.x);
+                        x.y = fmaf(y.y, theirs[h], x.y);
+                    }
+                    *at = x;
+                }
+            }
+        }
+        __syncthreads();
+        const int part = 2 * blockIdx.x + (w.j == 0 ? 1 : 0);
+        for (int rr = warp; rr < rows; rr += kStreamWarps) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = lane + 32 * k < dv ? O[rr * pitch + lane + 32 * k] : 0.f;
+            if (whole) {
+                finish_row<bf16>(p, w, row0 + rr, x, L[rr]);
+                continue;
+            }
+            float* to = p.part + ((long long)part * p.tile + rr) * dv;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (lane + 32 * k < dv) to[lane + 32 * k] = x[k];
+            if (lane < 2) p.ml[((long long)part * p.tile + rr) * 2 + lane] = lane ? L[rr] : M[rr];
+        }
+        if (u < u1) w.next(p, plan);
+    }
+    if (!ok) *(volatile int*)p.error_flag = 1;
+}
+
+
+// ---- many rows ---------------------------------------------------------------------------------------------------
+constexpr int kTile = 128;                     // query rows and keys per tile
+constexpr uint32_t kSeg = kTile * 128;         // bytes of 128 rows x 64 bfloat16
+constexpr int kTileThreads = 576, kTileMost = 128;
+constexpr int kMaxKeySlots = 8;
+
+struct TileParams {
+    Paged p;
+    int rows;                                  // query rows of a tile: whole groups, up to 128
+    int box;                                   // lines of a page in one load
+    int seg, segv, k_slots, v_stages;          // segments of 64 columns, ring of key segments, value tiles
+    float scale_log2;
+};
+
+struct TileShared {
+    uint64_t q_full, q_empty, k_full[kMaxKeySlots], k_empty[kMaxKeySlots], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2];
+    float row_max[2][2][kTile];                // [query tile][column half][row]; at the end of an item the row sums
+    uint32_t tmem;
+    int abort;
+};
+
+// The part of an item that a CTA takes: tiles of keys begin .. end - 1 in units of kTile positions, those that query tile g
+// takes part in, and the rows of g.
+struct Part {
+    int begin, end, row0[2], rows[2], first[2], last[2];
+    __device__ __forceinline__ Part(const TileParams& t, const Walk& w, long long left)
+    {
+        const int all = w.n * t.p.group, base = w.len - w.n;
+        begin = w.first + w.j;
+        end = w.first + (int)min((long long)w.count, w.j + left);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            row0[g] = w.t * t.p.tile + g * t.rows;
+            rows[g] = max(0, min(t.rows, all - row0[g]));
+            const int i0 = base + row0[g] / t.p.group, i1 = base + (row0[g] + rows[g] - 1) / t.p.group;
+            const int lo = t.p.a.window > 0 ? max(i0 - t.p.a.window + 1, 0) / kTile : 0;
+            first[g] = max(begin, lo);
+            last[g] = rows[g] > 0 && i1 >= 0 ? min(end - 1, i1 / kTile) : first[g] - 1;
+        }
+    }
+    __device__ __forceinline__ bool active(int g, int j) const { return g ? j >= first[1] && j <= last[1] : j >= first[0] && j <= last[0]; }
+};
+
+// A row of bfloat16 that did not come out finite, once more: its columns from `begin` to `end`.
+__device__ __noinline__ void finish_again(const Paged& p, const Walk& w, int row, int in_seq, int begin, int end)
+{
+    const int lane = threadIdx.x & 31, head = w.kv * p.group + row - in_seq * p.group, token = w.row0 + in_seq;
+    float x[8];
+    attend_row<bf16>(p, w.b, w.kv, token, head, w.len - w.n + in_seq, x);
+    bf16* out = (bf16*)p.a.out + (long long)token * p.a.o_tok + head * p.a.o_head;
+    const bf16* gate = p.a.gate ? (const bf16*)p.a.gate + (long long)token * p.a.gate_tok + head * p.a.gate_head : nullptr;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int c = lane + 32 * k;
+        if (c < begin || c >= end) continue;
+        if (gate) x[k] *= sigmoid_f(__bfloat162float(gate[c])) * p.a.out_scale;
+        out[c] = __float2bfloat16_rn(x[k]);
+    }
+}
+
+__global__ void __launch_bounds__(kTileThreads, 1)
+paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ TileParams t)
+{
+    extern __shared__ __align__(1024) uint8_t raw[];
+    chain_enter();
+    const Paged& p = t.p;
+    const zkfp_paged_attention_args& a = p.a;
+    uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t tile_bytes = (uint32_t)(2 * t.seg + t.k_slots + t.v_stages * t.segv) * kSeg;
+    TileShared& s = *reinterpret_cast<TileShared*>(base + tile_bytes);
+    const Plan plan(base + tile_bytes + ((sizeof(TileShared) + 15) & ~15), (int)a.batch);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t sQ = smem_u32(base), bytesQ = (uint32_t)t.seg * kSeg;
+    const uint32_t sK = sQ + 2 * bytesQ, sV = sK + (uint32_t)t.k_slots * kSeg, bytesV = (uint32_t)t.segv * kSeg;
+    volatile int* abort_flag = &s.abort;
+    if (threadIdx.x == 0) {
+        s.abort = 0;
+        mbar_init(smem_u32(&s.q_full), 1);
+        mbar_init(smem_u32(&s.q_empty), 1);
+        for (int i = 0; i < kMaxKeySlots; ++i) {
+            mbar_init(smem_u32(&s.k_full[i]), 1);
+            mbar_init(smem_u32(&s.k_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&s.v_full[i]), 1);
+            mbar_init(smem_u32(&s.v_empty[i]), 1);
+            mbar_init(smem_u32(&s.s_full[i]), 1);
+            mbar_init(smem_u32(&s.p_full[i]), 8);
+            mbar_init(smem_u32(&s.o_full[i]), 1);
+            mbar_init(smem_u32(&s.o_empty[i]), 8);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 1) tmem_alloc(smem_u32(&s.tmem), 512);
+    make_plan(p, plan);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s.tmem;
+    const long long units = plan.before[a.batch], u1 = range_begin(units, blockIdx.x + 1, p.grid);
+    long long u = range_begin(units, blockIdx.x, p.grid);
+    Walk w;
+    if (u < u1) w.locate(p, plan, u);
+
+    if (warp == 0) {
+        const uint32_t one = elect_one();
+        int ks = 0, vs = 0;
+        uint32_t kp = 0, vp = 0, qp = 0;
+        bool ok = true;
+        while (u < u1 && ok) {
+            const Part part(t, w, u1 - u);
+            if (!(ok = mbar_wait_warp(smem_u32(&s.q_empty), qp ^ 1u, abort_flag))) break;
+            qp ^= 1u;
+            const uint32_t row_bytes = (uint32_t)t.rows * 128u;
+            mbar_expect_tx(smem_u32(&s.q_full), (uint32_t)t.seg * row_bytes * (part.rows[1] > 0 ? 2 : 1), one);
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+                if (part.rows[g] > 0)
+                    for (int c = 0; c < t.seg; ++c)
+                        tma_load_4d(sQ + g * bytesQ + c * kSeg, &tmQ, c * 64, 0, w.kv, w.row0 + part.row0[g] / p.group, smem_u32(&s.q_full), one);
+            for (int j = part.begin; j < part.end && ok; ++j) {
+                // pages of this tile of keys: lane i holds that of its i-th box
+                int mine = (int)a.pages;                       // beyond the tensor: zeros
+                const int at = j * kTile + lane * t.box;
+                if (lane * t.box < kTile && at < w.len) {
+                    const long long page = page_of(p, w.b, at);
+                    if (page >= 0) mine = (int)page;
+                    else *(volatile int*)p.error_flag = 1;
+                }
+                __syncwarp();
+                const int line = (j * kTile) & (a.page - 1);
+                for (int c = 0; c < t.seg; ++c) {
+                    if (!(ok = mbar_wait_warp(smem_u32(&s.k_empty[ks]), kp ^ 1u, abort_flag))) break;
+                    const uint32_t bar = smem_u32(&s.k_full[ks]), dst = sK + (uint32_t)ks * kSeg;
+                    mbar_expect_tx(bar, kSeg, one);
+                    for (int i = 0; i * t.box < kTile; ++i)
+                        tma_load_4d(dst + i * t.box * 128, &tmK, c * 64, w.kv, line, __shfl_sync(0xffffffffu, mine, i), bar, one);
+                    if (++ks == t.k_slots) { ks = 0; kp ^= 1u; }
+                }
+                if (!ok || !(ok = mbar_wait_warp(smem_u32(&s.v_empty[vs]), vp ^ 1u, abort_flag))) break;
+                const uint32_t bar = smem_u32(&s.v_full[vs]), dst = sV + (uint32_t)vs * bytesV;
+                mbar_expect_tx(bar, bytesV, one);
+                for (int c = 0; c < t.segv; ++c)
+                    for (int i = 0; i * t.box < kTile; ++i)
+                        tma_load_4d(dst + c * kSeg + i * t.box * 128, &tmV, c * 64, w.kv, line, __shfl_sync(0xffffffffu, mine, i), bar, one);
+                if (++vs == t.v_stages) { vs = 0; vp ^= 1u; }
+            }
+            u += part.end - part.begin;
+            if (u < u1) w.next(p, plan);
+        }
+    } else if (warp == 1) {
+        const uint32_t one = elect_one(), tm = uniform(tmem);
+        const uint32_t idesc_s = idesc_bf16(kTile, kTile), idesc_o = idesc_bf16(kTile, (a.dv + 15) & ~15, true);
+        uint32_t pp[2] = {0, 0}, op[2] = {0, 0}, kp = 0, vp = 0, qp = 0;
+        int ks = 0, vs = 0;
+        bool ok = true;
+        while (u < u1 && ok) {
+            Part part(t, w, u1 - u);
+            part.begin = (int)uniform(part.begin);
+            part.end = (int)uniform(part.end);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                part.first[g] = (int)uniform(part.first[g]);
+                part.last[g] = (int)__reduce_max_sync(0xffffffffu, part.last[g]);
+            }
+            // the scores of query tile g with the keys at (ks, kp); `load` waits for their segments, `release` hands each back
+            auto scores = [&](int g, bool use, bool load, bool release) {
+                const uint32_t d = tm + (uint32_t)g * kTile;
+                int slot = ks;
+                uint32_t phase = kp;
+                for (int c = 0; c < t.seg; ++c) {
+                    if (load) {
+                        if (!mbar_wait_warp(smem_u32(&s.k_full[slot]), phase, abort_flag)) return false;
+                        tc_fence_after();
+                    }
+                    if (use) {
+                        const int cols = a.d - c * 64;
+                        const uint64_t ad = smem_desc_sw128(sQ + (uint32_t)g * bytesQ + (uint32_t)c * kSeg), bd = smem_desc_sw128(sK + (uint32_t)slot * kSeg);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k * 16 < cols) umma_bf16(d, ad + (uint64_t)(k * 2), bd + (uint64_t)(k * 2), idesc_s, (c | k) ? 1u : 0u, one);
+                    }
+                    if (release) umma_commit(smem_u32(&s.k_empty[slot]), one);
+                    if (++slot == t.k_slots) { slot = 0; phase ^= 1u; }
+                }
+                if (use) umma_commit(smem_u32(&s.s_full[g]), one);
+                if (release) { ks = slot; kp = phase; }
+                return true;
+            };
+            if (!(ok = mbar_wait_warp(smem_u32(&s.q_full), qp, abort_flag))) break;
+            qp ^= 1u;
+            for (int j = part.begin - 1; j < part.end && ok; ++j) {
+                if (j >= part.begin) {
+                    if (!(ok = mbar_wait_warp(smem_u32(&s.v_full[vs]), vp, abort_flag))) break;
+                    tc_fence_after();
+                }
+                for (int g = 0; g < 2 && ok; ++g) {
+                    if (j >= part.begin && part.active(g, j)) {
+                        const bool opens = j == (g ? part.first[1] : part.first[0]), closes = j == (g ? part.last[1] : part.last[0]);
+                        if (opens) {                           // the last item's sums have been read
+                            if (!(ok = mbar_wait_warp(smem_u32(&s.o_empty[g]), op[g] ^ 1u, abort_flag))) break;
+                            op[g] ^= 1u;
+                        }
+                        if (!(ok = mbar_wait_warp(smem_u32(&s.p_full[g]), pp[g], abort_flag))) break;
+                        pp[g] ^= 1u;
+                        tc_fence_after();
+                        const uint32_t ta = tm + (uint32_t)g * kTile, d = tm + 256u + (uint32_t)g * kTile;
+                        const uint64_t vd = smem_desc_mn_sw128(sV + (uint32_t)vs * bytesV, kSeg);
+#pragma unroll
+                        for (int k = 0; k < kTile / 16; ++k)
+                            umma_bf16_ts(d, ta + (uint32_t)k * 8u, vd + (uint64_t)(k * 128), idesc_o, (!opens || k) ? 1u : 0u, one);
+                        if (closes) umma_commit(smem_u32(&s.o_full[g]), one);
+                    }
+                    if (j >= part.begin && g == 1) umma_commit(smem_u32(&s.v_empty[vs]), one);
+                    // every segment is waited for once and handed back once, also when no query tile uses it
+                    if (j + 1 < part.end) {
+                        ok = scores(g, part.active(g, j + 1), g == 0, g == 1);
+                        if (ok && g == 1 && j + 2 == part.end) umma_commit(smem_u32(&s.q_empty), one);
+                    }
+                }
+                if (!ok) break;
+                if (j >= part.begin && ++vs == t.v_stages) { vs = 0; vp ^= 1u; }
+            }
+            u += part.end - part.begin;
+            if (u < u1) w.next(p, plan);
+        }
+    } else {
+        const int g = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane, c0 = half * 64;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t tS = tmem + (uint32_t)g * kTile + lanes, tO = tmem + 256u + (uint32_t)g * kTile + lanes;
+        const int middle = (a.dv / 2 + 31) & ~31, o_begin = half ? middle : 0, o_end = half ? a.dv : min(a.dv, middle);
+        auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quarter) : "memory"); };
+        uint32_t sp = 0, op = 0;
+        bool ok = true;
+        while (u < u1 && ok) {
+            const Part part(t, w, u1 - u);
+            const bool whole = w.j == 0 && part.end - part.begin == w.count;
+            const int rows = part.rows[g], first_tile = part.first[g], last_tile = part.last[g], row_all = part.row0[g] + row;
+            const int in_seq = row_all / p.group, pos = row < rows ? w.len - w.n + in_seq : -1;
+            float m_used = -INFINITY, l = 0.f;
+            for (int j = first_tile; j <= last_tile && ok; ++j) {
+                if (!(ok = mbar_wait_warp(smem_u32(&s.s_full[g]), sp, abort_flag))) break;
+                sp ^= 1u;
+                tc_fence_after();
+                float v[2][32];
+                tmem_ld32(tS + (uint32_t)c0, v[0]);
+                tmem_ld32(tS + (uint32_t)c0 + 32u, v[1]);
+                // visible columns of this row: c_lo .. c_hi
+                const int c_hi = pos - j * kTile, c_lo = a.window > 0 ? c_hi - a.window + 1 : -1;
+                const bool masked = __any_sync(0xffffffffu, c_hi < kTile - 1 || c_lo > 0);
+                tmem_ld_wait();
+                if (masked) {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c)
+                        if (c0 + c < c_lo || c0 + c > c_hi) v[c >> 5][c & 31] = -INFINITY;
+                }
+                float mp[8];                              // independent chains
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mp[i] = v[0][i];
+#pragma unroll
+                for (int c = 8; c < 64; ++c) mp[c & 7] = fmaxf(mp[c & 7], v[c >> 5][c & 31]);
+                const float mine = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
+                                         fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
+                s.row_max[g][half][row] = mine;
+                // also: both threads of every row have read their scores before either overwrites any of them
+                pair_sync();
+                const float m_new = fmaxf(m_used, fmaxf(mine, s.row_max[g][half ^ 1][row]) * t.scale_log2);
+                if (j == first_tile) {
+                    m_used = m_new;
+                } else if (__any_sync(0xffffffffu, m_new > m_used + 8.0f)) {     // the same rows, so the same decision in both warps
+                    const float f = m_used == -INFINITY ? 0.f : exp2_approx(m_used - m_new);
+                    for (int c = o_begin; c < o_end; c += 8) {
+                        int32_t o[8];
+                        tmem_ld8(tO + (uint32_t)c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) o[i] = __float_as_int(__int_as_float(o[i]) * f);
+                        tmem_st8(tO + (uint32_t)c, o);
+                    }
+                    l *= f;
+                    m_used = m_new;
+                }
+                const float m_sub = m_used == -INFINITY ? 0.f : m_used;
+                float lp[4] = {};
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t x[16];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[q][i] = exp2_approx(fmaf(v[q][i], t.scale_log2, -m_sub));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) lp[i & 3] += v[q][i];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = pack_bf16(v[q][2 * i], v[q][2 * i + 1]);
+                    tmem_st16(tS + (uint32_t)(half * 32 + q * 16), x);
+                }
+                l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s.p_full[g]));
+            }
+            if (!ok) break;
+            const bool any = first_tile <= last_tile;
+            if (any) {
+                pair_sync();                              // the last maxima have been read
+                s.row_max[g][half][row] = l;
+                pair_sync();
+                l += s.row_max[g][half ^ 1][row];
+                pair_sync();                              // the sums too, before the next item's maxima
+                if (!(ok = mbar_wait_warp(smem_u32(&s.o_full[g]), op, abort_flag))) break;
+                op ^= 1u;
+                tc_fence_after();
+            }
+            const int head = w.kv * p.group + row_all - in_seq * p.group;
+            const long long token = w.row0 + in_seq;
+            if (whole) {
+                const float r = pos >= 0 ? 1.0f / l : 0.f;
+                bf16* out = (bf16*)a.out + token * a.o_tok + head * a.o_head;
+                const bf16* gate = a.gate ? (const bf16*)a.gate + token * a.gate_tok + head * a.gate_head : nullptr;
+                bool finite = true;
+                for (int c = o_begin; c < o_end; c += 8) {
+                    int32_t x[8] = {};
+                    if (any) {
+                        tmem_ld8(tO + (uint32_t)c, x);
+                        tmem_ld_wait();
+                    }
+                    if (row < rows) {
+                        float y[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            y[k] = pos >= 0 ? __int_as_float(x[k]) * r : 0.f;
+                            finite = finite && isfinite(y[k]);
+                        }
+                        if (gate) {
+                            float z[8];
+                            load8(gate + c, z);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) y[k] *= sigmoid_f(z[k]) * a.out_scale;
+                        }
+                        store8(out + c, y);
+                    }
+                    __syncwarp();
+                }
+                for (unsigned again = __ballot_sync(0xffffffffu, !finite); again; again &= again - 1) {
+                    const int who = __ffs(again) - 1, rr = part.row0[g] + quarter * 32 + who, tok = rr / p.group;
+                    finish_again(p, w, rr, tok, o_begin, o_end);
+                }
+            } else {
+                const long long at = (2ll * blockIdx.x + (w.j == 0 ? 1 : 0)) * p.tile + g * t.rows + row;
+                for (int c = o_begin; c < o_end; c += 8) {
+                    int32_t x[8] = {};
+                    if (any) {
+                        tmem_ld8(tO + (uint32_t)c, x);
+                        tmem_ld_wait();
+                    }
+                    if (row < rows) {
+                        float y[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) y[k] = __int_as_float(x[k]);
+                        store8(p.part + at * a.dv + c, y);
+                    }
+                    __syncwarp();
+                }
+                if (row < rows) p.ml[at * 2 + half] = half ? l : m_used;
+            }
+            if (any) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s.o_empty[g]));
+            }
+            u += part.end - part.begin;
+            if (u < u1) w.next(p, plan);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, 512);
+    if (threadIdx.x == 0 && s.abort) *(volatile int*)p.error_flag = 1;
+}
+
+struct TileShape {
+    int rows, box, seg, segv, k_slots, v_stages;
+    size_t smem;
+    TileShape(const zkfp_paged_attention_args& a)
+    {
+        const int group = a.heads / a.kv_heads;
+        rows = group <= kTile ? kTile / group * group : 0;
+        box = a.page < kTile ? a.page : kTile;
+        seg = (a.d + 63) / 64;
+        segv = (a.dv + 63) / 64;
+        const size_t fixed = 1024 + ((sizeof(TileShared) + 15) & ~15) + plan_bytes(a.batch), segs = (kSharedMax - 1024 - fixed) / kSeg;
+        v_stages = 3 * seg + 2 * segv <= (int)segs ? 2 : 1;
+        const int left = (int)segs - 2 * seg - v_stages * segv;
+        k_slots = left < kMaxKeySlots ? left : kMaxKeySlots;
+        smem = fixed + kSeg * (size_t)(2 * seg + k_slots + v_stages * segv);
+    }
+};
+
+// [size][heads][lines][pages], pieces of 64 columns of one head of `rows` lines of a page
+bool pages_map(CUtensorMap* map, const void* base, int size, int heads, int page, long long pages, long long head, long long pos, long long stride,
+               int rows)
+{
+    auto at_least = [](long long s, long long least) { return (uint64_t)(s > 0 ? s : least) * 2; };       // one head, line or page has no stride
+    const uint64_t dims[4] = {(uint64_t)size, (uint64_t)heads, (uint64_t)page, (uint64_t)pages};
+    const uint64_t strides[3] = {at_least(head, size), at_least(pos, size), at_least(stride, size)};
+    const uint32_t box[4] = {64, 1, (uint32_t)rows, 1};
+    return fp_tensor_map(map, base, 4, dims, strides, box);
+}
+
+bool key_maps(CUtensorMap* k, CUtensorMap* v, const zkfp_paged_attention_args& a, int rows)
+{
+    return pages_map(k, a.k, a.d, a.kv_heads, a.page, a.pages, a.k_head, a.k_pos, a.k_page, rows) &&
+           pages_map(v, a.v, a.dv, a.kv_heads, a.page, a.pages, a.v_head, a.v_pos, a.v_page, rows);
+}
+
+}  // namespace
+
+bool paged_stream_takes(const zkfp_paged_attention_args& a)
+{
+    return a.dtype == ZKFP_BF16 && a.d <= kStreamMost && a.dv <= kStreamMost && a.max_tokens * (a.heads / a.kv_heads) <= kStreamRows &&
+           StreamShape(a).stages >= 2;
+}
+
+void paged_stream_shape(Paged& p)
+{
+    p.tile = kStreamRows;
+    p.block = kStreamKeys;
+    p.grid = 2 * fp_sm_count();
+}
+
+template <int SEGK, int SEGV>
+static int launch_stream(const Paged& p, const CUtensorMap& k, const CUtensorMap& v, const StreamShape& s, cudaStream_t st)
+{
+    ZKDS_CUDA(cudaFuncSetAttribute(paged_stream_kernel<SEGK, SEGV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024));
+    fp_launch(paged_stream_kernel<SEGK, SEGV>, dim3((unsigned)p.grid), dim3(kStreamWarps * 32), s.smem, st, k, v, p, s.box, s.stages);
+    return fp_launched();
+}
+
+bool paged_tile_takes(const zkfp_paged_attention_args& a)
+{
+    if (a.dtype != ZKFP_BF16 || a.d > kTileMost || a.dv > kTileMost) return false;
+    const TileShape s(a);
+    return s.rows > 0 && s.k_slots >= s.seg;
+}
+
+void paged_tile_shape(Paged& p)
+{
+    p.tile = 2 * TileShape(p.a).rows;
+    p.block = kTile;
+    p.grid = fp_sm_count();
+}
+
+int launch_paged_tile(const Paged& p, cudaStream_t st)
+{
+    const zkfp_paged_attention_args& a = p.a;
+    const TileShape s(a);
+    TileParams t;
+    t.p = p;
+    t.rows = s.rows; t.box = s.box; t.seg = s.seg; t.segv = s.segv; t.k_slots = s.k_slots; t.v_stages = s.v_stages;
+    t.scale_log2 = a.scale * kLog2e;
+    CUtensorMap q, k, v;
+    const uint64_t G = (uint64_t)p.group, head = (uint64_t)(a.q_head > 0 ? a.q_head : a.d) * 2;
+    const uint64_t dims[4] = {(uint64_t)a.d, G, (uint64_t)a.kv_heads, (uint64_t)a.tokens};
+    const uint64_t strides[3] = {head, head * G, a.q_tok > 0 ? (uint64_t)a.q_tok * 2 : head * G * a.kv_heads};
+    const uint32_t box[4] = {64, (uint32_t)G, 1, (uint32_t)(s.rows / p.group)};
+    if (!fp_tensor_map(&q, a.q, 4, dims, strides, box) || !key_maps(&k, &v, a, s.box)) return ZKDS_ERR_UNSUPPORTED;
+    ZKDS_CUDA(cudaFuncSetAttribute(paged_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - 1024));
+    // more than half the shared memory: one CTA per SM, so the tensor-memory allocation never waits
+    const size_t smem = s.smem < 120 * 1024 ? 120 * 1024 : s.smem;
+    fp_launch(paged_tile_kernel, dim3((unsigned)p.grid), dim3(kTileThreads), smem, st, q, k, v, t);
+    return fp_launched();
+}
+
+int launch_paged_stream(const Paged& p, cudaStream_t st)
+{
+    const StreamShape s(p.a);
+    CUtensorMap k, v;
+    if (!key_maps(&k, &v, p.a, s.box)) return ZKDS_ERR_UNSUPPORTED;
+    if (s.segk == 1) return s.segv == 1 ? launch_stream<1, 1>(p, k, v, s, st) : launch_stream<1, 2>(p, k, v, s, st);
+    return s.segv == 1 ? launch_stream<2, 1>(p, k, v, s, st) : launch_stream<2, 2>(p, k, v, s, st);
+}
+
+}  // namespace zkds
