@@ -40,27 +40,34 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
     float* M = P + kPlainRows * kPlainKeys;
     float *L = M + kPlainRows, *F = L + kPlainRows;
     make_plan(p, plan);
-    const long long units = plan.before[batch], u1 = range_begin(units, blockIdx.x + 1, p.grid);
-    long long u = range_begin(units, blockIdx.x, p.grid);
-    if (u >= u1) return;
+    const long long units = plan.before[batch];
+    const int ctas = sharing(p, units), cta = blockIdx.x;
+    if (tid == 0) no_cut(p, cta);
+    if (cta >= ctas || units == 0) return;
+    const long long u1 = range_begin(units, cta + 1, ctas);
+    long long u = range_begin(units, cta, ctas);
     Walk w;
     for (w.locate(p, plan, u); u < u1; w.next(p, plan)) {
-        const int j_end = (int)min((long long)w.count, w.j + (u1 - u));
-        const bool whole = w.j == 0 && j_end == w.count;
-        const int slot = 2 * blockIdx.x + (w.j == 0 ? 1 : 0), row0 = w.t * kPlainRows, rows = min(kPlainRows, w.n * p.group - row0);
+        const int taken = (int)min((long long)w.left(p), u1 - u), j_begin = w.begin(p), j_end = w.end(p, taken);
+        const long long end = u + w.left(p);
+        u += taken;
+        if (j_begin == j_end) continue;
+        const bool whole = j_begin == 0 && j_end == w.count;
+        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, units, ctas, w, end);
+        const int slot = 2 * cta + (j_begin == 0 ? 1 : 0), row0 = w.t * kPlainRows, rows = min(kPlainRows, w.n * p.group - row0);
         __syncthreads();
         for (int i = tid; i < kPlainRows * vd; i += kPlainThreads) {
             const int r = i / vd, c = (i - r * vd) * 8;
             float x[8] = {};
             if (r < rows) {
-                const int t = (row0 + r) / p.group, h = w.kv * p.group + (row0 + r) % p.group;
+                const int t = by_group(p, row0 + r), h = w.kv * p.group + row0 + r - t * p.group;
                 load8((const T*)a.q + (long long)(w.row0 + t) * a.q_tok + h * a.q_head + c, x);
             }
             store8(Q + r * d + c, x);
         }
         if (tid < kPlainRows) { M[tid] = -INFINITY; L[tid] = 0.f; }
         float acc[4][8] = {};
-        for (int j = w.j; j < j_end; ++j) {
+        for (int j = j_begin; j < j_end; ++j) {
             const int k0 = (w.first + j) * kPlainKeys, nk = min(kPlainKeys, w.len - k0);
             __syncthreads();                           // the block in front is done with keys, values and weights
             for (int i = tid; i < kPlainKeys * (vd + vv); i += kPlainThreads) {
@@ -98,7 +105,7 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
             __syncthreads();
             // softmax of the block, a warp per row
             for (int r = tid >> 5; r < rows; r += kPlainThreads / 32) {
-                const int pos = w.len - w.n + (row0 + r) / p.group;
+                const int pos = w.len - w.n + by_group(p, row0 + r);
                 float s[kPlainKeys / 32], m = M[r];
                 const float m_old = m;
 #pragma unroll
@@ -160,50 +167,51 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
             p.ml[((long long)slot * p.tile + tid) * 2] = M[tid];
             p.ml[((long long)slot * p.tile + tid) * 2 + 1] = L[tid];
         }
-        u += j_end - w.j;
     }
 }
 
 // ---- cut items ---------------------------------------------------------------------------------------------------
-// CTA x looks at the item that its namesake's range ends in: if that began there and goes on behind it, its parts are merged, a
-// warp per row, gridDim.y warps' rows side by side.  Maxima are in units of log2 where base2.
+// Block x merges the item that CTA x began and did not end, a warp per row.  Maxima are in units of log2 where base2.  Lanes take the
+// parts' maxima and sums, 32 at a time, then all of them the columns of one part after the other.
 template <typename T>
 __global__ void __launch_bounds__(128)
 paged_combine_kernel(const __grid_constant__ Paged p, int base2)
 {
     chain_enter();
-    extern __shared__ __align__(16) uint8_t sm[];
-    const Plan plan(sm, (int)p.a.batch);
-    make_plan(p, plan);
-    const int c = blockIdx.x, lane = threadIdx.x & 31, dv = p.a.dv;
-    const long long units = plan.before[p.a.batch], u0 = range_begin(units, c, p.grid), u1 = range_begin(units, c + 1, p.grid);
-    if (u0 >= u1) return;
+    const int c = blockIdx.x, lane = threadIdx.x & 31, dv = p.a.dv, parts = p.cut[c * 8];
+    if (parts == 0) return;
+    const int4 what = *(const int4*)(p.cut + c * 8), where = *(const int4*)(p.cut + c * 8 + 4);
     Walk w;
-    w.locate(p, plan, u1 - 1);
-    const long long begin = u1 - 1 - w.j, end = begin + w.count;
-    if (end <= u1 || begin < u0) return;
+    w.b = what.y; w.kv = what.z; w.t = what.w;
+    w.row0 = where.x; w.n = where.y; w.len = where.z;
     const int row0 = w.t * p.tile, rows = min(p.tile, w.n * p.group - row0);
-    for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += 4 * gridDim.y) {
-        float x[8] = {}, m = -INFINITY, l = 0.f;
-        for (int i = c; i < p.grid; ++i) {
-            if (i > c && range_begin(units, i, p.grid) >= end) break;
-            if (range_begin(units, i, p.grid) >= range_begin(units, i + 1, p.grid)) continue;
-            m = fmaxf(m, p.ml[((2ll * i + (i == c)) * p.tile + r) * 2]);
+    const int r = blockIdx.y * 4 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    float x[8] = {}, m = -INFINITY, l = 0.f;
+    auto place = [&](int i) { return (2ll * (c + i) + (i == 0)) * p.tile + r; };
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.ml[place(i) * 2]);
+    m = warp_max(m);
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        float f = 0.f;
+        if (i0 + lane < parts) {
+            const float2 ml = *(const float2*)(p.ml + place(i0 + lane) * 2);
+            // no key that the row sees: nothing, whatever the part's sums are
+            f = ml.x == -INFINITY ? 0.f : base2 ? exp2f(ml.x - m) : expf(ml.x - m);
+            l += ml.x == -INFINITY ? 0.f : f * ml.y;
         }
-        for (int i = c; i < p.grid; ++i) {
-            if (i > c && range_begin(units, i, p.grid) >= end) break;
-            if (range_begin(units, i, p.grid) >= range_begin(units, i + 1, p.grid)) continue;
-            const long long at = (2ll * i + (i == c)) * p.tile + r;
-            const float mi = p.ml[at * 2];
-            if (mi == -INFINITY) continue;             // no key that the row sees
-            const float f = base2 ? exp2f(mi - m) : expf(mi - m);
-            l = fmaf(f, p.ml[at * 2 + 1], l);
+        const unsigned some = __ballot_sync(0xffffffffu, f != 0.f);
+        const int n = min(parts - i0, 32);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float g = __shfl_sync(0xffffffffu, f, i);
+            if (!((some >> i) & 1)) continue;
+            const float* src = p.part + place(i0 + i) * dv + lane;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (lane + 32 * k < dv) x[k] = fmaf(f, p.part[at * dv + lane + 32 * k], x[k]);
+                if (lane + 32 * k < dv) x[k] = fmaf(g, src[32 * k], x[k]);
         }
-        finish_row<T>(p, w, row0 + r, x, l);
     }
+    finish_row<T>(p, w, row0 + r, x, warp_sum(l));
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
@@ -218,7 +226,7 @@ int plain_grid(const zkfp_paged_attention_args& a)
 template <typename T>
 int launch_combine(const Paged& p, int base2, cudaStream_t st)
 {
-    fp_launch(paged_combine_kernel<T>, dim3((unsigned)p.grid, (unsigned)(p.tile + 15) / 16), dim3(128), plan_bytes(p.a.batch), st, p, base2);
+    fp_launch(paged_combine_kernel<T>, dim3((unsigned)p.grid, (unsigned)(p.tile + 3) / 4), dim3(128), 0, st, p, base2);
     return fp_launched();
 }
 
@@ -237,12 +245,14 @@ int launch_plain(Paged& p, cudaStream_t st)
 void choose(Paged& p)
 {
     p.shift = page_shift(p.a.page);
-    p.group = p.a.heads / p.a.kv_heads;
+    set_group(p, p.a.heads / p.a.kv_heads);
     const int path = zkfp_paged_path(&p.a);
     if (path == 2) return paged_stream_shape(p);
     if (path == 1) return paged_tile_shape(p);
     p.tile = kPlainRows;
     p.block = kPlainKeys;
+    p.over = 0;
+    p.least = 1;
     p.grid = p.a.dtype == ZKFP_BF16 ? plain_grid<bf16>(p.a) : plain_grid<float>(p.a);
 }
 
@@ -250,7 +260,7 @@ bool paged_ok(const zkfp_paged_attention_args* a)
 {
     return a && a->q && a->k && a->v && a->out && a->table && a->rows && a->lengths && a->tokens >= 0 && a->pages > 0 && a->table_cols > 0 &&
            a->table_ld >= a->table_cols && a->batch > 0 && a->max_tokens >= 0 && a->kv_heads > 0 && a->heads > 0 &&
-           a->heads % a->kv_heads == 0 && a->d > 0 && a->dv > 0 && !(a->d & 7) && !(a->dv & 7) && page_shift(a->page) >= 0 && (unsigned)a->dtype <= 1 &&
+           a->heads % a->kv_heads == 0 && a->scale >= 0.f && a->scale < 3e38f && a->window >= 0 && !((uintptr_t)a->scratch & 15) && a->d > 0 && a->dv > 0 && !(a->d & 7) && !(a->dv & 7) && page_shift(a->page) >= 0 && (unsigned)a->dtype <= 1 &&
            !((a->q_tok | a->q_head | a->k_page | a->k_pos | a->k_head | a->v_page | a->v_pos | a->v_head | a->o_tok | a->o_head | a->gate_tok |
               a->gate_head) & 7) &&
            !(((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out | (uintptr_t)a->gate) & 15);
@@ -281,7 +291,7 @@ long long zkfp_paged_scratch(const zkfp_paged_attention_args* a)
     Paged p;
     p.a = *a;
     choose(p);
-    return 2ll * p.grid * p.tile * (a->dv + 2);
+    return 2ll * p.grid * p.tile * (a->dv + 2) + 8ll * p.grid;
 }
 
 int zkfp_paged_attention(const zkfp_paged_attention_args* a, void* stream)
@@ -295,6 +305,7 @@ int zkfp_paged_attention(const zkfp_paged_attention_args* a, void* stream)
     choose(p);
     p.part = a->scratch;
     p.ml = a->scratch + 2ll * p.grid * p.tile * a->dv;
+    p.cut = (int*)(p.ml + 4ll * p.grid * p.tile);
     p.error_flag = fp_error_flag();
     if (!p.error_flag) return ZKDS_ERR_WORKSPACE;
     cudaStream_t st = (cudaStream_t)stream;

@@ -25,18 +25,22 @@ __device__ __forceinline__ int sequence_of_row(const int* rows, int batch, long 
 
 // ---- attention over pages: how the work is shared ----------------------------------------------------------------
 // An item is a tile of query rows (token, head of a group, in this order) of one sequence and one key head; it takes a
-// number of units, blocks of keys from the first that any of its rows sees to the last.  All units in the order
-// sequence, key head, tile, block are cut into equal ranges, one per CTA, so that one long sequence among short ones,
-// a prompt among decoding sequences or a single sequence all keep every SM busy, and neither grid nor scratch depends on
+// number of units: `over` for what an item costs by itself (queries, sums, results), then blocks of keys from the first that any
+// of its rows sees to the last.  All units in the order sequence, key head, tile, block are cut into equal ranges, one
+// per CTA (fewer CTAs where a range would have less than `least`), so that one long sequence among short ones, a prompt
+// among decoding sequences or a single sequence all keep every SM busy, and neither grid nor scratch depends on
 // lengths that only the device knows.  An item that one CTA takes whole goes straight to `out`; of one that is cut, every CTA
 // leaves its sums, and paged_combine_kernel merges them in the order of the keys.  Results depend on lengths alone, not on timing.
 constexpr int kPagedBatch = 1024;
 
 struct Paged {
     zkfp_paged_attention_args a;
-    int shift, group, tile, block, grid;
+    int shift, group, tile, block, grid, over, least;
+    uint32_t group_mul;              // a division by `group`: the high bits of a product
+    int group_shift;
     float* part;                     // [2 * grid][tile][dv] weighted sums; first the item that began in front of a CTA's
     float* ml;                       // [2 * grid][tile][2] maximum, sum        range, then the one that ends behind it
+    int* cut;                        // [grid][8] the item that begins in a CTA's range and ends behind it
     int* error_flag;
 };
 
@@ -54,18 +58,33 @@ struct Plan {
 };
 inline size_t plan_bytes(long long batch) { return ((size_t)(batch + 1) * 8 + (size_t)batch * 12 + 15) & ~(size_t)15; }
 
+// x / group for x < 2^30 (the multiplier is 2^shift / group rounded up, its error times x below 2^shift)
+inline void set_group(Paged& p, int group)
+{
+    int s = 0;
+    while ((1 << s) < group) ++s;
+    p.group = group;
+    p.group_shift = 30 + s;
+    p.group_mul = (uint32_t)(((1ull << p.group_shift) + group - 1) / group);
+}
+__device__ __forceinline__ int by_group(const Paged& p, int x) { return (int)(((uint64_t)(uint32_t)x * p.group_mul) >> p.group_shift); }
+
 // blocks of keys that tile t of a sequence with n rows and len positions visits: first .. first + count - 1, one at least
 __device__ __forceinline__ void tile_blocks(const Paged& p, int n, int len, int t, int& first, int& count)
 {
     const int last_row = min((t + 1) * p.tile, n * p.group) - 1;
-    const int i0 = len - n + t * p.tile / p.group, i1 = len - n + last_row / p.group;
+    const int i0 = len - n + by_group(p, t * p.tile), i1 = len - n + by_group(p, last_row);
     if (i1 < 0) { first = 0; count = 1; return; }
     const int lo = p.a.window > 0 ? max(i0 - p.a.window + 1, 0) : 0;
     first = lo / p.block;
     count = i1 / p.block - first + 1;
 }
 
-__device__ __forceinline__ int tiles_of(const Paged& p, int n) { return (n * p.group + p.tile - 1) / p.tile; }
+__device__ __forceinline__ int tiles_of(const Paged& p, int n)
+{
+    const int rows = n * p.group;
+    return rows <= p.tile ? (rows > 0 ? 1 : 0) : (rows + p.tile - 1) / p.tile;
+}
 
 __device__ __forceinline__ long long warp_sum64(long long v)
 {
@@ -98,7 +117,7 @@ __device__ __forceinline__ void make_plan(const Paged& p, const Plan& s)
             for (int t = 0; t < tiles; ++t) {
                 int first, count;
                 tile_blocks(p, n, len, t, first, count);
-                units += count;
+                units += count + p.over;
             }
         for (unsigned left = __ballot_sync(0xffffffffu, tiles > 8); left; left &= left - 1) {
             const int who = __ffs(left) - 1, nn = __shfl_sync(0xffffffffu, n, who), ll = __shfl_sync(0xffffffffu, len, who);
@@ -106,7 +125,7 @@ __device__ __forceinline__ void make_plan(const Paged& p, const Plan& s)
             for (int t = lane; t < tiles_of(p, nn); t += 32) {
                 int first, count;
                 tile_blocks(p, nn, ll, t, first, count);
-                sum += count;
+                sum += count + p.over;
             }
             sum = warp_sum64(sum);
             if (lane == who) units = sum;
@@ -137,15 +156,24 @@ __device__ __forceinline__ void make_plan(const Paged& p, const Plan& s)
     __syncthreads();
 }
 
-__device__ __forceinline__ long long range_begin(long long units, int cta, int grid) { return units * cta / grid; }
+// CTAs that share the units
+__device__ __forceinline__ int sharing(const Paged& p, long long units)
+{
+    const long long most = units / p.least;
+    return most < 1 ? 1 : most < p.grid ? (int)most : p.grid;
+}
+__device__ __forceinline__ long long range_begin(long long units, int cta, int ctas)
+{
+    if (units < 0x200000) return (uint32_t)units * (uint32_t)cta / (uint32_t)ctas;      // ctas < 2048
+    return units * cta / ctas;
+}
 
 // one item and the part of it that starts at unit u; whole warps walk, every warp by itself
 struct Walk {
     int b, kv, t, tiles;             // sequence, key head, tile
-    int first, count, j;             // blocks of the item, and the one that u is
+    int first, count, at;            // blocks of the item, and which of its units (those for itself in front) u is
     int row0, n, len;
 
-    __device__ __forceinline__ void item(const Paged& p) { tile_blocks(p, n, len, t, first, count); }
     __device__ __forceinline__ void sequence(const Paged& p, const Plan& s)
     {
         row0 = s.row0[b]; n = s.n[b]; len = s.len[b];
@@ -167,9 +195,9 @@ struct Walk {
         rest -= kv * per;
         const int lane = threadIdx.x & 31;
         for (int t0 = 0;; t0 += 32) {                  // ends: rest < per, the sum of all tiles
-            int f = 0, c = 0;
+            int f = 0, c = -p.over;
             if (t0 + lane < tiles) tile_blocks(p, n, len, t0 + lane, f, c);
-            int sum = c;
+            int sum = c + p.over;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int w = __shfl_up_sync(0xffffffffu, sum, o);
@@ -179,7 +207,7 @@ struct Walk {
             if (past || t0 + 32 >= tiles) {
                 const int who = past ? __ffs(past) - 1 : 31;
                 t = t0 + who;
-                j = (int)rest - __shfl_sync(0xffffffffu, sum - c, who);
+                at = (int)rest - __shfl_sync(0xffffffffu, sum - c - p.over, who);
                 first = __shfl_sync(0xffffffffu, f, who);
                 count = __shfl_sync(0xffffffffu, c, who);
                 return;
@@ -187,9 +215,14 @@ struct Walk {
             rest -= __shfl_sync(0xffffffffu, sum, 31);
         }
     }
+    // units of the item from here on
+    __device__ __forceinline__ int left(const Paged& p) const { return p.over + count - at; }
+    // blocks of the item, from its first, in front of this unit and of the one `taken` further on
+    __device__ __forceinline__ int begin(const Paged& p) const { return max(at - p.over, 0); }
+    __device__ __forceinline__ int end(const Paged& p, int taken) const { return max(at + taken - p.over, 0); }
     __device__ __forceinline__ void next(const Paged& p, const Plan& s)
     {
-        j = 0;
+        at = 0;
         if (++t == tiles) {
             t = 0;
             if (++kv == p.a.kv_heads) {
@@ -200,9 +233,20 @@ struct Walk {
                 sequence(p, s);
             }
         }
-        item(p);
+        if (tiles > 1 || kv == 0) tile_blocks(p, n, len, t, first, count);      // else as for the key head in front
     }
 };
+
+// What paged_combine_kernel has to know of the item whose first block CTA `cta` takes and whose last one it does not: in how many
+// parts it was taken, 0 for none.  `end`: the unit behind the item's last.  One thread writes it, of every CTA of the grid.
+__device__ __forceinline__ void no_cut(const Paged& p, int cta) { p.cut[cta * 8] = 0; }
+__device__ __forceinline__ void write_cut(const Paged& p, int cta, long long units, int ctas, const Walk& w, long long end)
+{
+    const long long behind = min((end * ctas + units - 1) / units, (long long)ctas);      // the first CTA whose range begins behind it
+    int4* to = (int4*)(p.cut + cta * 8);
+    to[0] = make_int4((int)behind - cta, w.b, w.kv, w.t);
+    to[1] = make_int4(w.row0, w.n, w.len, 0);
+}
 
 // page of position j, or -1
 __device__ __forceinline__ long long page_of(const Paged& p, int b, int j)
@@ -264,7 +308,7 @@ __device__ __noinline__ void attend_row(const Paged& p, int b, int kv, int token
 template <typename T>
 __device__ __forceinline__ void finish_row(const Paged& p, const Walk& w, int row, float (&x)[8], float l)
 {
-    const int lane = threadIdx.x & 31, in_seq = row / p.group, head = w.kv * p.group + row - in_seq * p.group;
+    const int lane = threadIdx.x & 31, in_seq = by_group(p, row), head = w.kv * p.group + row - in_seq * p.group;
     const int token = w.row0 + in_seq, pos = w.len - w.n + in_seq;
     if (pos < 0) {
 #pragma unroll

@@ -40,6 +40,9 @@ __device__ __forceinline__ float exp2_approx(float x)
 constexpr int kStreamWarps = 4, kStretch = 16, kStreamRows = 16, kStreamKeys = kStreamWarps * kStretch, kStreamMost = 128;
 constexpr int kStretchSeg = kStretch * 128;            // bytes of 16 keys x 64 columns
 constexpr int kStreamStages = 4;
+// An item by itself costs about as much as 4 blocks of 64 keys, or 3 tiles of 128 (64 sequences up to 8192, microseconds, at 1, 2, 3, 4: 150,
+// 123, 107, 94; a chunk beside decoding sequences at 1, 3, 5: 221, 132, 137; a prompt 251, 206, 216).
+constexpr int kStreamOver = 4, kStreamLeast = 4, kTileOver = 3, kTileLeast = 3;
 
 struct StreamShape {
     int segk, segv, box, stages;
@@ -49,8 +52,9 @@ struct StreamShape {
         segk = (a.d + 63) / 64;
         segv = (a.dv + 63) / 64;
         box = a.page < kStretch ? a.page : kStretch;
-        const size_t fixed = 1024 + plan_bytes(a.batch) + (size_t)kStreamRows * (a.dv + 4) * 4 + 2 * kStreamRows * 4 + 256;
-        const size_t stage = (size_t)kStreamWarps * (segk + segv) * kStretchSeg, room = 112 * 1024 - fixed;
+        const size_t fixed = 1024 + plan_bytes(a.batch) + kStreamWarps * (kStreamStages * 8 + 2 * kStreamRows * 4 + 8) + 16;
+        const size_t load = (size_t)(segk + segv) * kStretchSeg, least = (size_t)segv * 4096;
+        const size_t stage = kStreamWarps * (load > least ? load : least), room = 112 * 1024 - fixed;
         stages = (int)(room / stage < kStreamStages ? room / stage : kStreamStages);
         smem = fixed + stages * stage;
     }
@@ -72,18 +76,85 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// the stretch of keys that a warp takes of a unit, and whether any row of the item sees some of it
-struct Stretch {
-    int k0;
-    bool seen;
-    __device__ __forceinline__ Stretch(const Paged& p, const Walk& w, int j, int warp)
+// A row of bfloat16 that did not come out finite, once more: its columns from `begin` to `end`.
+__device__ __noinline__ void finish_again(const Paged& p, int b, int kv, int token, int head, int pos, int begin, int end)
+{
+    const int lane = threadIdx.x & 31;
+    float x[8];
+    attend_row<bf16>(p, b, kv, token, head, pos, x);
+    bf16* out = (bf16*)p.a.out + (long long)token * p.a.o_tok + head * p.a.o_head;
+    const bf16* gate = p.a.gate ? (const bf16*)p.a.gate + (long long)token * p.a.gate_tok + head * p.a.gate_head : nullptr;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int c = lane + 32 * k;
+        if (c < begin || c >= end) continue;
+        if (gate) x[k] *= sigmoid_f(__bfloat162float(gate[c])) * p.a.out_scale;
+        out[c] = __float2bfloat16_rn(x[k]);
+    }
+}
+
+// Where a warp stands: the part of an item that the CTA takes, and the block of keys that comes next.
+struct Cursor {
+    Walk w;
+    long long u, item_end;           // behind this part; behind the item
+    int j, j_end, lo, hi;            // blocks of the part; the positions that any row of the item sees
+    bool begins, whole;
+
+    // the part that starts at u, or the next one that has blocks
+    __device__ __forceinline__ bool part(const Paged& p, const Plan& plan, long long u1)
     {
-        const int rows = min(p.tile, w.n * p.group - w.t * p.tile), base = w.len - w.n;
-        const int i0 = base + w.t * p.tile / p.group, i1 = base + (w.t * p.tile + rows - 1) / p.group;
-        k0 = (w.first + j) * kStreamKeys + warp * kStretch;
-        seen = k0 <= i1 && (p.a.window <= 0 || k0 + kStretch > i0 - p.a.window + 1);
+        for (;;) {
+            const int left = w.left(p), taken = (int)min((long long)left, u1 - u);
+            j = w.begin(p);
+            j_end = w.end(p, taken);
+            item_end = u + left;
+            u += taken;
+            if (j < j_end) break;
+            if (u >= u1) return false;
+            w.next(p, plan);
+        }
+        begins = j == 0;
+        whole = begins && j_end == w.count;
+        const int base = w.len - w.n, last_row = min((w.t + 1) * p.tile, w.n * p.group) - 1;
+        hi = base + by_group(p, last_row);
+        lo = p.a.window > 0 ? base + by_group(p, w.t * p.tile) - p.a.window + 1 : 0;
+        return true;
+    }
+    __device__ __forceinline__ bool next(const Paged& p, const Plan& plan, long long u1)
+    {
+        if (u >= u1) return false;
+        w.next(p, plan);
+        return part(p, plan, u1);
     }
 };
+
+// x[0 .. 3]: weighted sums of columns 4 lane .. 4 lane + 3 of a row, l the sum of its weights
+__device__ __forceinline__ void finish_four(const Paged& p, const Walk& w, int row, float (&x)[4], float l)
+{
+    const int lane = threadIdx.x & 31, in_seq = by_group(p, row), head = w.kv * p.group + row - in_seq * p.group;
+    const long long token = w.row0 + in_seq;
+    const bool mine = lane * 4 < p.a.dv, none = w.len - w.n + in_seq < 0;
+    const float r = none ? 0.f : 1.0f / l;
+    float z[4] = {};
+    if (p.a.gate && mine) {
+        const uint2 g = *(const uint2*)((const bf16*)p.a.gate + token * p.a.gate_tok + head * p.a.gate_head + lane * 4);
+        z[0] = bf16_lo(g.x); z[1] = bf16_hi(g.x); z[2] = bf16_lo(g.y); z[3] = bf16_hi(g.y);
+    }
+    bool finite = true;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        x[k] = none || !mine ? 0.f : x[k] * r;
+        finite = finite && isfinite(x[k]);
+        if (p.a.gate) x[k] *= sigmoid_for<bf16>(z[k]) * p.a.out_scale;
+    }
+    if (!__all_sync(0xffffffffu, finite)) {
+        finish_again(p, w.b, w.kv, (int)token, head, w.len - w.n + in_seq, 0, p.a.dv);
+        return;
+    }
+    if (mine)
+        *(uint2*)((bf16*)p.a.out + token * p.a.o_tok + head * p.a.o_head + lane * 4) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
 
 template <int SEGK, int SEGV>
 __global__ void __launch_bounds__(kStreamWarps * 32, 2)
@@ -93,114 +164,122 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     extern __shared__ uint8_t raw[];
     chain_enter();
     const zkfp_paged_attention_args& a = p.a;
+    constexpr uint32_t kLoad = (SEGK + SEGV) * kStretchSeg, kStage = kLoad > SEGV * 4096 ? kLoad : SEGV * 4096;      // also room for 16 rows of sums
+    constexpr int kPitch = SEGV * 64;
     uint8_t* ring = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = (int)a.batch, dv = a.dv, pitch = dv + 4;
-    constexpr uint32_t kStage = (SEGK + SEGV) * kStretchSeg;
-    uint8_t* behind = ring + kStreamWarps * stages * kStage;
-    uint64_t* bars = (uint64_t*)behind;                        // [warp][stage]
-    float* M = (float*)(bars + kStreamWarps * kStreamStages);
-    float *L = M + kStreamRows, *O = L + kStreamRows;
-    int* gave_up = (int*)(O + kStreamRows * pitch);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, batch = (int)a.batch, dv = a.dv;
+    uint64_t* bars = (uint64_t*)(ring + kStreamWarps * stages * kStage);           // [warp][stage]
+    float* M = (float*)(bars + kStreamWarps * kStreamStages);                      // [warp][row], and the sums of weights
+    float* L = M + kStreamWarps * kStreamRows;
+    const uint8_t** sums = (const uint8_t**)(L + kStreamWarps * kStreamRows);      // where a warp left its rows
+    int* gave_up = (int*)(sums + kStreamWarps);
     const Plan plan((uint8_t*)(gave_up + 4), batch);
     volatile int* abort_flag = gave_up;
     if (threadIdx.x == 0) {
         *gave_up = 0;
+        no_cut(p, blockIdx.x);
         for (int i = 0; i < kStreamWarps * stages; ++i) mbar_init(smem_u32(bars + i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     make_plan(p, plan);
-    const long long units = plan.before[batch], u1 = range_begin(units, blockIdx.x + 1, p.grid);
-    long long u = range_begin(units, blockIdx.x, p.grid), ui = u;
-    if (u >= u1) return;
-    const uint32_t one = elect_one(), my_ring = smem_u32(ring) + warp * stages * kStage, my_bars = smem_u32(bars + warp * stages);
-    Walk w, wi;
-    w.locate(p, plan, u);
-    wi = w;
-    int ji = wi.j, slot_i = 0, slot = 0;
+    const long long units = plan.before[batch];
+    const int ctas = sharing(p, units), cta = blockIdx.x;
+    if (cta >= ctas || units == 0) return;
+    const long long u1 = range_begin(units, cta + 1, ctas);
+    const uint32_t one = elect_one(), my_bars = smem_u32(bars + warp * stages);
+    uint8_t* my_ring = ring + warp * stages * kStage;
+    Cursor at;
+    at.u = range_begin(units, cta, ctas);
+    at.w.locate(p, plan, at.u);
+    bool more = at.part(p, plan, u1), loads = more, ok = true;
+    Cursor in = at;                                            // the loads, as far ahead as the ring holds
+    int slot_in = 0, slot = 0, ahead = 0;
     uint32_t phase = 0;
-    // pages of the next 32 stretches of the item that is being loaded: lane i holds that of unit base + i
+    // pages of the next 32 stretches of the item that is being loaded: lane i holds that of block base + i
     int page_base = -1, page_id = 0, page_id2 = 0;
-    auto issue = [&] {
-        if (ui >= u1) return;
-        const Stretch st(p, wi, ji, warp);
-        if (page_base < 0 || ji >= page_base + 32) {
-            page_base = ji;
-            const int j = ji + lane;
-            page_id = page_id2 = (int)a.pages;                 // beyond the tensor: the tile is filled with zeros
-            if (j < wi.count) {
-                const int k = (wi.first + j) * kStreamKeys + warp * kStretch;
-                bool bad = false;
-                if (k < wi.len) {
-                    const long long page = page_of(p, wi.b, k);
-                    if (page >= 0) page_id = (int)page;
-                    else bad = true;
-                }
-                if (box < kStretch && k + 8 < wi.len) {
-                    const long long page = page_of(p, wi.b, k + 8);
-                    if (page >= 0) page_id2 = (int)page;
-                    else bad = true;
-                }
-                if (bad) *(volatile int*)p.error_flag = 1;
+    auto fill = [&] {
+        while (loads && ahead < stages) {
+            if (in.j == in.j_end) {
+                loads = in.next(p, plan, u1);
+                page_base = -1;
+                continue;
             }
-        }
-        if (st.seen) {
-            const int page = __shfl_sync(0xffffffffu, page_id, ji - page_base), page2 = __shfl_sync(0xffffffffu, page_id2, ji - page_base);
-            const uint32_t bar = my_bars + slot_i * 8, dst = my_ring + slot_i * kStage;
-            const int line = st.k0 & (a.page - 1);
-            mbar_expect_tx(bar, kStage, one);
+            const int k0 = (in.w.first + in.j) * kStreamKeys + warp * kStretch;
+            if (k0 > in.hi || k0 + kStretch <= in.lo) {        // a stretch that no row sees takes no place
+                ++in.j;
+                continue;
+            }
+            if (page_base < 0 || in.j >= page_base + 32) {
+                page_base = in.j;
+                const int j = in.j + lane;
+                page_id = page_id2 = (int)a.pages;             // beyond the tensor: the tile is filled with zeros
+                if (j < in.j_end) {
+                    const int k = (in.w.first + j) * kStreamKeys + warp * kStretch;
+                    bool bad = false;
+                    if (k < in.w.len) {
+                        const long long page = page_of(p, in.w.b, k);
+                        if (page >= 0) page_id = (int)page;
+                        else bad = true;
+                    }
+                    if (box < kStretch && k + 8 < in.w.len) {
+                        const long long page = page_of(p, in.w.b, k + 8);
+                        if (page >= 0) page_id2 = (int)page;
+                        else bad = true;
+                    }
+                    if (bad) *(volatile int*)p.error_flag = 1;
+                }
+                __syncwarp();
+            }
+            const int page = __shfl_sync(0xffffffffu, page_id, in.j - page_base), page2 = __shfl_sync(0xffffffffu, page_id2, in.j - page_base);
+            const uint32_t bar = my_bars + slot_in * 8, dst = smem_u32(my_ring) + slot_in * kStage;
+            const int line = k0 & (a.page - 1);
+            mbar_expect_tx(bar, kLoad, one);
 #pragma unroll
             for (int c = 0; c < SEGK + SEGV; ++c) {
                 const CUtensorMap* map = c < SEGK ? &tmK : &tmV;
                 const int x = (c < SEGK ? c : c - SEGK) * 64;
-                tma_load_4d(dst + c * kStretchSeg, map, x, wi.kv, line, page, bar, one);
-                if (box < kStretch) tma_load_4d(dst + c * kStretchSeg + 1024, map, x, wi.kv, 0, page2, bar, one);
+                tma_load_4d(dst + c * kStretchSeg, map, x, in.w.kv, line, page, bar, one);
+                if (box < kStretch) tma_load_4d(dst + c * kStretchSeg + 1024, map, x, in.w.kv, 0, page2, bar, one);
             }
-            if (++slot_i == stages) slot_i = 0;
-        }
-        ++ui;
-        if (++ji == wi.count && ui < u1) {
-            wi.next(p, plan);
-            ji = 0;
-            page_base = -1;
-        }
-    };
-    // a stretch that no row sees takes no place in the ring: as many are on their way as the ring holds
-    auto loads = [&](const Walk& at, int j) { return Stretch(p, at, j, warp).seen; };
-    int ahead = 0;
-    auto fill = [&] {
-        while (ui < u1 && ahead < stages) {
-            ahead += loads(wi, ji) ? 1 : 0;
-            issue();
+            if (++slot_in == stages) slot_in = 0;
+            ++ahead;
+            ++in.j;
         }
     };
     fill();
-    bool ok = true;
-    for (; u < u1;) {
-        const int j_end = (int)min((long long)w.count, w.j + (u1 - u));
-        const bool whole = w.j == 0 && j_end == w.count;
-        const int row0 = w.t * p.tile, rows = min(p.tile, w.n * p.group - row0), r = lane >> 2, cq = (lane & 3) * 2;
+    const int r = lane >> 2, cq = (lane & 3) * 2;
+    const float scale = a.scale * kLog2e;
+    for (; more; more = at.next(p, plan, u1)) {
+        const Walk& w = at.w;
+        const int row0 = w.t * p.tile, rows = min(p.tile, w.n * p.group - row0), halves = rows > 8 ? 2 : 1;
+        if (threadIdx.x == 0 && at.begins && !at.whole) write_cut(p, cta, units, ctas, w, at.item_end);
         // queries: rows r and r + 8, elements cq, cq + 1 and eight further on of every 16
         uint32_t q[SEGK * 4][4];
-        int pos[2];
+        int pos[2] = {-1, -1};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int rr = row0 + r + 8 * h, t = rr / p.group, head = w.kv * p.group + rr - t * p.group;
-            const bool in = r + 8 * h < rows;
-            pos[h] = in ? w.len - w.n + t : -1;
-            const bf16* src = (const bf16*)a.q + (long long)(w.row0 + t) * a.q_tok + head * a.q_head;
+#pragma unroll
+            for (int k = 0; k < SEGK * 4; ++k) q[k][h] = q[k][h + 2] = 0u;
+            if (h >= halves) break;
+            const int rr = row0 + r + 8 * h, t = by_group(p, rr), head = w.kv * p.group + rr - t * p.group;
+            if (r + 8 * h >= rows) continue;
+            pos[h] = w.len - w.n + t;
+            const bf16* src = (const bf16*)a.q + (long long)(w.row0 + t) * a.q_tok + head * a.q_head + cq;
 #pragma unroll
             for (int k = 0; k < SEGK * 4; ++k) {
-                const int c = k * 16 + cq;
-                q[k][h] = in && c < a.d ? *(const uint32_t*)(src + c) : 0u;
-                q[k][h + 2] = in && c + 8 < a.d ? *(const uint32_t*)(src + c + 8) : 0u;
+                if (k * 16 < a.d) q[k][h] = *(const uint32_t*)(src + k * 16);
+                if (k * 16 + 8 < a.d) q[k][h + 2] = *(const uint32_t*)(src + k * 16 + 8);
             }
         }
+        const int low_pos = w.len - w.n + by_group(p, row0), all_lo = a.window > 0 ? at.hi - a.window : -1;
         float o[SEGV * 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
-        const float scale = a.scale * kLog2e;
-        for (int j = w.j; j < j_end; ++j, ++u) {
-            const Stretch st(p, w, j, warp);
-            if (!st.seen) continue;
-            const uint32_t tile = my_ring + slot * kStage;
+        uint8_t* mine = nullptr;                               // the place read last
+        for (int j = at.j; j < at.j_end; ++j) {
+            const int k0 = (w.first + j) * kStreamKeys + warp * kStretch;
+            if (k0 > at.hi || k0 + kStretch <= at.lo) continue;
+            fill();
+            mine = my_ring + slot * kStage;
+            const uint32_t tile = smem_u32(mine);
             if (ok) ok = mbar_wait_warp(my_bars + slot * 8, phase, abort_flag);
             float s[2][4] = {};
 #pragma unroll
@@ -215,35 +294,34 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 }
             }
             // s[t][2 h + e]: row r + 8 h, key k0 + 8 t + cq + e
-            float f[2];
+            const bool edge = k0 + kStretch - 1 > low_pos || k0 <= all_lo;         // some row does not see all of them
+            float f[2] = {1.f, 1.f};
+            uint32_t pa[4] = {};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float top = -INFINITY;
-                const int lo = a.window > 0 ? pos[h] - a.window : -1;
+                if (h >= halves) break;
+                if (edge) {
+                    const int lo = a.window > 0 ? pos[h] - a.window : -1;
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int key = st.k0 + 8 * t + cq + e;
-                        float& x = s[t][2 * h + e];
-                        x = key <= pos[h] && key > lo ? x * scale : -INFINITY;
-                        top = fmaxf(top, x);
-                    }
+                        for (int e = 0; e < 2; ++e) {
+                            const int key = k0 + 8 * t + cq + e;
+                            if (key > pos[h] || key <= lo) s[t][2 * h + e] = -INFINITY;
+                        }
+                }
+                float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float m_new = fmaxf(m[h], top), m_sub = m_new == -INFINITY ? 0.f : m_new;
+                const float m_new = fmaxf(m[h], top * scale), m_sub = m_new == -INFINITY ? 0.f : m_new;
                 f[h] = exp2_approx(m[h] - m_sub);
                 m[h] = m_new;
-                float sum = 0.f;
+                float e[4];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = s[t][2 * h + e];
-                        x = exp2_approx(x - m_sub);
-                        sum += x;
-                    }
-                l[h] = l[h] * f[h] + sum;
+                for (int i = 0; i < 4; ++i) e[i] = exp2_approx(fmaf(s[i >> 1][2 * h + (i & 1)], scale, -m_sub));
+                l[h] = fmaf(l[h], f[h], (e[0] + e[1]) + (e[2] + e[3]));
+                pa[h] = pack_bf16(e[0], e[1]);
+                pa[h + 2] = pack_bf16(e[2], e[3]);
             }
             if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
@@ -252,16 +330,12 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     o[c][2] *= f[1]; o[c][3] *= f[1];
                 }
             }
-            if (st.k0 + kStretch > w.len) {                    // lines that the sequence does not hold: no value, whatever is there
-                for (int i = lane; i < SEGV * 128; i += 32) {
-                    const int c = i >> 7, line = (i >> 3) & 15;
-                    if (st.k0 + line >= w.len)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (SEGK + c) * kStretchSeg + (i & 127) * 16), "r"(0) : "memory");
-                }
+            if (k0 + kStretch > w.len) {                       // lines that the sequence does not hold: no value, whatever is there
+                for (int i = lane; i < SEGV * 128; i += 32)
+                    if (k0 + ((i >> 3) & 15) >= w.len) *(uint4*)(mine + (SEGK + (i >> 7)) * kStretchSeg + (i & 127) * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
-            const uint32_t pa[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
 #pragma unroll
             for (int c = 0; c < SEGV * 4; ++c) {
                 uint32_t b[4];
@@ -273,69 +347,55 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             __syncwarp();                                      // every lane has read the tile
             --ahead;
             if (++slot == stages) { slot = 0; phase ^= 1u; }
-            fill();
         }
+        // The warps' sums meet in the places that they have read last, eight columns at a time turned by the row so that no two rows
+        // of a store fall on one bank; a warp that had no keys stays out.
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        }
-        // the warps' sums, one after the other
-        for (int i = 0; i < kStreamWarps; ++i) {
-            __syncthreads();
-            if (warp != i) continue;
-            float mine[2] = {1.f, 1.f}, theirs[2] = {};
-            if (i) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float mo = M[r + 8 * h], top = fmaxf(mo, m[h]);
-                    mine[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - top);
-                    theirs[h] = mo == -INFINITY ? 0.f : exp2_approx(mo - top);
-                    l[h] = l[h] * mine[h] + L[r + 8 * h] * theirs[h];
-                    m[h] = top;
-                }
-                __syncwarp();
+            if (h >= halves) break;
+            if ((lane & 3) == 0) {
+                M[warp * kStreamRows + r + 8 * h] = m[h];
+                L[warp * kStreamRows + r + 8 * h] = l[h];
             }
+            if (mine)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int rr = r + 8 * h;
-                if ((lane & 3) == 0) { M[rr] = m[h]; L[rr] = l[h]; }
-                if (rr >= rows) continue;
-#pragma unroll
-                for (int c = 0; c < SEGV * 8; ++c) {
-                    if (c * 8 + cq >= dv) continue;
-                    float2* at = (float2*)(O + rr * pitch + c * 8 + cq);
-                    float2 x = make_float2(o[c][2 * h] * mine[h], o[c][2 * h + 1] * mine[h]);
-                    if (theirs[h] != 0.f) {
-                        const float2 y = *at;
-                        x.x = fmaf(y.x, theirs[h], x.x);
-                        x.y = fmaf(y.y, theirs[h], x.y);
-                    }
-                    *at = x;
-                }
-            }
+                for (int c = 0; c < SEGV * 8; ++c)
+                    *(float2*)(mine + ((r + 8 * h) * kPitch + ((c ^ r) * 8) + cq) * 4) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
         }
+        if (lane == 0) sums[warp] = mine;
         __syncthreads();
-        const int part = 2 * blockIdx.x + (w.j == 0 ? 1 : 0);
         for (int rr = warp; rr < rows; rr += kStreamWarps) {
-            float x[8];
+            float top = -INFINITY, sum = 0.f, x[4] = {};
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = lane + 32 * k < dv ? O[rr * pitch + lane + 32 * k] : 0.f;
-            if (whole) {
-                finish_row<bf16>(p, w, row0 + rr, x, L[rr]);
+            for (int i = 0; i < kStreamWarps; ++i) top = fmaxf(top, M[i * kStreamRows + rr]);
+#pragma unroll
+            for (int i = 0; i < kStreamWarps; ++i) {
+                const float mi = M[i * kStreamRows + rr];
+                if (mi == -INFINITY) continue;
+                const float g = exp2_approx(mi - top);
+                sum = fmaf(g, L[i * kStreamRows + rr], sum);
+                if (lane * 4 < kPitch) {
+                    const float4 y = *(const float4*)(sums[i] + (rr * kPitch + (((lane >> 1) ^ (rr & 7)) * 8) + (lane & 1) * 4) * 4);
+                    x[0] = fmaf(g, y.x, x[0]); x[1] = fmaf(g, y.y, x[1]);
+                    x[2] = fmaf(g, y.z, x[2]); x[3] = fmaf(g, y.w, x[3]);
+                }
+            }
+            if (at.whole) {
+                finish_four(p, w, row0 + rr, x, sum);
                 continue;
             }
-            float* to = p.part + ((long long)part * p.tile + rr) * dv;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (lane + 32 * k < dv) to[lane + 32 * k] = x[k];
-            if (lane < 2) p.ml[((long long)part * p.tile + rr) * 2 + lane] = lane ? L[rr] : M[rr];
+            const long long to = (2ll * cta + (at.begins ? 1 : 0)) * p.tile + rr;
+            if (lane * 4 < dv) *(float4*)(p.part + to * dv + lane * 4) = make_float4(x[0], x[1], x[2], x[3]);
+            if (lane == 0) *(float2*)(p.ml + to * 2) = make_float2(top, sum);
         }
-        if (u < u1) w.next(p, plan);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");               // the places are loaded into again
+        __syncthreads();
+        fill();
     }
     if (!ok) *(volatile int*)p.error_flag = 1;
 }
-
 
 // ---- many rows ---------------------------------------------------------------------------------------------------
 constexpr int kTile = 128;                     // query rows and keys per tile
@@ -362,41 +422,30 @@ struct TileShared {
 // takes part in, and the rows of g.
 struct Part {
     int begin, end, row0[2], rows[2], first[2], last[2];
+    int taken;                                 // units of the item, those for itself among them
+    bool begins, whole;
     __device__ __forceinline__ Part(const TileParams& t, const Walk& w, long long left)
     {
         const int all = w.n * t.p.group, base = w.len - w.n;
-        begin = w.first + w.j;
-        end = w.first + (int)min((long long)w.count, w.j + left);
+        taken = (int)min((long long)w.left(t.p), left);
+        begin = w.begin(t.p);
+        end = w.end(t.p, taken);
+        begins = begin == 0;
+        whole = begins && end == w.count;
+        begin += w.first;
+        end += w.first;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             row0[g] = w.t * t.p.tile + g * t.rows;
             rows[g] = max(0, min(t.rows, all - row0[g]));
-            const int i0 = base + row0[g] / t.p.group, i1 = base + (row0[g] + rows[g] - 1) / t.p.group;
+            const int i0 = base + by_group(t.p, row0[g]), i1 = rows[g] > 0 ? base + by_group(t.p, row0[g] + rows[g] - 1) : -1;
             const int lo = t.p.a.window > 0 ? max(i0 - t.p.a.window + 1, 0) / kTile : 0;
             first[g] = max(begin, lo);
-            last[g] = rows[g] > 0 && i1 >= 0 ? min(end - 1, i1 / kTile) : first[g] - 1;
+            last[g] = i1 >= 0 ? min(end - 1, i1 / kTile) : first[g] - 1;
         }
     }
     __device__ __forceinline__ bool active(int g, int j) const { return g ? j >= first[1] && j <= last[1] : j >= first[0] && j <= last[0]; }
 };
-
-// A row of bfloat16 that did not come out finite, once more: its columns from `begin` to `end`.
-__device__ __noinline__ void finish_again(const Paged& p, const Walk& w, int row, int in_seq, int begin, int end)
-{
-    const int lane = threadIdx.x & 31, head = w.kv * p.group + row - in_seq * p.group, token = w.row0 + in_seq;
-    float x[8];
-    attend_row<bf16>(p, w.b, w.kv, token, head, w.len - w.n + in_seq, x);
-    bf16* out = (bf16*)p.a.out + (long long)token * p.a.o_tok + head * p.a.o_head;
-    const bf16* gate = p.a.gate ? (const bf16*)p.a.gate + (long long)token * p.a.gate_tok + head * p.a.gate_head : nullptr;
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int c = lane + 32 * k;
-        if (c < begin || c >= end) continue;
-        if (gate) x[k] *= sigmoid_f(__bfloat162float(gate[c])) * p.a.out_scale;
-        out[c] = __float2bfloat16_rn(x[k]);
-    }
-}
 
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -439,18 +488,24 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s.tmem;
-    const long long units = plan.before[a.batch], u1 = range_begin(units, blockIdx.x + 1, p.grid);
-    long long u = range_begin(units, blockIdx.x, p.grid);
+    const long long units = plan.before[a.batch];
+    const int ctas = sharing(p, units), cta = blockIdx.x;
+    const bool works = cta < ctas && units > 0;
+    long long u = works ? range_begin(units, cta, ctas) : 0;
+    const long long u1 = works ? range_begin(units, cta + 1, ctas) : 0;
     Walk w;
-    if (u < u1) w.locate(p, plan, u);
+    if (works) w.locate(p, plan, u);
 
     if (warp == 0) {
         const uint32_t one = elect_one();
         int ks = 0, vs = 0;
         uint32_t kp = 0, vp = 0, qp = 0;
         bool ok = true;
+        if (one) no_cut(p, cta);
         while (u < u1 && ok) {
             const Part part(t, w, u1 - u);
+            if (part.begin == part.end) break;                 // units of an item that others take
+            if (one && part.begins && !part.whole) write_cut(p, cta, units, ctas, w, u + w.left(p));
             if (!(ok = mbar_wait_warp(smem_u32(&s.q_empty), qp ^ 1u, abort_flag))) break;
             qp ^= 1u;
             const uint32_t row_bytes = (uint32_t)t.rows * 128u;
@@ -459,7 +514,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             for (int g = 0; g < 2; ++g)
                 if (part.rows[g] > 0)
                     for (int c = 0; c < t.seg; ++c)
-                        tma_load_4d(sQ + g * bytesQ + c * kSeg, &tmQ, c * 64, 0, w.kv, w.row0 + part.row0[g] / p.group, smem_u32(&s.q_full), one);
+                        tma_load_4d(sQ + g * bytesQ + c * kSeg, &tmQ, c * 64, 0, w.kv, w.row0 + by_group(p, part.row0[g]), smem_u32(&s.q_full), one);
             for (int j = part.begin; j < part.end && ok; ++j) {
                 // pages of this tile of keys: lane i holds that of its i-th box
                 int mine = (int)a.pages;                       // beyond the tensor: zeros
@@ -487,7 +542,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         tma_load_4d(dst + c * kSeg + i * t.box * 128, &tmV, c * 64, w.kv, line, __shfl_sync(0xffffffffu, mine, i), bar, one);
                 if (++vs == t.v_stages) { vs = 0; vp ^= 1u; }
             }
-            u += part.end - part.begin;
+            u += part.taken;
             if (u < u1) w.next(p, plan);
         }
     } else if (warp == 1) {
@@ -498,6 +553,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         bool ok = true;
         while (u < u1 && ok) {
             Part part(t, w, u1 - u);
+            if (part.begin == part.end) break;
             part.begin = (int)uniform(part.begin);
             part.end = (int)uniform(part.end);
 #pragma unroll
@@ -563,7 +619,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (!ok) break;
                 if (j >= part.begin && ++vs == t.v_stages) { vs = 0; vp ^= 1u; }
             }
-            u += part.end - part.begin;
+            u += part.taken;
             if (u < u1) w.next(p, plan);
         }
     } else {
@@ -576,9 +632,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         bool ok = true;
         while (u < u1 && ok) {
             const Part part(t, w, u1 - u);
-            const bool whole = w.j == 0 && part.end - part.begin == w.count;
+            if (part.begin == part.end) break;
             const int rows = part.rows[g], first_tile = part.first[g], last_tile = part.last[g], row_all = part.row0[g] + row;
-            const int in_seq = row_all / p.group, pos = row < rows ? w.len - w.n + in_seq : -1;
+            const int in_seq = by_group(p, row_all), pos = row < rows ? w.len - w.n + in_seq : -1;
             float m_used = -INFINITY, l = 0.f;
             for (int j = first_tile; j <= last_tile && ok; ++j) {
                 if (!(ok = mbar_wait_warp(smem_u32(&s.s_full[g]), sp, abort_flag))) break;
@@ -655,7 +711,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
             const int head = w.kv * p.group + row_all - in_seq * p.group;
             const long long token = w.row0 + in_seq;
-            if (whole) {
+            if (part.whole) {
                 const float r = pos >= 0 ? 1.0f / l : 0.f;
                 bf16* out = (bf16*)a.out + token * a.o_tok + head * a.o_head;
                 const bf16* gate = a.gate ? (const bf16*)a.gate + token * a.gate_tok + head * a.gate_head : nullptr;
@@ -684,11 +740,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     __syncwarp();
                 }
                 for (unsigned again = __ballot_sync(0xffffffffu, !finite); again; again &= again - 1) {
-                    const int who = __ffs(again) - 1, rr = part.row0[g] + quarter * 32 + who, tok = rr / p.group;
-                    finish_again(p, w, rr, tok, o_begin, o_end);
+                    const int who = __ffs(again) - 1, rr = part.row0[g] + quarter * 32 + who, tok = by_group(p, rr);
+                    finish_again(p, w.b, w.kv, w.row0 + tok, w.kv * p.group + rr - tok * p.group, w.len - w.n + tok, o_begin, o_end);
                 }
             } else {
-                const long long at = (2ll * blockIdx.x + (w.j == 0 ? 1 : 0)) * p.tile + g * t.rows + row;
+                const long long at = (2ll * cta + (part.begins ? 1 : 0)) * p.tile + g * t.rows + row;
                 for (int c = o_begin; c < o_end; c += 8) {
                     int32_t x[8] = {};
                     if (any) {
@@ -710,7 +766,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s.o_empty[g]));
             }
-            u += part.end - part.begin;
+            u += part.taken;
             if (u < u1) w.next(p, plan);
         }
     }
@@ -769,6 +825,8 @@ void paged_stream_shape(Paged& p)
     p.tile = kStreamRows;
     p.block = kStreamKeys;
     p.grid = 2 * fp_sm_count();
+    p.over = kStreamOver;
+    p.least = kStreamLeast;
 }
 
 template <int SEGK, int SEGV>
@@ -791,6 +849,8 @@ void paged_tile_shape(Paged& p)
     p.tile = 2 * TileShape(p.a).rows;
     p.block = kTile;
     p.grid = fp_sm_count();
+    p.over = kTileOver;
+    p.least = kTileLeast;
 }
 
 int launch_paged_tile(const Paged& p, cudaStream_t st)

@@ -391,8 +391,8 @@ def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, windo
         _refuse(what, "head sizes %d and %d are no multiples of 8" % (d, dv))
     qs, os = _heads(what, "q", q, dt, dev, (tokens, heads, d)), _heads(what, "out", out, dt, dev, (tokens, heads, dv))
     gs = _heads(what, "gate", gate, dt, dev, (tokens, heads, dv)) if gate is not None else (0, 0)
-    if window < 0 or (max_tokens is not None and max_tokens < 0):
-        _refuse(what, "a negative window or bound")
+    if window < 0 or (max_tokens is not None and max_tokens < 0) or not 0 <= scale < 3e38:
+        _refuse(what, "a negative window, bound or scale")
     a = PagedAttentionArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ptr(gate), table.data_ptr(),
                            rows.data_ptr(), lengths.data_ptr(), None, *qs, *ks, *vs, *os, *gs, tokens, k_pages.shape[0], table.shape[1],
                            ld, table.shape[0], tokens if max_tokens is None else max_tokens, heads, kv, d, dv, k_pages.shape[1],
