@@ -1,232 +1,433 @@
 // One token per row of logits from given random numbers: temperature, the k largest, the likeliest p, at least min_p.
 //
-// Weights are w = 2^((l - max) log2(e) / temperature), held as whole multiples of 2^-44: their sums are exact in any order,
-// so that neither the threads' timing nor the shape of the launch moves a border between two tokens.  2^y is made in 64
-// bits: y by one product, 2^y from a table of 2^(i / 256) and the series of 2^r, |r| <= 1 / 512, to its fifth term (the sixth
-// is 2^-57 of it).
+// Weights are w = 2^((l - max) log2(e) / temperature), held as whole multiples of 2^-44: their sums are exact in any order, so
+// that neither the threads' timing nor the shape of the launch moves a border between two tokens.  2^y is made in 64 bits: y
+// by one product, 2^y from a table of 2^(i / 256) and the series of 2^r, |r| <= 1 / 512, to its fourth power (the fifth is 2^-54).
 //
-// What a row keeps is a prefix of its tokens in falling order of (logit, then rising index): the threshold is found on the logits'
-// bits, ordered as whole numbers, 8 of 32 bits at a time: how many tokens, or how much weight, lies in each of the 256
-// continuations of the bits found so far.
+// A row belongs to a cluster of 1 to 8 CTAs, each of which keeps its slice of the row in shared memory as keys (the logits' bits in the
+// order of whole numbers), so the row is read from memory once.  What a row keeps is a prefix of its tokens in falling order of rank:
+// the key, then the lower index.  The prefix's last token is found in two steps: a histogram of 2048 equal stretches
+// between the smallest and the largest logit, of counts or of weights, names the stretch that it lies in; the tokens of that
+// stretch, a few hundred at most on logits of a model, meet in the first CTA, which ranks them.  Where they are more than its list
+// holds (logits that are equal, or nearly), the key is found 8 bits at a time instead.
+#include <cooperative_groups.h>
+
 #include "float_common.cuh"
 
 namespace zkds {
 
 namespace {
 
-constexpr int kSampleThreads = 512;
-constexpr double kWeightOne = 17592186044416.0;        // 2^44
+namespace cg = cooperative_groups;
 
-// larger logits have larger keys; NaN the key of -infinity
+constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32, kStretches = 2048, kListed = 1024, kClusterMost = 8;
+
+// larger logits have larger keys; NaN has the key of -infinity, both zeros the same
 __device__ __forceinline__ uint32_t key_of(float l)
 {
     if (l != l) l = -INFINITY;
-    if (l == 0.f) l = 0.f;                             // both zeros are equal
-    const uint32_t u = __float_as_uint(l);
+    const uint32_t u = __float_as_uint(l + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float logit_of(uint32_t key)
 {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+__device__ __forceinline__ uint64_t rank_of(uint32_t key, uint32_t index) { return (uint64_t)key << 32 | (uint32_t)~index; }
 
 struct Weigher {
-    const double* table;             // 2^(i / 256) 2^44
-    double top, scale;
+    const double* table;             // 2^(i / 256)
+    double top, scale;               // scale: 256 log2(e) / temperature
+    uint32_t best;
     bool infinite;                   // the largest logit is: its like have weight 1, all others none
-    __device__ __forceinline__ double exponent(float l) const
+    // 256 times the exponent
+    __device__ __forceinline__ double exponent(uint32_t key) const
     {
-        return infinite ? (l == INFINITY ? 0.0 : -100.0) : ((double)l - top) * scale;
+        if (infinite) return key == best ? 0.0 : -1e6;
+        return ((double)logit_of(key) - top) * scale;
     }
     __device__ __forceinline__ uint64_t operator()(uint32_t key) const
     {
-        const double y = exponent(logit_of(key));
-        if (!(y > -46.0)) return 0;
-        const double n = rint(y * 256.0);
-        const double r = (y - n * 0.00390625) * 0.6931471805599453;
-        const int i = (int)n;
-        const double e = 1.0 + r * (1.0 + r * (0.5 + r * (1.0 / 6 + r * (1.0 / 24 + r * (1.0 / 120)))));
-        return (uint64_t)(ldexp(table[i & 255] * e, i >> 8) + 0.5);
+        const double y = exponent(key);
+        if (!(y > -46.0 * 256)) return 0;
+        const double magic = 6755399441055744.0;       // 1.5 * 2^52: adding it rounds to a whole number, in the low bits
+        const double n = y + magic;
+        const int i = (int)__double_as_longlong(n);
+        const double r = (y - (n - magic)) * 0.0027076061740622863;               // ln(2) / 256
+        const double e = fma(r, fma(r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0) * table[i & 255];
+        const uint64_t bits = (uint64_t)__double_as_longlong(e), m = (bits & 0xfffffffffffffull) | 0x10000000000000ull;
+        const int drop = 8 - (i >> 8) + 1023 - (int)(bits >> 52);      // a little below 1 where r is negative and i a multiple of 256
+        return (m + (1ull << (drop - 1))) >> drop;
     }
 };
 
-__device__ __forceinline__ uint64_t block_sum64(uint64_t v, uint64_t* red)
+struct SampleShared {
+    double table[256];
+    unsigned low[kStretches], high[kStretches];        // words of the weights of a stretch; low alone: a count
+    unsigned long long list[kListed];                  // ranks of the border's tokens (first CTA)
+    unsigned listed;
+    unsigned count[256];
+    uint32_t best[kClusterMost], least[kClusterMost], first[kClusterMost];
+    unsigned long long share[kClusterMost], share2[kClusterMost];
+    unsigned long long found[2], border;
+    unsigned long long red[kSampleWarps], red2[kSampleWarps];
+};
+
+__device__ __forceinline__ uint64_t warp_scan64(uint64_t v)
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += w;
+    }
+    return v;
+}
+__device__ __forceinline__ uint64_t warp_add64(uint64_t v)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    uint64_t t = 0;
-    for (int i = 0; i < kSampleThreads / 32; ++i) t += red[i];
-    return t;
+    return v;
 }
 
-// The smallest prefix in falling order that is complete: `wanted` tokens, or tokens until the weight in front reaches `mass`.  In:
-// what a row keeps so far (keys above `low`, and the first `ties` equal to it).  Out: the same of the prefix.
-template <typename T>
-__global__ void __launch_bounds__(kSampleThreads)
-sample_kernel(const zkfp_sample_args a)
+// 64-bit sums in two words, each by a native atomic: a word that passes 2^32 hands its carry on
+__device__ __forceinline__ void add_weight(unsigned* low, unsigned* high, uint64_t w)
 {
+    const unsigned a = (unsigned)w, old = atomicAdd(low, a), up = (unsigned)(w >> 32) + (old + a < old ? 1u : 0u);
+    if (up) atomicAdd(high, up);
+}
+
+template <typename T, int C>
+struct Sampler {
+    cg::cluster_group cluster;
+    SampleShared& s;
+    const uint32_t* keys;
+    int n, base, me, tid, lane, warp;                  // keys of this CTA, index of the first
+    Weigher weight;
+    float top, per;                                    // stretches per logit
+    uint64_t floor;                                    // kept: ranks from here on
+
+    __device__ __forceinline__ SampleShared& of(int r) { return C == 1 ? s : *cluster.map_shared_rank(&s, r); }
+    __device__ __forceinline__ void sync()
+    {
+        if (C == 1) __syncthreads();
+        else cluster.sync();
+    }
+    __device__ __forceinline__ int stretch(uint32_t key) const
+    {
+        if (weight.infinite) return key == weight.best ? 0 : kStretches - 1;
+        return (int)fminf((top - logit_of(key)) * per, (float)(kStretches - 1));       // -infinity: the last one
+    }
+
+    // the prefix of `wanted` tokens, or (by weight) up to the token in front of which lies a share of p of all weight or more
+    __device__ __forceinline__ void narrow(bool by_weight, uint64_t wanted, double p)
+    {
+        __syncthreads();
+        for (int i = tid; i < kStretches; i += kSampleThreads) s.low[i] = s.high[i] = 0;
+        if (tid == 0) s.listed = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kSampleThreads) {
+            const uint32_t key = keys[i];
+            if (rank_of(key, base + i) < floor) continue;
+            const int b = stretch(key);
+            if (!by_weight) {
+                atomicAdd(&s.low[b], 1u);
+                continue;
+            }
+            const uint64_t w = weight(key);
+            if (w) add_weight(&s.low[b], &s.high[b], w);
+        }
+        sync();
+        // every CTA sums its share of the stretches over all CTAs
+        constexpr int kMine = kStretches / C, kPer = (kMine + kSampleThreads - 1) / kSampleThreads;
+        uint64_t v[kPer], mine = 0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            v[k] = 0;
+            const int b = me * kMine + tid * kPer + k;
+            if (tid * kPer < kMine)
+#pragma unroll
+                for (int r = 0; r < C; ++r) v[k] += (uint64_t)of(r).high[b] << 32 | of(r).low[b];
+            mine += v[k];
+        }
+        uint64_t run = warp_scan64(mine);
+        if (lane == 31) s.red[warp] = run;
+        __syncthreads();
+        uint64_t all = 0, front = 0;
+        for (int i = 0; i < kSampleWarps; ++i) {
+            if (i == warp) front = all;
+            all += s.red[i];
+        }
+        if (tid < C) of(tid).share[me] = all;
+        sync();
+        uint64_t before = front + run - mine, total = 0;
+        for (int r = 0; r < C; ++r) {
+            if (r < me) before += s.share[r];
+            total += s.share[r];
+        }
+        if (!by_weight && wanted >= total) return;                     // the same in every CTA
+        const double limit = by_weight ? fmax(p * (double)total, 1.0) : (double)wanted;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (tid * kPer < kMine && (double)before < limit && (double)(before + v[k]) >= limit)
+                for (int r = 0; r < C; ++r) {
+                    of(r).found[0] = me * kMine + tid * kPer + k;
+                    of(r).found[1] = before;
+                }
+            before += v[k];
+        }
+        sync();
+        const int border = (int)s.found[0];
+        before = s.found[1];
+        SampleShared& one = of(0);
+        for (int i = tid; i < n; i += kSampleThreads) {
+            const uint32_t key = keys[i];
+            const uint64_t rank = rank_of(key, base + i);
+            if (rank < floor || stretch(key) != border) continue;
+            const unsigned at = atomicAdd(&one.listed, 1u);
+            if (at < kListed) one.list[at] = rank;
+        }
+        sync();
+        if (one.listed <= kListed) {
+            if (me == 0) {
+                const int m = (int)s.listed;
+                unsigned long long* w = (unsigned long long*)s.low;
+                for (int i = tid; i < m; i += kSampleThreads) w[i] = by_weight ? weight((uint32_t)(s.list[i] >> 32)) : 1;
+                __syncthreads();
+                for (int i = tid; i < m; i += kSampleThreads) {
+                    const uint64_t rank = s.list[i];
+                    uint64_t in_front = before;
+                    for (int k = 0; k < m; ++k) in_front += s.list[k] > rank ? w[k] : 0;
+                    if ((double)in_front < limit && (double)(in_front + w[i]) >= limit)
+                        for (int r = 0; r < C; ++r) of(r).border = rank;
+                }
+            }
+        } else {
+            by_bits(by_weight, limit, border, before);
+        }
+        sync();
+        floor = s.border;
+    }
+
+    // the same among the many tokens of one stretch
+    __device__ __noinline__ void by_bits(bool by_weight, double limit, int border, uint64_t before)
+    {
+        uint32_t prefix = 0;
+        uint64_t here = 0;
+        for (int bits = 24; bits >= 0; bits -= 8) {
+            if (tid < 256) s.low[tid] = s.high[tid] = s.count[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += kSampleThreads) {
+                const uint32_t key = keys[i];
+                if (rank_of(key, base + i) < floor || stretch(key) != border || (bits < 24 && key >> (bits + 8) != prefix >> (bits + 8))) continue;
+                const int d = (key >> bits) & 255;
+                atomicAdd(&s.count[d], 1u);
+                const uint64_t w = by_weight ? weight(key) : 1;
+                if (w) add_weight(&s.low[d], &s.high[d], w);
+            }
+            sync();
+            // every CTA looks through the sums of all, from the largest digit down
+            if (tid < 256) {
+                uint64_t sum = 0, many = 0;
+                for (int r = 0; r < C; ++r) {
+                    sum += (uint64_t)of(r).high[tid] << 32 | of(r).low[tid];
+                    many += of(r).count[tid];
+                }
+                s.list[tid] = sum;
+                s.list[tid + 256] = many;
+            }
+            __syncthreads();
+            int d = 255;
+            for (; d > 0; --d) {
+                if (s.list[256 + d] && (double)(before + s.list[d]) >= limit) break;
+                before += s.list[d];
+            }
+            prefix |= (uint32_t)d << bits;
+            here = s.list[256 + d];
+            sync();                                    // the sums have been read
+        }
+        // `here` tokens have this key: as many of them as it takes, the lower indices first
+        const uint64_t w = by_weight ? weight(prefix) : 1;
+        const double ties = w ? ceil((limit - (double)before) / (double)w) : (double)here;
+        const uint64_t take = ties < 1.0 ? 1 : ties > (double)here ? here : (uint64_t)ties;
+        const int stretch_keys = (n + kSampleThreads - 1) / kSampleThreads * 32, i0 = warp * stretch_keys, i1 = min(i0 + stretch_keys, n);
+        auto same = [&](int i) { return i < i1 && keys[i] == prefix && rank_of(prefix, base + i) >= floor; };
+        uint64_t mine = 0;
+        for (int i = i0; i < i1; i += 32) mine += __popc(__ballot_sync(0xffffffffu, same(i + lane)));
+        if (lane == 0) s.red2[warp] = mine;
+        __syncthreads();
+        uint64_t all = 0, front = 0;
+        for (int i = 0; i < kSampleWarps; ++i) {
+            if (i == warp) front = all;
+            all += s.red2[i];
+        }
+        if (tid < C) of(tid).share2[me] = all;
+        sync();
+        for (int r = 0; r < me; ++r) front += s.share2[r];
+        if (front < take && take <= front + mine)
+            for (int i = i0; i < i1; i += 32) {
+                const unsigned b = __ballot_sync(0xffffffffu, same(i + lane));
+                if (same(i + lane) && front + __popc(b & ((2u << lane) - 1)) == take)
+                    for (int r = 0; r < C; ++r) of(r).border = rank_of(prefix, base + i + lane);
+                front += __popc(b);
+            }
+    }
+};
+
+template <typename T, int C>
+__global__ void __launch_bounds__(kSampleThreads) __cluster_dims__(C, 1, 1)
+sample_kernel(const __grid_constant__ zkfp_sample_args a, int slice, int vectors)
+{
+    extern __shared__ __align__(16) uint32_t keys[];
+    __shared__ SampleShared s;
     chain_enter();
-    __shared__ double table[256];
-    __shared__ unsigned long long mass[256];
-    __shared__ unsigned count[256];
-    __shared__ uint64_t red[kSampleThreads / 32], red2[kSampleThreads / 32];
-    __shared__ unsigned s_key;
-    __shared__ unsigned long long s_mass, s_count;
-    const long long row = blockIdx.x;
-    const T* l = (const T*)a.logits + row * a.ld;
-    const int V = (int)a.vocab, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // nobody touches another CTA's shared memory before that has started
+    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const long long row = blockIdx.x / C;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = C == 1 ? 0 : (int)(blockIdx.x % C), V = (int)a.vocab;
+    const int base = me * slice, n = max(0, min(slice, V - base));
+    const T* l = (const T*)a.logits + row * a.ld + base;
     const float temperature = a.temperature ? a.temperature[row] : a.value_temperature;
     const int top_k = a.top_k ? a.top_k[row] : a.value_top_k;
-    const float top_p = a.top_p ? a.top_p[row] : a.value_top_p, min_p = a.min_p ? a.min_p[row] : a.value_min_p;
-    if (tid < 256) table[tid] = exp2((double)tid / 256.0) * kWeightOne;
-    uint32_t best = 0;
-    for (int i = tid; i < V; i += kSampleThreads) best = max(best, key_of(to_f32(l[i])));
+    const float top_p = a.top_p ? a.top_p[row] : a.value_top_p, min_p = a.min_p ? a.min_p[row] : a.value_min_p, u = a.random[row];
+    if (tid < 256) s.table[tid] = exp2((double)tid / 256.0);
+    // the largest key, and the smallest of a finite logit
+    uint32_t best = 0, least = 0xffffffffu;
+    const uint32_t none = key_of(-INFINITY);
+    auto take = [&](int i, float x) {
+        const uint32_t k = key_of(x);
+        keys[i] = k;
+        best = max(best, k);
+        if (k != none) least = min(least, k);
+    };
+    const int whole = vectors ? n / 8 * 8 : 0;
+    for (int i = tid * 8; i < whole; i += kSampleThreads * 8) {
+        float x[8];
+        load8(l + i, x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) take(i + k, x[k]);
+    }
+    for (int i = whole + tid; i < n; i += kSampleThreads) take(i, to_f32(l[i]));
     best = __reduce_max_sync(0xffffffffu, best);
-    if (lane == 0) red[warp] = best;
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 0) s.red[warp] = (uint64_t)best << 32 | least;
     __syncthreads();
-    for (int i = 0; i < kSampleThreads / 32; ++i) best = max(best, (uint32_t)red[i]);
+    for (int i = 0; i < kSampleWarps; ++i) {
+        best = max(best, (uint32_t)(s.red[i] >> 32));
+        least = min(least, (uint32_t)s.red[i]);
+    }
+    Sampler<T, C> p{cg::this_cluster(), s, keys, n, base, me, tid, lane, warp};
+    if (C > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (tid < C) {
+            p.of(tid).best[me] = best;
+            p.of(tid).least[me] = least;
+        }
+        p.sync();
+        for (int r = 0; r < C; ++r) {
+            best = max(best, s.best[r]);
+            least = min(least, s.least[r]);
+        }
+    }
     const float top = logit_of(best);
     if (top == -INFINITY) {
-        if (tid == 0) a.out[row] = -1;
+        if (tid == 0 && me == 0) a.out[row] = -1;
         return;
     }
     const bool greedy = !(temperature > 0.f);
-    const Weigher weight{table, (double)top, greedy ? 0.0 : 1.4426950408889634 / (double)temperature, top == INFINITY};
-    uint32_t low = 0;
-    unsigned long long ties = V;               // kept: keys above low, and the first `ties` equal to it
-    // finds the prefix; by count if by_mass is false
-    auto narrow = [&](bool by_mass, unsigned long long wanted, double limit) {
-        const uint32_t floor_key = low;
-        const unsigned long long floor_ties = ties;
-        uint32_t prefix = 0;
-        unsigned long long before_mass = 0, before_count = 0;        // of keys above the bits found so far
-        for (int bits = 24; bits >= 0; bits -= 8) {
-            __syncthreads();
-            if (tid < 256) { mass[tid] = 0; count[tid] = 0; }
-            __syncthreads();
-            for (int i = tid; i < V; i += kSampleThreads) {
-                const uint32_t k = key_of(to_f32(l[i]));
-                if (k < floor_key || (bits < 24 && (k >> (bits + 8)) != (prefix >> (bits + 8)))) continue;
-                atomicAdd(&count[(k >> bits) & 255], 1u);
-                if (by_mass) atomicAdd(&mass[(k >> bits) & 255], (unsigned long long)weight(k));
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int bin = 255;
-                for (; bin > 0; --bin) {
-                    const bool done = by_mass ? (double)(before_mass + mass[bin]) >= limit : before_count + count[bin] >= wanted;
-                    if (count[bin] && done) break;
-                    before_mass += mass[bin];
-                    before_count += count[bin];
-                }
-                s_key = prefix | ((uint32_t)bin << bits);
-                s_mass = before_mass;
-                s_count = before_count;
-            }
-            __syncthreads();
-            prefix = s_key;
-            before_mass = s_mass;
-            before_count = s_count;
-        }
-        // all keys equal to prefix: how many of them
-        const unsigned long long here = count[prefix & 255];
-        unsigned long long n;
-        if (by_mass) {
-            const double w = (double)weight(prefix), rest = limit - (double)before_mass;
-            n = w > 0.0 ? (unsigned long long)fmin(ceil(rest / w), (double)here) : here;
-            if (n < 1) n = 1;
-        } else {
-            n = min(wanted - before_count, here);
-        }
-        if (prefix == floor_key) n = min(n, floor_ties);
-        low = prefix;
-        ties = n;
-    };
+    p.weight = Weigher{s.table, (double)top, greedy ? 0.0 : 256 * 1.4426950408889634 / (double)temperature, best, top == INFINITY};
+    p.top = top;
+    p.floor = 0;
+    {
+        // logits below 2^-46 of the largest weight share the last stretch
+        const float low = fmaxf(logit_of(least), greedy ? -INFINITY : top - fminf(32.f * temperature, 3e38f));
+        const float span = top - low;
+        p.per = span > 0.f && span < INFINITY ? (float)kStretches / span : 0.f;
+        if (!(p.per < 3e38f)) p.per = 0.f;
+    }
     if (greedy) {
-        low = best;
-        ties = 1;
-    } else {
-        if (top_k > 0 && top_k < V) narrow(false, (unsigned long long)top_k, 0.0);
-        if (top_p < 1.f) {
-            uint64_t m = 0, t = 0;
-            for (int i = tid; i < V; i += kSampleThreads) {
-                const uint32_t k = key_of(to_f32(l[i]));
-                if (k > low) m += weight(k);
-                else if (k == low) ++t;
-            }
-            m = block_sum64(m, red);
-            t = block_sum64(t, red2);
-            m += min((unsigned long long)t, ties) * weight(low);
-            narrow(true, 0, (double)(top_p > 0.f ? top_p : 0.f) * (double)m);
-        }
-        if (min_p > 0.f) {
-            // the smallest key that is likely enough
-            const double least = fmin(log2((double)min_p), 0.0);
-            uint32_t lowest = 0xffffffffu;
-            for (int i = tid; i < V; i += kSampleThreads) {
-                const uint32_t k = key_of(to_f32(l[i]));
-                if (weight.exponent(logit_of(k)) >= least) lowest = min(lowest, k);
-            }
-            lowest = __reduce_min_sync(0xffffffffu, lowest);
-            __syncthreads();
-            if (lane == 0) red[warp] = lowest;
-            __syncthreads();
-            for (int i = 0; i < kSampleThreads / 32; ++i) lowest = min(lowest, (uint32_t)red[i]);
-            if (lowest > low) {
-                low = lowest;
-                ties = V;
-            }
-        }
+        uint32_t first = 0xffffffffu;
+        for (int i = tid; i < n; i += kSampleThreads)
+            if (keys[i] == best) first = min(first, (uint32_t)(base + i));
+        first = __reduce_min_sync(0xffffffffu, first);
+        __syncthreads();
+        if (lane == 0) s.red[warp] = first;
+        __syncthreads();
+        for (int i = 0; i < kSampleWarps; ++i) first = min(first, (uint32_t)s.red[i]);
+        if (tid < C) p.of(tid).first[me] = first;
+        p.sync();
+        for (int r = 0; r < C; ++r) first = min(first, s.first[r]);
+        if (tid == 0 && me == 0) a.out[row] = first;
+        return;
     }
+    if (top_k > 0 && top_k < V) p.narrow(false, (uint64_t)top_k, 0.0);
+    if (top_p < 1.f) p.narrow(true, 0, top_p > 0.f ? (double)top_p : 0.0);
+    const double enough = min_p > 0.f ? 256 * fmin(log2((double)min_p), 0.0) : -INFINITY;
     // kept weight by warps, each a stretch of the indices; then the token inside its stretch
-    const int stretch = (V + kSampleThreads - 1) / kSampleThreads * 32, i0 = warp * stretch, i1 = min(i0 + stretch, V);
-    uint64_t above = 0, equal = 0;
-    for (int i = i0 + lane; i < i1; i += 32) {
-        const uint32_t k = key_of(to_f32(l[i]));
-        if (k > low) above += weight(k);
-        else if (k == low) ++equal;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        above += __shfl_xor_sync(0xffffffffu, above, o);
-        equal += __shfl_xor_sync(0xffffffffu, equal, o);
-    }
+    const int keys_each = (n + kSampleThreads - 1) / kSampleThreads * 32, i0 = warp * keys_each, i1 = min(i0 + keys_each, n);
+    auto kept = [&](int i) -> uint64_t {
+        if (i >= i1) return 0;
+        const uint32_t key = keys[i];
+        if (rank_of(key, base + i) < p.floor || (min_p > 0.f && !(p.weight.exponent(key) >= enough))) return 0;
+        return p.weight(key);
+    };
+    uint64_t mine = 0;
+    for (int i = i0; i < i1; i += 32) mine += kept(i + lane);
+    mine = warp_add64(mine);
     __syncthreads();
-    if (lane == 0) { red[warp] = above; red2[warp] = equal; }
+    if (lane == 0) s.red[warp] = mine;
     __syncthreads();
-    const uint64_t w_low = weight(low);
-    uint64_t total = 0, mine = 0, mine_ties = 0, seen = 0;           // in front of this warp's stretch
-    for (int i = 0; i < kSampleThreads / 32; ++i) {
-        if (i == warp) { mine = total; mine_ties = seen; }
-        const uint64_t here = seen >= ties ? 0 : min((uint64_t)(ties - seen), red2[i]);
-        total += red[i] + here * w_low;
-        seen += red2[i];
+    uint64_t all = 0, front = 0, total = 0;
+    for (int i = 0; i < kSampleWarps; ++i) {
+        if (i == warp) front = all;
+        all += s.red[i];
+    }
+    if (C > 1) {
+        __syncthreads();
+        if (tid < C) p.of(tid).share2[me] = all;
+        p.sync();
+        for (int r = 0; r < C; ++r) {
+            if (r < me) front += s.share2[r];
+            total += s.share2[r];
+        }
+    } else {
+        total = all;
     }
     // random < 1, so some token passes it; rounding must not take it to the total itself
-    const uint64_t target = min((uint64_t)((double)a.random[row] * (double)total), total - 1);
-    const uint64_t kept = mine_ties >= ties ? 0 : min((uint64_t)(ties - mine_ties), equal);
-    if (target < mine || target >= mine + above + kept * w_low) return;
-    uint64_t sum = mine, tie = mine_ties;
+    const uint64_t target = min((uint64_t)((double)u * (double)total), total - 1);
+    if (target < front || target >= front + mine) return;
     for (int i = i0; i < i1; i += 32) {
-        const uint32_t k = i + lane < i1 ? key_of(to_f32(l[i + lane])) : 0;
-        const unsigned same = __ballot_sync(0xffffffffu, i + lane < i1 && k == low);
-        const bool keep = i + lane < i1 && (k > low || (k == low && tie + __popc(same & ((1u << lane) - 1)) < ties));
-        uint64_t v = keep ? weight(k) : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += w;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, sum + v > target);
+        const uint64_t run = warp_scan64(kept(i + lane));
+        const unsigned past = __ballot_sync(0xffffffffu, front + run > target);
         if (past) {
-            if (lane == 0) a.out[row] = i + __ffs(past) - 1;
+            if (lane == 0) a.out[row] = base + i + __ffs(past) - 1;
             return;
         }
-        sum += __shfl_sync(0xffffffffu, v, 31);
-        tie += __popc(same);
+        front += __shfl_sync(0xffffffffu, run, 31);
+    }
+}
+
+template <typename T, int C>
+int launch_sample(const zkfp_sample_args& a, cudaStream_t st)
+{
+    const int slice = (int)((a.vocab + C * 8 - 1) / (C * 8) * 8);
+    const int vectors = !((uintptr_t)a.logits & 15) && !(a.ld * (long long)sizeof(T) & 15);
+    ZKDS_CUDA(cudaFuncSetAttribute(sample_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax - (int)sizeof(SampleShared) - 1024));
+    fp_launch(sample_kernel<T, C>, dim3((unsigned)(a.rows * C)), dim3(kSampleThreads), (size_t)slice * 4, st, a, slice, vectors);
+    return fp_launched();
+}
+
+template <typename T>
+int launch_sample(const zkfp_sample_args& a, cudaStream_t st)
+{
+    // slices of up to 18000 keys leave room for two CTAs per SM; few rows are cut further, down to 2048 keys
+    int c = 1;
+    while (c < kClusterMost && (a.vocab > 18000 * c || (a.rows * c < fp_sm_count() && a.vocab > 2048 * c))) c *= 2;
+    switch (c) {
+    case 1: return launch_sample<T, 1>(a, st);
+    case 2: return launch_sample<T, 2>(a, st);
+    case 4: return launch_sample<T, 4>(a, st);
+    default: return launch_sample<T, 8>(a, st);
     }
 }
 
@@ -239,9 +440,7 @@ using namespace zkds;
 extern "C" int zkfp_sample(const zkfp_sample_args* a, void* stream)
 {
     if (!a || !a->logits || !a->random || !a->out || a->rows < 0 || a->vocab <= 0 || a->ld < a->vocab || (unsigned)a->dtype > 1) return ZKDS_ERR_ARG;
-    if (a->rows > 0x7fffffffll || a->vocab > (1 << 18)) return ZKDS_ERR_UNSUPPORTED;
+    if (a->rows > 0x7fffffffll / kClusterMost || a->vocab > (1 << 18)) return ZKDS_ERR_UNSUPPORTED;
     if (a->rows == 0) return ZKDS_OK;
-    if (a->dtype == ZKFP_BF16) fp_launch(sample_kernel<bf16>, dim3((unsigned)a->rows), dim3(kSampleThreads), 0, (cudaStream_t)stream, *a);
-    else fp_launch(sample_kernel<float>, dim3((unsigned)a->rows), dim3(kSampleThreads), 0, (cudaStream_t)stream, *a);
-    return fp_launched();
+    return a->dtype == ZKFP_BF16 ? launch_sample<bf16>(*a, (cudaStream_t)stream) : launch_sample<float>(*a, (cudaStream_t)stream);
 }
