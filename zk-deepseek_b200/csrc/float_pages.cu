@@ -163,15 +163,17 @@ int zkfp_copy_pages(const zkfp_page_buffer* buffers, int n_buffers, const int* s
 {
     if (n_buffers < 0 || moves < 0 || (n_buffers && !buffers) || (moves && (!source || !target))) return ZKDS_ERR_ARG;
     if (!n_buffers || !moves) return ZKDS_OK;
-    long long pages = buffers[0].pages;
+    long long pages = 0x7fffffffll;
     for (int i = 0; i < n_buffers; ++i) {
         const zkfp_page_buffer& p = buffers[i];
+        if (p.bytes == 0) continue;
         if (!p.base || p.bytes < 0 || p.stride < p.bytes || ((p.bytes | p.stride) & 15) || ((uintptr_t)p.base & 15) || p.pages <= 0 ||
-            p.pages > 0x7fffffffll)
+            p.pages >= 0x7fffffffll)
             return ZKDS_ERR_ARG;
         if (p.bytes > 0x400000000ll) return ZKDS_ERR_UNSUPPORTED;
         pages = p.pages < pages ? p.pages : pages;
     }
+    if (pages == 0x7fffffffll) return ZKDS_OK;         // nothing of any buffer
     if (!moves_ok(source, target, moves, pages)) return ZKDS_ERR_ARG;
     for (int b0 = 0; b0 < n_buffers; b0 += kBuffers) {
         CopyList list;

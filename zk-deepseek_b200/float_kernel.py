@@ -4,6 +4,7 @@ Tensors go in as torch CUDA tensors; every call is launched on torch's current s
 There is no CPU or PyTorch fallback: a missing library raises at import, a failed launch raises `FloatOpsError`.
 """
 import ctypes
+import math
 import os
 import threading
 
@@ -322,52 +323,68 @@ def _refuse(what, why):
     raise ValueError("%s: %s" % (what, why))
 
 
-def _tensor(what, name, t, dtype, dims, device=None, shape=None):
+def _tensor(what, name, t, dtype, dims, device, shape=None):
+    """the tensor's address; refuses what is not on the device, or not of this type and shape"""
     if not isinstance(t, torch.Tensor) or t.dim() != dims:
         _refuse(what, "%s is no tensor of %d dimensions" % (name, dims))
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         _refuse(what, "%s is %s, not %s" % (name, t.dtype, dtype))
-    if t.device.type != "cuda":
-        _refuse(what, "%s is on %s" % (name, t.device))
-    device = torch.cuda.current_device() if device is None else device
-    if t.device.index != device:
+    if t.get_device() != device:
         _refuse(what, "%s is on %s, the call goes to cuda:%d" % (name, t.device, device))
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         _refuse(what, "%s is %s, not %s" % (name, list(t.shape), list(shape)))
-    return t
+    return t.data_ptr()
 
 
-def _heads(what, name, t, dtype, device, shape):
-    """a tensor of heads: the elements of a head adjacent, everything on 16-byte pieces"""
-    _tensor(what, name, t, dtype, len(shape), device, shape)
+def _device(what, name, t):
+    """the current device, which the call goes to"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _refuse(what, "%s is no tensor on a GPU" % name)
+    return torch.cuda.current_device()
+
+
+def _heads(what, name, t, dtype, dims, device, shape=None):
+    """address and strides of a tensor of heads: the elements of a head adjacent, everything on 16-byte pieces"""
+    at = _tensor(what, name, t, dtype, dims, device, shape)
     strides = t.stride()
-    if (t.shape[-1] > 1 and strides[-1] != 1) or any(s & 7 and n > 1 for s, n in zip(strides[:-1], t.shape)) or t.data_ptr() & 15:
-        _refuse(what, "%s has strides %s: heads must be contiguous, all else multiples of 8 elements" % (name, list(strides)))
-    # a dimension of one element has no stride of its own
-    return [s if n > 1 else 0 for s, n in zip(strides[:-1], t.shape)]
+    bits = at >> 1                             # 16-byte pieces are eight elements of bfloat16 (and two of float32's)
+    for s in strides[:-1]:
+        bits |= s
+    if bits & 7 or strides[-1] != 1:
+        n = t.shape                            # a dimension of one element has no stride of its own
+        if at & 15 or (n[-1] > 1 and strides[-1] != 1) or any(s & 7 and k > 1 for s, k in zip(strides[:-1], n)):
+            _refuse(what, "%s has strides %s: heads must be contiguous, all else multiples of 8 elements" % (name, list(strides)))
+        strides = [s if k > 1 else 0 for s, k in zip(strides, n)]
+    return at, strides[:-1]
 
 
 def _pool(what, k, v, table, rows, lengths):
-    dev = k.device.index if isinstance(k, torch.Tensor) else None
-    if not isinstance(k, torch.Tensor) or k.dtype not in (torch.float32, torch.bfloat16):
+    """device, addresses and strides of the pages, addresses of the rest, row pitch of the table, shapes"""
+    dev = _device(what, "k_pages", k)
+    dt = k.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float32:
         _refuse(what, "pages hold float32 or bfloat16")
-    _tensor(what, "k_pages", k, k.dtype, 4)
-    _tensor(what, "v_pages", v, k.dtype, 4, dev)
-    ks, vs = _heads(what, "k_pages", k, k.dtype, dev, k.shape), _heads(what, "v_pages", v, k.dtype, dev, tuple(k.shape[:3]) + (v.shape[3],))
-    if k.shape[1] not in (8, 16, 32, 64, 128, 256, 512, 1024):
-        _refuse(what, "pages of %d positions" % k.shape[1])
-    _tensor(what, "table", table, torch.int32, 2, dev)
-    batch = table.shape[0]
-    _tensor(what, "rows", rows, torch.int32, 1, dev, (batch + 1,))
-    _tensor(what, "lengths", lengths, torch.int32, 1, dev, (batch,))
-    if not batch or not table.shape[1] or not k.shape[0]:
-        _refuse(what, "no sequences, no pages or no columns")
-    if (table.shape[1] > 1 and table.stride(1) != 1) or rows.stride(0) != 1 or (batch > 1 and lengths.stride(0) != 1):
+    kp, ks = _heads(what, "k_pages", k, dt, 4, dev)
+    vp, vs = _heads(what, "v_pages", v, dt, 4, dev)
+    shape, vshape = k.shape, v.shape
+    if shape[:3] != vshape[:3]:
+        _refuse(what, "pages of keys are %s, of values %s" % (list(shape), list(vshape)))
+    pages, page, kv, d = shape
+    if not 8 <= page <= 1024 or page & (page - 1):
+        _refuse(what, "pages of %d positions" % page)
+    dv = vshape[3]
+    if d & 7 or dv & 7 or not d or not dv:
+        _refuse(what, "head sizes %d and %d are no multiples of 8" % (d, dv))
+    tp = _tensor(what, "table", table, torch.int32, 2, dev)
+    batch, cols = table.shape
+    rp, lp = _tensor(what, "rows", rows, torch.int32, 1, dev, (batch + 1,)), _tensor(what, "lengths", lengths, torch.int32, 1, dev, (batch,))
+    if not batch or not cols or not pages or not kv:
+        _refuse(what, "no sequences, no columns, no pages or no heads")
+    ld, step = table.stride()
+    ld = ld if batch > 1 else cols
+    if (cols > 1 and step != 1) or ld < cols or rows.stride(0) != 1 or (batch > 1 and lengths.stride(0) != 1):
         _refuse(what, "table, rows and lengths must be contiguous along their last dimension")
-    ld = table.stride(0) if batch > 1 else table.shape[1]
-    if ld < table.shape[1]:
-        _refuse(what, "rows of the table overlap")
-    return dev, ks, vs, ld
+    return dev, dt, kp, ks, vp, vs, tp, rp, lp, ld, batch, cols, pages, page, kv, d, dv
 
 
 def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, window=0, max_tokens=None, gate=None, out_scale=1.0):
@@ -379,25 +396,21 @@ def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, windo
     max_tokens: most rows that a sequence brings (default: all), which chooses the kernel.  gate [tokens, heads, dv]: out is
     multiplied by sigmoid(gate) * out_scale."""
     what = "paged_attention"
-    dev, ks, vs, ld = _pool(what, k_pages, v_pages, table, rows, lengths)
-    dt = k_pages.dtype
-    if not isinstance(q, torch.Tensor) or q.dim() != 3:
-        _refuse(what, "q is no tensor of 3 dimensions")
-    tokens, heads, d = q.shape
-    kv, dv = k_pages.shape[2], v_pages.shape[3]
-    if not kv or not heads or heads % kv or d != k_pages.shape[3]:
-        _refuse(what, "%d query heads of %d over %d key heads of %d" % (heads, d, kv, k_pages.shape[3]))
-    if d & 7 or dv & 7 or not d or not dv:
-        _refuse(what, "head sizes %d and %d are no multiples of 8" % (d, dv))
-    qs, os = _heads(what, "q", q, dt, dev, (tokens, heads, d)), _heads(what, "out", out, dt, dev, (tokens, heads, dv))
-    gs = _heads(what, "gate", gate, dt, dev, (tokens, heads, dv)) if gate is not None else (0, 0)
-    if window < 0 or (max_tokens is not None and max_tokens < 0) or not 0 <= scale < 3e38:
+    dev, dt, kp, ks, vp, vs, tp, rp, lp, ld, batch, cols, pages, page, kv, d, dv = _pool(what, k_pages, v_pages, table, rows, lengths)
+    qp, qs = _heads(what, "q", q, dt, 3, dev)
+    tokens, heads, size = q.shape
+    if not heads or heads % kv or d != size:
+        _refuse(what, "%d query heads of %d over %d key heads of %d" % (heads, size, kv, d))
+    shape = (tokens, heads, dv)
+    op, os = _heads(what, "out", out, dt, 3, dev, shape)
+    gp, gs = _heads(what, "gate", gate, dt, 3, dev, shape) if gate is not None else (None, (0, 0))
+    if max_tokens is None:
+        max_tokens = tokens
+    if window < 0 or max_tokens < 0 or not 0 <= scale < 3e38:
         _refuse(what, "a negative window, bound or scale")
-    a = PagedAttentionArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ptr(gate), table.data_ptr(),
-                           rows.data_ptr(), lengths.data_ptr(), None, *qs, *ks, *vs, *os, *gs, tokens, k_pages.shape[0], table.shape[1],
-                           ld, table.shape[0], tokens if max_tokens is None else max_tokens, heads, kv, d, dv, k_pages.shape[1],
-                           min(window, 0x7fffffff), code(dt), scale, out_scale)
     if tokens:
+        a = PagedAttentionArgs(qp, kp, vp, op, gp, tp, rp, lp, None, *qs, *ks, *vs, *os, *gs, tokens, pages, cols, ld, batch, max_tokens, heads,
+                               kv, d, dv, page, min(window, 0x7fffffff), code(dt), scale, out_scale)
         _with_scratch(_paged, _paged_scratch, a, what, q.device, (q, k_pages, v_pages, table, rows, lengths, out, gate))
     return out
 
@@ -410,30 +423,30 @@ def write_pages(k, v, k_pages, v_pages, table, rows, lengths, q=None, q_out=None
     with layout "pairs", (i, i + pairs) with "half"; None: nothing does.  A row at a position without angles keeps its own, a row
     without a place in the pages is not written."""
     what = "write_pages"
-    dev, ks, vs, ld = _pool(what, k_pages, v_pages, table, rows, lengths)
-    dt, (kv, d), dv = k_pages.dtype, k_pages.shape[2:], v_pages.shape[3]
-    if not isinstance(k, torch.Tensor) or k.dim() != 3 or layout not in ("pairs", "half") or (q is None) != (q_out is None):
-        _refuse(what, "k has three dimensions, layout is 'pairs' or 'half', q and q_out come together")
+    dev, dt, kp, ks, vp, vs, tp, rp, lp, ld, batch, cols, pages, page, kv, d, dv = _pool(what, k_pages, v_pages, table, rows, lengths)
+    if layout not in ("pairs", "half") or (q is None) != (q_out is None):
+        _refuse(what, "layout is 'pairs' or 'half', q and q_out come together")
+    ka, kt = _heads(what, "k", k, dt, 3, dev)
     tokens = k.shape[0]
-    if d & 7 or dv & 7 or not d or not dv:
-        _refuse(what, "head sizes %d and %d are no multiples of 8" % (d, dv))
-    kt, vt = _heads(what, "k", k, dt, dev, (tokens, kv, d)), _heads(what, "v", v, dt, dev, (tokens, kv, dv))
-    heads, qs, os = 0, (0, 0), (0, 0)
+    if k.shape != (tokens, kv, d):
+        _refuse(what, "k is %s for pages of %d heads of %d" % (list(k.shape), kv, d))
+    va, vt = _heads(what, "v", v, dt, 3, dev, (tokens, kv, dv))
+    heads, qa, qs, oa, os = 0, None, (0, 0), None, (0, 0)
     if q is not None:
-        if not isinstance(q, torch.Tensor) or q.dim() != 3 or not q.shape[1]:
-            _refuse(what, "q is no tensor of 3 dimensions")
+        qa, qs = _heads(what, "q", q, dt, 3, dev)
         heads = q.shape[1]
-        qs, os = _heads(what, "q", q, dt, dev, (tokens, heads, d)), _heads(what, "q_out", q_out, dt, dev, (tokens, heads, d))
-    positions = pairs = 0
+        if not heads or q.shape != (tokens, heads, d):
+            _refuse(what, "q is %s beside %d keys of %d" % (list(q.shape), tokens, d))
+        oa, os = _heads(what, "q_out", q_out, dt, 3, dev, q.shape)
+    ca, positions, pairs = None, 0, 0
     if cos_sin is not None:
-        _tensor(what, "cos_sin", cos_sin, torch.float32, 3, dev)
-        positions, pairs = cos_sin.shape[:2]
-        if cos_sin.shape[2] != 2 or not cos_sin.is_contiguous() or 2 * pairs > d:
+        ca = _tensor(what, "cos_sin", cos_sin, torch.float32, 3, dev)
+        positions, pairs, two = cos_sin.shape
+        if two != 2 or not cos_sin.is_contiguous() or 2 * pairs > d:
             _refuse(what, "cos_sin %s is no contiguous [positions, pairs, 2] for heads of %d" % (list(cos_sin.shape), d))
-    a = WritePagesArgs(ptr(q), k.data_ptr(), v.data_ptr(), ptr(q_out), k_pages.data_ptr(), v_pages.data_ptr(), ptr(cos_sin), table.data_ptr(),
-                       rows.data_ptr(), lengths.data_ptr(), *qs, *kt, *vt, *os, *ks, *vs, tokens, k_pages.shape[0], table.shape[1], ld,
-                       table.shape[0], positions, heads, kv, d, dv, k_pages.shape[1], pairs, int(layout == "half"), code(dt))
     if tokens:
+        a = WritePagesArgs(qa, ka, va, oa, kp, vp, ca, tp, rp, lp, *qs, *kt, *vt, *os, *ks, *vs, tokens, pages, cols, ld, batch, positions, heads,
+                           kv, d, dv, page, pairs, int(layout == "half"), code(dt))
         _call(_write_pages, (ctypes.byref(a),), what, q, k, v, q_out, k_pages, v_pages, cos_sin, table, rows, lengths)
 
 
@@ -442,32 +455,35 @@ def copy_pages(buffers, source, target, positions=None):
     copies happen at once: no page may be a target twice, or both a source and a target.  source and target: page numbers on the
     host."""
     what = "copy_pages"
-    if len(source) != len(target):
-        _refuse(what, "%d sources, %d targets" % (len(source), len(target)))
-    if not buffers or not len(source):
-        return
-    dev = None
-    list_ = (PageBuffer * len(buffers))()
-    for p, t in zip(list_, buffers):
-        if not isinstance(t, torch.Tensor) or t.dim() < 2 or t.device.type != "cuda":
-            _refuse(what, "a buffer is no [pages, page, ...] tensor on a GPU")
-        dev = torch.cuda.current_device() if dev is None else dev
-        if t.device.index != dev:
-            _refuse(what, "a buffer is on %s, the call goes to cuda:%d" % (t.device, dev))
-        if t.numel() and not t[0].is_contiguous():
-            _refuse(what, "pages are not contiguous: strides %s" % (list(t.stride()),))
-        n = t.shape[1] if positions is None else positions
-        if not 0 <= n <= t.shape[1]:
-            _refuse(what, "%d positions of pages of %d" % (n, t.shape[1]))
-        size = t.element_size()
-        page = t[0].numel() * size if t.shape[0] else 0
-        p.base, p.pages, p.bytes = t.data_ptr(), t.shape[0], page // t.shape[1] * n if t.shape[1] else 0
-        p.stride = t.stride(0) * size if t.shape[0] > 1 else page
-        if (p.base | p.stride | p.bytes) & 15:
-            _refuse(what, "pages, or the part of them that is copied, do not lie on 16-byte pieces")
     n = len(source)
-    src, dst = (_i * n)(*source), (_i * n)(*target)
-    _call(_copy_pages, (list_, len(buffers), src, dst, n), what, *buffers)
+    if n != len(target):
+        _refuse(what, "%d sources, %d targets" % (n, len(target)))
+    if not buffers or not n:
+        return
+    dev = _device(what, "a buffer", buffers[0])
+    list_ = (PageBuffer * len(buffers))()
+    for i, t in enumerate(buffers):
+        if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dim() < 2:
+            _refuse(what, "buffer %d is no [pages, page, ...] tensor on cuda:%d" % (i, dev))
+        pages, lines, *rest = t.shape
+        stride, line, *inner = t.stride()
+        size = t.element_size()
+        row = math.prod(rest) * size
+        if positions is not None and not 0 <= positions <= lines:
+            _refuse(what, "%d positions of pages of %d" % (positions, lines))
+        if not pages or not lines or not row:
+            if pages <= max(max(source), max(target)):
+                _refuse(what, "buffer %d has %d pages" % (i, pages))
+            continue
+        dense = len(rest) == 1 and inner[0] == 1 and (line == rest[0] or lines == 1)
+        if not dense and not t[0].is_contiguous():
+            _refuse(what, "pages of buffer %d are not contiguous: strides %s" % (i, list(t.stride())))
+        at, whole, some = t.data_ptr(), row * lines, row * (lines if positions is None else positions)
+        stride = stride * size if pages > 1 else whole
+        if (at | stride | some) & 15:
+            _refuse(what, "pages of buffer %d, or the part of them that is copied, do not lie on 16-byte pieces" % i)
+        list_[i] = (at, stride, some, pages)
+    _call(_copy_pages, (list_, len(buffers), (_i * n)(*source), (_i * n)(*target), n), what, *buffers)
 
 
 def sample(logits, random, out=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -479,38 +495,42 @@ def sample(logits, random, out=None, temperature=1.0, top_k=0, top_p=1.0, min_p=
     the largest.  Each of the four is a number or a tensor [rows] (float32; top_k int32).  A row of nothing but -infinity and
     NaN gives -1."""
     what = "sample"
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16):
+    dev = _device(what, "logits", logits)
+    dt = logits.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float32:
         _refuse(what, "logits are float32 or bfloat16")
-    _tensor(what, "logits", logits, logits.dtype, 2)
-    rows, vocab = logits.shape
-    dev = logits.device.index
-    if not vocab or (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+    at = _tensor(what, "logits", logits, dt, 2, dev)
+    (rows, vocab), (ld, step) = logits.shape, logits.stride()
+    if rows == 1:
+        ld = vocab
+    if not vocab or (vocab > 1 and step != 1) or ld < vocab:
         _refuse(what, "logits %s with strides %s" % (list(logits.shape), list(logits.stride())))
+    shape = (rows,)
 
     def per_row(name, t, dtype):
-        _tensor(what, name, t, dtype, 1, dev, (rows,))
+        at = _tensor(what, name, t, dtype, 1, dev, shape)
         if rows > 1 and t.stride(0) != 1:
             _refuse(what, "%s is not contiguous" % name)
-        return t.data_ptr()
+        return at
 
-    out = torch.empty(rows, dtype=torch.int64, device=logits.device) if out is None else out
-    pointers, values, held = [], [], []
-    for name, x, dtype, least in (("temperature", temperature, torch.float32, 0), ("top_k", top_k, torch.int32, 0), ("top_p", top_p, torch.float32, 0),
-                                  ("min_p", min_p, torch.float32, 0)):
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    f32, at_u, at_out = torch.float32, per_row("random", random, torch.float32), per_row("out", out, torch.int64)
+    pointers, values, held = [], [], [logits, random, out]
+    for name, x, dtype in (("temperature", temperature, f32), ("top_k", top_k, torch.int32), ("top_p", top_p, f32), ("min_p", min_p, f32)):
         if isinstance(x, torch.Tensor):
             pointers.append(per_row(name, x, dtype))
+            values.append(0)
             held.append(x)
-            x = 0
         else:
-            pointers.append(None)
-            if not x >= least:
+            if not x >= 0:
                 _refuse(what, "%s is %r" % (name, x))
-        values.append(x)
-    if values[1] != int(values[1]):
+            pointers.append(None)
+            values.append(x)
+    temperature, top_k, top_p, min_p = values
+    if top_k != int(top_k):
         _refuse(what, "top_k is %r" % (top_k,))
-    a = SampleArgs(logits.data_ptr(), per_row("random", random, torch.float32), per_row("out", out, torch.int64), *pointers,
-                   logits.stride(0) if rows > 1 else vocab, rows, vocab, code(logits.dtype), values[0], min(int(values[1]), 0x7fffffff), values[2],
-                   values[3])
     if rows:
-        _call(_sample, (ctypes.byref(a),), what, logits, random, out, *held)
+        a = SampleArgs(at, at_u, at_out, *pointers, ld, rows, vocab, code(dt), temperature, min(int(top_k), 0x7fffffff), top_p, min_p)
+        _call(_sample, (ctypes.byref(a),), what, *held)
     return out
