@@ -274,6 +274,15 @@ typedef struct {
 } zkfp_write_pages_args;
 int zkfp_write_pages(const zkfp_write_pages_args* a, void* stream);
 
+/* zkfp_heads_post into pages: cache is [pages][page][pitch], slot_stride the elements between pages, the positions of sequence b
+ * are in the pages of table row b (slots is not read), and no position is beyond cols * page. */
+typedef struct {
+    const int* table;
+    long long cols, ld, pages;
+    int page;
+} zkfp_page_table;
+int zkfp_heads_post_paged(const zkfp_heads_args* a, const zkfp_page_table* pages, void* stream);
+
 /* Copies the first `bytes` of page source[i] over those of page target[i] in every buffer, all of them at once: no page
  * may be a target twice, or a source and a target.  source and target are host memory and are read before the call
  * returns. */

@@ -1,6 +1,7 @@
 // Grouped attention layers: heads after the projection (norm, rotation, cache write) and attention of a few tokens per
 // sequence over the cache.  Norms, rotations, scores and weights are 32-bit in both number formats.
 #include "float_common.cuh"
+#include "float_paged.cuh"
 
 namespace zkds {
 
@@ -8,9 +9,10 @@ namespace {
 
 // ---- norm, rotation, cache write -----------------------------------------------------------------------------
 // LANES lanes of a warp take one head of one row, eight elements each and V such vectors.
+// With a table of pages, slot_stride is a page's and the row of the table is the sequence's.
 template <typename T, int LANES, int V>
 __global__ void __launch_bounds__(256)
-heads_post_kernel(const zkfp_heads_args a)
+heads_post_kernel(const zkfp_heads_args a, const zkfp_page_table pages, int shift, int* error_flag)
 {
     chain_enter();
     const int lane = threadIdx.x % LANES, units = a.heads + a.kv_heads;
@@ -21,10 +23,21 @@ heads_post_kernel(const zkfp_heads_args a)
     const int head = (int)(unit - r * units), b = (int)(r / a.seq);
     const int pos = a.start[b] + (int)(r - (long long)b * a.seq);
     if (pos < 0 || pos >= a.capacity) return;
+    long long block = 0, line = pos;
+    if (pages.table) {
+        block = pages.table[b * pages.ld + (pos >> shift)];
+        line = pos & (pages.page - 1);
+        if (block < 0 || block >= pages.pages) {               // the same for the whole row
+            if (threadIdx.x % LANES == 0) *(volatile int*)error_flag = 1;
+            return;
+        }
+    } else {
+        block = a.slots[b];
+    }
     const bool is_q = head < a.heads;
     const int kv = head - a.heads;
     const T* src = (const T*)a.y + r * a.ldy + (is_q ? a.q_col + (long long)head * a.d : a.k_col + (long long)kv * a.d);
-    T* row = (T*)a.cache + a.slots[b] * a.slot_stride + (long long)pos * a.pitch;
+    T* row = (T*)a.cache + block * a.slot_stride + line * a.pitch;
     T* dst = is_q ? (T*)a.q + (r * a.heads + head) * a.d : row + (long long)kv * a.d;
     const float* w = is_q ? a.wq : a.wk;
     float x[V][8];
@@ -65,21 +78,23 @@ heads_post_kernel(const zkfp_heads_args a)
 }
 
 template <typename T, int LANES, int V>
-int heads_post(const zkfp_heads_args& a, cudaStream_t st)
+int heads_post(const zkfp_heads_args& a, const zkfp_page_table& pages, cudaStream_t st)
 {
     const long long per = 256 / LANES, blocks = (a.rows * (a.heads + a.kv_heads) + per - 1) / per;
     if (blocks > 0x7fffffffll) return ZKDS_ERR_UNSUPPORTED;
-    fp_launch(heads_post_kernel<T, LANES, V>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    int* flag = pages.table ? fp_error_flag() : nullptr;
+    if (pages.table && !flag) return ZKDS_ERR_WORKSPACE;
+    fp_launch(heads_post_kernel<T, LANES, V>, dim3((unsigned)blocks), dim3(256), 0, st, a, pages, pages.table ? page_shift(pages.page) : 0, flag);
     return fp_launched();
 }
 
 template <typename T>
-int heads_post(const zkfp_heads_args& a, cudaStream_t st)
+int heads_post(const zkfp_heads_args& a, const zkfp_page_table& pages, cudaStream_t st)
 {
-    if (a.d <= 64) return heads_post<T, 8, 1>(a, st);
-    if (a.d <= 128) return heads_post<T, 16, 1>(a, st);
-    if (a.d <= 256) return heads_post<T, 32, 1>(a, st);
-    if (a.d <= 1024) return heads_post<T, 32, 4>(a, st);
+    if (a.d <= 64) return heads_post<T, 8, 1>(a, pages, st);
+    if (a.d <= 128) return heads_post<T, 16, 1>(a, pages, st);
+    if (a.d <= 256) return heads_post<T, 32, 1>(a, pages, st);
+    if (a.d <= 1024) return heads_post<T, 32, 4>(a, pages, st);
     return ZKDS_ERR_UNSUPPORTED;
 }
 
@@ -297,15 +312,25 @@ using namespace zkds;
 
 extern "C" {
 
-int zkfp_heads_post(const zkfp_heads_args* a, void* stream)
+static int heads_post(const zkfp_heads_args* a, const zkfp_page_table& pages, void* stream)
 {
-    if (!a || !a->y || !a->wq || !a->wk || !a->q || !a->cache || !a->table || !a->start || !a->slots || a->rows < 0 ||
+    if (!a || !a->y || !a->wq || !a->wk || !a->q || !a->cache || !a->table || !a->start || (!a->slots && !pages.table) || a->rows < 0 ||
         a->seq <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->d <= 0 || (a->d & 7) || a->dim <= 0 || a->dim > a->d ||
         a->pairs < 0 || 2 * a->pairs > a->d || a->pitch < 2ll * a->kv_heads * a->d ||
         ((a->ldy | a->q_col | a->k_col | a->pitch | a->slot_stride) & 7))
         return ZKDS_ERR_ARG;
     if (a->rows == 0) return ZKDS_OK;
-    return a->dtype == ZKFP_BF16 ? heads_post<bf16>(*a, (cudaStream_t)stream) : heads_post<float>(*a, (cudaStream_t)stream);
+    return a->dtype == ZKFP_BF16 ? heads_post<bf16>(*a, pages, (cudaStream_t)stream) : heads_post<float>(*a, pages, (cudaStream_t)stream);
+}
+
+int zkfp_heads_post(const zkfp_heads_args* a, void* stream) { return heads_post(a, zkfp_page_table{}, stream); }
+
+int zkfp_heads_post_paged(const zkfp_heads_args* a, const zkfp_page_table* pages, void* stream)
+{
+    if (!a || !pages || !pages->table || pages->cols <= 0 || pages->ld < pages->cols || pages->pages <= 0 || page_shift(pages->page) < 0 ||
+        a->capacity < 0 || a->capacity > pages->cols * pages->page)
+        return ZKDS_ERR_ARG;
+    return heads_post(a, *pages, stream);
 }
 
 long long zkfp_grouped_scratch(const zkfp_grouped_args* a)

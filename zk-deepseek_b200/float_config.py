@@ -27,10 +27,25 @@ DESIGNS = {"Munalorn": Design("Munalorn"),
 
 
 @dataclass(frozen=True)
+class RotaryScaling:
+    """angles of a model that is run on longer contexts than it was trained on.  "linear": positions divided by `factor`.
+    "yarn": the slow pairs alone, those that turn less than `slow` times over the `original` positions, are divided,
+    the fast ones, more than `fast` times, are not, and between the two the share falls evenly with the index of the pair;
+    cosines and sines are multiplied by `magnitude` (None: 1 + ln(factor) / 10)."""
+    kind: str
+    factor: float
+    original: int = 0
+    fast: float = 32.0
+    slow: float = 1.0
+    magnitude: Optional[float] = None
+
+
+@dataclass(frozen=True)
 class Rotary:
     base: float
     dims: int                           # rotated dimensions
     layout: str = "pairs"               # turns (2i, 2i + 1), or with "half" (i, i + dims / 2)
+    scaling: Optional[RotaryScaling] = None
 
 
 @dataclass(frozen=True)
@@ -113,6 +128,8 @@ class DecoderArgs:
     layers: List[LayerConfig] = field(default_factory=list)
     max_seq_len: int = 4096
     max_batch_size: int = 1
+    page: int = 0                       # positions of a page of the cache; 0: a slot of max_seq_len positions per sequence
+    pages: Optional[int] = None         # pages of the pool; None: as many as all sequences could fill
 
     @property
     def n_layers(self):
@@ -121,6 +138,23 @@ class DecoderArgs:
 
 class ConfigError(ValueError):
     pass
+
+
+def _scaling(where, rot):
+    """the "scaling" of a config's rotation: {"type": "linear" or "yarn", "factor": .., "original": .., ...}"""
+    s = rot.get("scaling")
+    if not s:
+        return None
+    kind, factor = s.get("type"), float(s.get("factor", 0))
+    if kind not in ("linear", "yarn") or not 1.0 <= factor < float("inf"):
+        raise ConfigError("%s: a rotation scaled by %r, factor %s" % (where, kind, factor))
+    if kind == "linear":
+        return RotaryScaling(kind, factor)
+    r = RotaryScaling(kind, factor, int(s.get("original") or 0), float(s.get("fast", 32.0)), float(s.get("slow", 1.0)),
+                      None if s.get("magnitude") is None else float(s["magnitude"]))
+    if r.original <= 0 or not 0 < r.slow < r.fast:
+        raise ConfigError("%s: a rotation scaled from %d positions, pairs from %s to %s turns" % (where, r.original, r.slow, r.fast))
+    return r
 
 
 def _size(d, key, shapes, tensor, axis, divide=1, less=0):
@@ -142,11 +176,13 @@ def _latent_attention(i, mx, shapes, layers):
     H = int(mx["heads"])
     rot = mx.get("rot")
     if rot is None and kv_from is not None:
-        rot = {"base": layers[kv_from].mixer.rot.base, "dims": layers[kv_from].mixer.rot.dims}
+        rot, scaling = {"base": layers[kv_from].mixer.rot.base, "dims": layers[kv_from].mixer.rot.dims}, layers[kv_from].mixer.rot.scaling
+    else:
+        scaling = _scaling("layer %d" % i, rot or {})
     if not rot:
         raise ConfigError("layer %d has no rotation" % i)
     rot_dim = int(mx["rot_dim"]) if mx.get("rot_dim") is not None else int(rot["dims"])
-    rotary = Rotary(float(rot["base"]), int(rot.get("dims", rot_dim)))
+    rotary = Rotary(float(rot["base"]), int(rot.get("dims", rot_dim)), scaling=scaling)
     if rotary.dims != rot_dim or rot_dim % 2:
         raise ConfigError("layer %d: the rotated part has %d dimensions, the rotation %d" % (i, rot_dim, rotary.dims))
     mask = mx.get("mask") or {}
@@ -166,7 +202,7 @@ def _rotary(where, mx, dim):
     rot = mx.get("rot")
     if not rot:
         raise ConfigError("%s has no rotation" % where)
-    r = Rotary(float(rot["base"]), int(rot.get("dims", dim)), "half")
+    r = Rotary(float(rot["base"]), int(rot.get("dims", dim)), "half", _scaling(where, rot))
     if r.dims % 2 or not 0 < r.dims <= dim:
         raise ConfigError("%s: a rotation of %d of %d dimensions" % (where, r.dims, dim))
     return r

@@ -106,6 +106,10 @@ class WritePagesArgs(ctypes.Structure):
                 ("page", _i), ("pairs", _i), ("half", _i), ("dtype", _i)]
 
 
+class PageTable(ctypes.Structure):
+    _fields_ = [("table", _vp), ("cols", _ll), ("ld", _ll), ("pages", _ll), ("page", _i)]
+
+
 class PageBuffer(ctypes.Structure):
     _fields_ = [("base", _vp), ("stride", _ll), ("bytes", _ll), ("pages", _ll)]
 
@@ -130,6 +134,7 @@ _scratch = _sig("zkfp_attention_scratch", [ctypes.POINTER(AttentionArgs)], _ll)
 linear_path = _sig("zkfp_linear_path", [ctypes.POINTER(LinearArgs)])
 attention_path = _sig("zkfp_attention_path", [ctypes.POINTER(AttentionArgs)])
 _heads_post = _sig("zkfp_heads_post", [ctypes.POINTER(HeadsArgs), _vp])
+_heads_post_paged = _sig("zkfp_heads_post_paged", [ctypes.POINTER(HeadsArgs), ctypes.POINTER(PageTable), _vp])
 _grouped = _sig("zkfp_grouped_attention", [ctypes.POINTER(GroupedArgs), _vp])
 _grouped_scratch = _sig("zkfp_grouped_scratch", [ctypes.POINTER(GroupedArgs)], _ll)
 _conv = _sig("zkfp_short_conv", [ctypes.POINTER(ConvArgs), _vp])
@@ -288,6 +293,11 @@ def attention_scratch(args):
 
 def heads_post(args, *tensors):
     _call(_heads_post, (ctypes.byref(args),), "heads_post", *tensors)
+
+
+def heads_post_paged(args, pages, *tensors):
+    """heads_post whose cache is a pool [pages, page, pitch]; `pages` is a PageTable"""
+    _call(_heads_post_paged, (ctypes.byref(args), ctypes.byref(pages)), "heads_post_paged", *tensors)
 
 
 def _with_scratch(fn, size, args, what, device, tensors):

@@ -26,9 +26,11 @@ from torch import nn
 
 try:
     from . import float_kernel as K
+    from .paged_cache import PagedCache
     from .sequence_cache import SequenceCache
 except ImportError:  # pragma: no cover - this directory first on sys.path
     import float_kernel as K
+    from paged_cache import PagedCache
     from sequence_cache import SequenceCache
 
 # a step with at most this many tokens per sequence takes the decode form of attention: over the latents themselves, or over
@@ -46,16 +48,29 @@ def _padded(t, shape, dtype, device):
 
 
 def rotary_table(rot, positions, device):
-    """(cos, sin) of p * base^(-2i/dims) as float32 [positions, dims / 2, 2], computed in float64"""
+    """(cos, sin) of p * base^(-2i/dims) as float32 [positions, dims / 2, 2], computed in float64; see `RotaryScaling` for
+    angles that are scaled"""
     i = torch.arange(rot.dims // 2, dtype=torch.float64)
-    ang = torch.outer(torch.arange(positions, dtype=torch.float64), float(rot.base) ** (-2.0 * i / rot.dims))
-    return torch.stack((ang.cos(), ang.sin()), dim=-1).to(device=device, dtype=torch.float32).contiguous()
+    speed, size, s = float(rot.base) ** (-2.0 * i / rot.dims), 1.0, rot.scaling
+    if s is not None and s.kind == "linear":
+        speed = speed / s.factor
+    elif s is not None:
+        # the pair (a real number) that turns n times over the original positions
+        pair = lambda n: rot.dims * math.log(s.original / (n * 2 * math.pi)) / (2 * math.log(rot.base))
+        low, high = max(math.floor(pair(s.fast)), 0), min(math.ceil(pair(s.slow)), rot.dims - 1)
+        slow = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+        speed = speed * (1 - slow) + speed / s.factor * slow
+        size = 1.0 + 0.1 * math.log(s.factor) if s.magnitude is None else s.magnitude
+    ang = torch.outer(torch.arange(positions, dtype=torch.float64), speed)
+    return (torch.stack((ang.cos(), ang.sin()), dim=-1) * size).to(device=device, dtype=torch.float32).contiguous()
 
 
 class Step:
     """What the layers need to know about the step that is running."""
 
-    def __init__(self, batch, seq, start_pos, start, slots, host_slots, cache):
+    def __init__(self, batch, seq, start_pos, start, slots, host_slots, cache, paged=None):
+        # of a cache in pages: (table [batch, columns], rows [batch + 1], positions [batch]), device int32
+        self.paged = paged
         self.batch, self.seq, self.rows = batch, seq, batch * seq
         self.start_pos = start_pos        # None in a recorded step
         self.start, self.slots = start, slots          # device int32 [batch]
@@ -330,10 +345,18 @@ class KeyValuedAttention(StackedMixer):
         q = torch.empty(st.rows, c.heads, d, dtype=dt, device=y.device)
         a = K.HeadsArgs(y.data_ptr(), self.q_norm.data_ptr(), self.k_norm.data_ptr(), q.data_ptr(), cache.data_ptr(),
                         self.rot_table.data_ptr(), st.start.data_ptr(), st.slots.data_ptr(), y.stride(0), 0, self.q_cols,
-                        st.rows, st.seq, cache.stride(0), cache.stride(1), cache.shape[1], c.heads, c.kv_heads, d, c.dim,
+                        st.rows, st.seq, cache.stride(0), cache.stride(1), st.cache.capacity, c.heads, c.kv_heads, d, c.dim,
                         c.rot.dims // 2, K.code(dt), self.eps)
-        K.heads_post(a, y, q, cache, self.q_norm, self.k_norm, self.rot_table, st.start, st.slots)
         gate = y[:, self.q_cols + self.k_cols:]
+        if st.paged is not None:
+            table, rows, lengths = st.paged
+            t = K.PageTable(table.data_ptr(), table.shape[1], table.stride(0), cache.shape[0], cache.shape[1])
+            K.heads_post_paged(a, t, y, q, cache, self.q_norm, self.k_norm, self.rot_table, st.start, table)
+            heads = lambda x, n: x.unflatten(-1, (n, d))
+            K.paged_attention(q, heads(cache[..., :self.k_cols], c.kv_heads), heads(cache[..., self.k_cols:], c.kv_heads), table, rows, lengths,
+                              heads(out, c.heads), c.scale, c.window, st.seq, heads(gate[:, :self.q_cols], c.heads), self.out_scale)
+            return
+        K.heads_post(a, y, q, cache, self.q_norm, self.k_norm, self.rot_table, st.start, st.slots)
         es = y.element_size()
         if st.seq <= ABSORB_MAX_TOKENS:
             bound = min(st.bound, c.window + st.seq - 1) if c.window else st.bound
@@ -607,9 +630,11 @@ class FloatTransformer(nn.Module):
     def load_weights(self, W, device):
         """W(name, shape) returns a checked tensor"""
         args = self.args
+        if args.page and any(isinstance(layer.mixer, LatentAttention) for layer in self.layers):
+            raise NotImplementedError("layers of design %s keep latents, which live in slots and not in pages" % args.design.name)
 
         def tables(rot):
-            key = rot.base, rot.dims
+            key = rot.base, rot.dims, rot.scaling
             if key not in self._tables:
                 self._tables[key] = rotary_table(rot, args.max_seq_len, device)
             return self._tables[key]
@@ -621,8 +646,9 @@ class FloatTransformer(nn.Module):
         self.embed = _padded(W("embed", shape), padded, self.dtype, device)
         self.head = self.embed if args.design.tied_output else _padded(W("head", shape), padded, self.dtype, device)
         mixers = [l.mixer for l in self.layers]
-        self.cache = SequenceCache([m.cache_pitch() for m in mixers], [m.cache_owner() for m in mixers], args.max_batch_size,
-                                   args.max_seq_len, self.dtype, device, [m.state_shapes(self.dtype) for m in mixers])
+        kept = ([m.cache_pitch() for m in mixers], [m.cache_owner() for m in mixers], args.max_batch_size, args.max_seq_len, self.dtype,
+                device, [m.state_shapes(self.dtype) for m in mixers])
+        self.cache = PagedCache(*kept, page=args.page, pages=args.pages) if args.page else SequenceCache(*kept)
         return self
 
     def tensor_names(self):
@@ -646,14 +672,34 @@ class FloatTransformer(nn.Module):
         for s in slots:
             self.cache.release(s)
 
+    def fork(self, slots, n):
+        """n slots in the place of every slot: itself and n - 1 new ones that stand where it does"""
+        new = []
+        try:
+            out = []
+            for s in slots:
+                out.append(s)
+                for _ in range(n - 1):
+                    new.append(self.cache.fork(s))
+                    out.append(new[-1])
+            return out
+        except Exception:
+            self.end_batch(new)
+            raise
+
+    def _paging(self, slots, start_pos, S):
+        """what a step over pages takes with it (host int32): table, rows, positions"""
+        B = len(slots)
+        return self.cache.table(slots), torch.arange(B + 1, dtype=torch.int32) * S, torch.full((B,), start_pos + S, dtype=torch.int32)
+
     # -- one step --------------------------------------------------------------------------------------
     def prep_inference(self, tokens, start_pos, slots):
         """(activations, step) of tokens [B, S] that follow position start_pos - 1 of the given slots"""
         B, S = tokens.shape
-        for s in slots:
-            self.cache.extend(s, start_pos, S)
+        self.cache.extend_all(slots, start_pos, S)
         meta = torch.tensor([[start_pos] * B, list(slots)], dtype=torch.int32).to(self.device, non_blocking=True)
-        st = Step(B, S, start_pos, meta[0], meta[1], list(slots), self.cache)
+        paged = [t.to(self.device, non_blocking=True) for t in self._paging(slots, start_pos, S)] if self.args.page else None
+        st = Step(B, S, start_pos, meta[0], meta[1], list(slots), self.cache, paged)
         return self._embed(tokens.to(self.device)), st
 
     def _embed(self, tokens):
@@ -727,8 +773,7 @@ class FloatTransformer(nn.Module):
 
     def _decode(self, tokens, start_pos, slots):
         B = tokens.shape[0]
-        for s in slots:
-            self.cache.extend(s, start_pos, 1)
+        self.cache.extend_all(slots, start_pos, 1)
         if B not in self._recorded:
             self._recorded[B] = RecordedStep(self, B)
         return self._recorded[B].run(tokens, start_pos, slots)
@@ -750,6 +795,13 @@ class RecordedStep:
         self.host = torch.zeros(STEPS_AHEAD, 2, B, dtype=torch.int32).pin_memory()
         self.host_tokens = torch.zeros(STEPS_AHEAD, B, 1, dtype=torch.int64).pin_memory()
         self.rows = torch.arange(B, dtype=torch.int32, device=dev)
+        self.paged = None
+        if model.args.page:
+            self.lengths = torch.zeros(B, dtype=torch.int32, device=dev)
+            self.paged = (torch.zeros(B, model.cache.columns, dtype=torch.int32, device=dev), torch.arange(B + 1, dtype=torch.int32, device=dev),
+                          self.lengths)
+            self.host_table = torch.zeros(STEPS_AHEAD, B, model.cache.columns, dtype=torch.int32).pin_memory()
+            self.shown = None          # slots and version of the table that the device holds
         self.copied, self.turn = [torch.cuda.Event() for _ in range(STEPS_AHEAD)], 0
 
     def run(self, tokens, start_pos, slots):
@@ -758,6 +810,12 @@ class RecordedStep:
         copied.synchronize()              # the inputs of the step that used these buffers have left them
         host.copy_(torch.tensor([[start_pos] * len(slots), slots], dtype=torch.int32))
         self.meta.copy_(host, non_blocking=True)
+        if self.paged is not None:
+            torch.add(self.meta[0], 1, out=self.lengths)
+            now = (tuple(slots), self.model.cache.version)
+            if now != self.shown:
+                self.paged[0].copy_(self.host_table[self.turn].copy_(self.model.cache.table(slots)), non_blocking=True)
+                self.shown = now
         if tokens.device.type == "cpu":   # the caller may overwrite its buffer, pinned or not, once this call returns
             tokens = self.host_tokens[self.turn].copy_(tokens)
         self.tokens.copy_(tokens, non_blocking=True)
@@ -766,7 +824,7 @@ class RecordedStep:
             self.calls.replay()
             return self.logits.clone()
         m = self.model
-        st = Step(self.tokens.shape[0], 1, None, self.meta[0], self.meta[1], None, m.cache)
+        st = Step(self.tokens.shape[0], 1, None, self.meta[0], self.meta[1], None, m.cache, self.paged)
         with K.Recording() as calls:
             h = m._embed(self.tokens)
             for layer in m.layers:

@@ -82,12 +82,13 @@ class TensorFiles:
 
 
 # ---- loading ---------------------------------------------------------------------------------------------
-def load_float_model(model_dir, dtype="bfloat16", device="cuda", max_seq_len=4096, max_batch_size=1, cfg=None):
+def load_float_model(model_dir, dtype="bfloat16", device="cuda", max_seq_len=4096, max_batch_size=1, cfg=None, page=0, pages=None):
     import torch
     cfg = cfg if cfg is not None else float_config.read_config(model_dir)
     files = TensorFiles(model_dir)
     args = float_config.parse_config(cfg, files.shapes())
     args.max_seq_len, args.max_batch_size = int(max_seq_len), int(max_batch_size)
+    args.page, args.pages = int(page), pages
     _build.build(library=_build.FLOAT_LIBRARY)
     fm = _module("float_model")
     model = fm.FloatTransformer(args, getattr(torch, dtype) if isinstance(dtype, str) else dtype)
@@ -109,10 +110,13 @@ def load_integer_model(model_dir, device="cuda", max_seq_len=None, max_batch_siz
     return _module("generate").load_resident(model_dir, args, device=device, cache_batch=max_batch_size)
 
 
-def load(model_dir, dtype="bfloat16", device="cuda", max_seq_len=4096, max_batch_size=1):
+def load(model_dir, dtype="bfloat16", device="cuda", max_seq_len=4096, max_batch_size=1, page=0, pages=None):
     """The model of a checkpoint directory, ready to run on `device`.  dtype belongs to the floating-point designs;
-    the integer model has one number format."""
+    the integer model has one number format.  page: positions of a page, for a cache in a pool of `pages` pages that sequences
+    share (0: a slot of max_seq_len positions each); for designs whose layers keep keys and values or a state."""
     cfg = float_config.read_config(model_dir)
     if architecture_of(cfg) == INTEGER_MODEL:
+        if page:
+            raise NotImplementedError("the integer model keeps its cache in slots")
         return load_integer_model(model_dir, device, max_seq_len, max_batch_size, cfg)
-    return load_float_model(model_dir, dtype, device, max_seq_len, max_batch_size, cfg)
+    return load_float_model(model_dir, dtype, device, max_seq_len, max_batch_size, cfg, page, pages)

@@ -66,6 +66,25 @@ class SequenceCache:
             raise ValueError("the recurrent state of slot %d stands at position %d" % (slot, self.lengths[slot]))
         self.lengths[slot] = length
 
+    def fork(self, slot):
+        """a new slot that holds what this one does: its positions and its recurrent state are copied"""
+        if slot in self._free or not 0 <= slot < self.slots:
+            raise ValueError("slot %d is not in use" % slot)
+        try:
+            from .paged_cache import _copy_pages, copy_states
+        except ImportError:  # pragma: no cover - this directory first on sys.path
+            from paged_cache import _copy_pages, copy_states
+        new, n = self.acquire(), self.lengths[slot]
+        if n:
+            _copy_pages([b for b in self.buffers if b is not None], [slot], [new], positions=n)
+            copy_states(_copy_pages, self.states, slot, new)
+        self.lengths[new] = n
+        return new
+
+    def extend_all(self, slots, start, n):
+        for s in slots:
+            self.extend(s, start, n)
+
     def free_slots(self):
         return len(self._free)
 
