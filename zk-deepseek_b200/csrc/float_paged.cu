@@ -158,9 +158,10 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
         if (whole) {
             __syncthreads();
             for (int r = tid >> 5; r < rows; r += kPlainThreads / 32) {
-                float x[8];
+                float x[2][4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = lane + 32 * k < dv ? O[r * dv + lane + 32 * k] : 0.f;
+                for (int k = 0; k < 2; ++k)
+                    if (4 * lane + 128 * k < dv) load4(O + r * dv + 4 * lane + 128 * k, x[k]);
                 finish_row<T>(p, w, row0 + r, x, L[r]);
             }
         } else if (tid < rows) {
@@ -172,43 +173,58 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
 
 // ---- cut items ---------------------------------------------------------------------------------------------------
 // Block x merges the item that CTA x began and did not end, a warp per row.  Maxima are in units of log2 where base2.  Lanes take the
-// parts' maxima and sums, 32 at a time, then all of them the columns of one part after the other.
-template <typename T>
+// parts' maxima and sums, 32 at a time, then all of them the columns of eight parts at a time.
+template <typename T, int K>
 __global__ void __launch_bounds__(128)
 paged_combine_kernel(const __grid_constant__ Paged p, int base2)
 {
     chain_enter();
-    const int c = blockIdx.x, lane = threadIdx.x & 31, dv = p.a.dv, parts = p.cut[c * 8];
-    if (parts == 0) return;
+    const int c = blockIdx.x, lane = threadIdx.x & 31, dv = p.a.dv;
     const int4 what = *(const int4*)(p.cut + c * 8), where = *(const int4*)(p.cut + c * 8 + 4);
+    const int parts = what.x;
+    if (parts == 0) return;
     Walk w;
     w.b = what.y; w.kv = what.z; w.t = what.w;
     w.row0 = where.x; w.n = where.y; w.len = where.z;
     const int row0 = w.t * p.tile, rows = min(p.tile, w.n * p.group - row0);
     const int r = blockIdx.y * 4 + (threadIdx.x >> 5);
     if (r >= rows) return;
-    float x[8] = {}, m = -INFINITY, l = 0.f;
+    // the first part lies in the second place of its CTA, the others in the first of theirs
     auto place = [&](int i) { return (2ll * (c + i) + (i == 0)) * p.tile + r; };
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.ml[place(i) * 2]);
-    m = warp_max(m);
+    float x[K][4] = {}, m = -INFINITY, l = 0.f;
     for (int i0 = 0; i0 < parts; i0 += 32) {
-        float f = 0.f;
-        if (i0 + lane < parts) {
-            const float2 ml = *(const float2*)(p.ml + place(i0 + lane) * 2);
-            // no key that the row sees: nothing, whatever the part's sums are
-            f = ml.x == -INFINITY ? 0.f : base2 ? exp2f(ml.x - m) : expf(ml.x - m);
-            l += ml.x == -INFINITY ? 0.f : f * ml.y;
-        }
-        const unsigned some = __ballot_sync(0xffffffffu, f != 0.f);
         const int n = min(parts - i0, 32);
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-            const float g = __shfl_sync(0xffffffffu, f, i);
-            if (!((some >> i) & 1)) continue;
-            const float* src = p.part + place(i0 + i) * dv + lane;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < n) ml = *(const float2*)(p.ml + place(i0 + lane) * 2);
+        const float m_new = fmaxf(m, warp_max(ml.x)), m_sub = m_new == -INFINITY ? 0.f : m_new;
+        // a part without a key that the row sees has no say, whatever its sums are
+        const float f = ml.x == -INFINITY ? 0.f : base2 ? exp2f(ml.x - m_sub) : expf(ml.x - m_sub);
+        const float old = m == -INFINITY ? 0.f : base2 ? exp2f(m - m_sub) : expf(m - m_sub);
+        l = l * old + (ml.x == -INFINITY ? 0.f : f * ml.y);
+        m = m_new;
+        const unsigned some = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+        if (i0)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (lane + 32 * k < dv) x[k] = fmaf(g, src[32 * k], x[k]);
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[k][q] *= old;
+        for (int i = 0; i < n; i += 8) {
+            float y[8][K][4];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (i + e < n && (some >> (i + e) & 1) && 4 * lane + 128 * k < dv) load4(p.part + place(i0 + i + e) * dv + 4 * lane + 128 * k, y[e][k]);
+                    else y[e][k][0] = y[e][k][1] = y[e][k][2] = y[e][k][3] = 0.f;
+                }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float g = __shfl_sync(0xffffffffu, f, (i + e) & 31);
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) x[k][q] = fmaf(g, y[e][k][q], x[k][q]);
+            }
         }
     }
     finish_row<T>(p, w, row0 + r, x, warp_sum(l));
@@ -226,7 +242,9 @@ int plain_grid(const zkfp_paged_attention_args& a)
 template <typename T>
 int launch_combine(const Paged& p, int base2, cudaStream_t st)
 {
-    fp_launch(paged_combine_kernel<T>, dim3((unsigned)p.grid, (unsigned)(p.tile + 3) / 4), dim3(128), 0, st, p, base2);
+    const dim3 grid((unsigned)p.grid, (unsigned)(p.tile + 3) / 4);
+    if (p.a.dv <= 128) fp_launch(paged_combine_kernel<T, 1>, grid, dim3(128), 0, st, p, base2);
+    else fp_launch(paged_combine_kernel<T, 2>, grid, dim3(128), 0, st, p, base2);
     return fp_launched();
 }
 

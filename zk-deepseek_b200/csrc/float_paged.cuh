@@ -304,34 +304,70 @@ __device__ __noinline__ void attend_row(const Paged& p, int b, int kv, int token
     for (int k = 0; k < 8; ++k) o[k] /= l;
 }
 
-// A warp finishes a row: x[k] is the weighted sum of column lane + 32 k, l the sum of the weights.
+// The row's columns from `begin` to `end` in `out`, from the definition
 template <typename T>
-__device__ __forceinline__ void finish_row(const Paged& p, const Walk& w, int row, float (&x)[8], float l)
+__device__ __noinline__ void finish_again(const Paged& p, int b, int kv, int token, int head, int pos, int begin, int end)
 {
-    const int lane = threadIdx.x & 31, in_seq = by_group(p, row), head = w.kv * p.group + row - in_seq * p.group;
-    const int token = w.row0 + in_seq, pos = w.len - w.n + in_seq;
-    if (pos < 0) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = 0.f;
-    } else {
-        bool finite = true;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (lane + 32 * k < p.a.dv) x[k] /= l;
-            else x[k] = 0.f;
-            finite = finite && isfinite(x[k]);
-        }
-        if (!__all_sync(0xffffffffu, finite)) attend_row<T>(p, w.b, w.kv, token, head, pos, x);
-    }
+    float x[8];
+    attend_row<T>(p, b, kv, token, head, pos, x);
+    const int lane = threadIdx.x & 31;
     T* out = (T*)p.a.out + (long long)token * p.a.o_tok + head * p.a.o_head;
     const T* gate = p.a.gate ? (const T*)p.a.gate + (long long)token * p.a.gate_tok + head * p.a.gate_head : nullptr;
+    __syncwarp();
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const int c = lane + 32 * k;
-        if (c >= p.a.dv) continue;
+        if (c < begin || c >= end) continue;
         if (gate) x[k] *= sigmoid_f(to_f32(gate[c])) * p.a.out_scale;
         out[c] = from_f32<T>(x[k]);
     }
+}
+
+__device__ __forceinline__ void load4(const float* p, float (&v)[4])
+{
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+__device__ __forceinline__ void load4(const bf16* p, float (&v)[4])
+{
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    v[0] = bf16_lo(x.x); v[1] = bf16_hi(x.x); v[2] = bf16_lo(x.y); v[3] = bf16_hi(x.y);
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(bf16* p, const float (&v)[4])
+{
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+}
+
+// A warp finishes a row: x[k] are the weighted sums of columns 4 lane + 128 k and the three behind, l is the sum of the weights.
+template <typename T, int K>
+__device__ __forceinline__ void finish_row(const Paged& p, const Walk& w, int row, float (&x)[K][4], float l)
+{
+    const int lane = threadIdx.x & 31, in_seq = by_group(p, row), head = w.kv * p.group + row - in_seq * p.group;
+    const int token = w.row0 + in_seq, pos = w.len - w.n + in_seq;
+    T* out = (T*)p.a.out + (long long)token * p.a.o_tok + head * p.a.o_head;
+    const T* gate = p.a.gate ? (const T*)p.a.gate + (long long)token * p.a.gate_tok + head * p.a.gate_head : nullptr;
+    float none = 0.f;                                  // stays zero where everything is finite
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = 4 * lane + 128 * k;
+        if (c >= p.a.dv) break;
+        float z[4];
+        if (gate) load4(gate + c, z);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[k][i] = pos < 0 ? 0.f : x[k][i] / l;
+            none = fmaf(x[k][i], 0.f, none);
+            if (gate) x[k][i] *= sigmoid_for<T>(z[i]) * p.a.out_scale;
+        }
+    }
+    if (!__all_sync(0xffffffffu, none == 0.f)) {
+        finish_again<T>(p, w.b, w.kv, token, head, pos, 0, p.a.dv);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (4 * lane + 128 * k < p.a.dv) store4(out + 4 * lane + 128 * k, x[k]);
 }
 
 // ---- kernels on the tensor cores (float_paged_tc.cu): whether they take a call, their tile and grid, and the launch -----

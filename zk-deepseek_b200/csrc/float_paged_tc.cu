@@ -11,10 +11,13 @@
 // memory, bfloat16 weights overwrite their scores and are the tensor-memory operand of the second product; while one tile is
 // in its softmax the tensor core works for the other.  The rows of a tile are (token, head) pairs, so that all heads of a
 // group share the keys that they read.
-//   warp 0      TMA loads          warp 1      MMA issue
+//   warp 0      the parts of items that the CTA takes, TMA loads
+//   warp 1      MMA issue
 //   warps 2-9   softmax, tile 0    warps 10-17 softmax, tile 1: two threads share a query row, half of the columns each
-// The running maximum only replaces the one in use when it has grown by more than 2^8; the output tile is then rescaled in
-// place.  CTAs stay and take one part of an item after the other.
+// The running maximum only replaces the one in use when it has grown by more than 2^8, and then in front of the next tile, where the
+// output tile is rescaled in place: a tile's weights are made from the maximum in use, without looking for the new one first (what
+// outgrows even 32 bits that way does not come out finite, and is taken again).  Weights go to the second product in halves, so that it
+// starts under the other half.  CTAs stay and take one part of an item after the other.
 #include <cuda.h>
 
 #include "float_paged.cuh"
@@ -36,13 +39,24 @@ __device__ __forceinline__ float exp2_approx(float x)
     return y;
 }
 
+// mbar_wait_warp without a time to be parked for, for the warp that the tensor core waits for (a prompt of 4096: 175 -> 170 us)
+__device__ __forceinline__ bool wait_awake(uint32_t bar, uint32_t parity, volatile int* abort_flag)
+{
+    for (uint32_t it = 0; it < kSpinLimit * 4; ++it) {
+        if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+        if ((it & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag)) return false;
+    }
+    *abort_flag = 1;
+    return false;
+}
+
 // ---- few rows ----------------------------------------------------------------------------------------------------
 constexpr int kStreamWarps = 4, kStretch = 16, kStreamRows = 16, kStreamKeys = kStreamWarps * kStretch, kStreamMost = 128;
 constexpr int kStretchSeg = kStretch * 128;            // bytes of 16 keys x 64 columns
 constexpr int kStreamStages = 4;
-// An item by itself costs about as much as 4 blocks of 64 keys, or 3 tiles of 128 (64 sequences up to 8192, microseconds, at 1, 2, 3, 4: 150,
-// 123, 107, 94; a chunk beside decoding sequences at 1, 3, 5: 221, 132, 137; a prompt 251, 206, 216).
-constexpr int kStreamOver = 4, kStreamLeast = 4, kTileOver = 3, kTileLeast = 3;
+// An item by itself costs about as much as 6 blocks of 64 keys, or 2 tiles of 128 (64 sequences up to 8192, microseconds, at 2, 3, 4, 5, 6: 127,
+// 110, 95, 91, 88; a chunk beside decoding sequences at 2, 3, 4: 116, 117, 119; a prompt 170, 171, 175).
+constexpr int kStreamOver = 6, kStreamLeast = 4, kTileOver = 2, kTileLeast = 2;
 
 struct StreamShape {
     int segk, segv, box, stages;
@@ -74,24 +88,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// A row of bfloat16 that did not come out finite, once more: its columns from `begin` to `end`.
-__device__ __noinline__ void finish_again(const Paged& p, int b, int kv, int token, int head, int pos, int begin, int end)
-{
-    const int lane = threadIdx.x & 31;
-    float x[8];
-    attend_row<bf16>(p, b, kv, token, head, pos, x);
-    bf16* out = (bf16*)p.a.out + (long long)token * p.a.o_tok + head * p.a.o_head;
-    const bf16* gate = p.a.gate ? (const bf16*)p.a.gate + (long long)token * p.a.gate_tok + head * p.a.gate_head : nullptr;
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int c = lane + 32 * k;
-        if (c < begin || c >= end) continue;
-        if (gate) x[k] *= sigmoid_f(__bfloat162float(gate[c])) * p.a.out_scale;
-        out[c] = __float2bfloat16_rn(x[k]);
-    }
 }
 
 // Where a warp stands: the part of an item that the CTA takes, and the block of keys that comes next.
@@ -128,33 +124,6 @@ struct Cursor {
         return part(p, plan, u1);
     }
 };
-
-// x[0 .. 3]: weighted sums of columns 4 lane .. 4 lane + 3 of a row, l the sum of its weights
-__device__ __forceinline__ void finish_four(const Paged& p, const Walk& w, int row, float (&x)[4], float l)
-{
-    const int lane = threadIdx.x & 31, in_seq = by_group(p, row), head = w.kv * p.group + row - in_seq * p.group;
-    const long long token = w.row0 + in_seq;
-    const bool mine = lane * 4 < p.a.dv, none = w.len - w.n + in_seq < 0;
-    const float r = none ? 0.f : 1.0f / l;
-    float z[4] = {};
-    if (p.a.gate && mine) {
-        const uint2 g = *(const uint2*)((const bf16*)p.a.gate + token * p.a.gate_tok + head * p.a.gate_head + lane * 4);
-        z[0] = bf16_lo(g.x); z[1] = bf16_hi(g.x); z[2] = bf16_lo(g.y); z[3] = bf16_hi(g.y);
-    }
-    bool finite = true;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        x[k] = none || !mine ? 0.f : x[k] * r;
-        finite = finite && isfinite(x[k]);
-        if (p.a.gate) x[k] *= sigmoid_for<bf16>(z[k]) * p.a.out_scale;
-    }
-    if (!__all_sync(0xffffffffu, finite)) {
-        finish_again(p, w.b, w.kv, (int)token, head, w.len - w.n + in_seq, 0, p.a.dv);
-        return;
-    }
-    if (mine)
-        *(uint2*)((bf16*)p.a.out + token * p.a.o_tok + head * p.a.o_head + lane * 4) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-}
 
 template <int SEGK, int SEGV>
 __global__ void __launch_bounds__(kStreamWarps * 32, 2)
@@ -367,7 +336,7 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (lane == 0) sums[warp] = mine;
         __syncthreads();
         for (int rr = warp; rr < rows; rr += kStreamWarps) {
-            float top = -INFINITY, sum = 0.f, x[4] = {};
+            float top = -INFINITY, sum = 0.f, x[1][4] = {};
 #pragma unroll
             for (int i = 0; i < kStreamWarps; ++i) top = fmaxf(top, M[i * kStreamRows + rr]);
 #pragma unroll
@@ -378,16 +347,16 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 sum = fmaf(g, L[i * kStreamRows + rr], sum);
                 if (lane * 4 < kPitch) {
                     const float4 y = *(const float4*)(sums[i] + (rr * kPitch + (((lane >> 1) ^ (rr & 7)) * 8) + (lane & 1) * 4) * 4);
-                    x[0] = fmaf(g, y.x, x[0]); x[1] = fmaf(g, y.y, x[1]);
-                    x[2] = fmaf(g, y.z, x[2]); x[3] = fmaf(g, y.w, x[3]);
+                    x[0][0] = fmaf(g, y.x, x[0][0]); x[0][1] = fmaf(g, y.y, x[0][1]);
+                    x[0][2] = fmaf(g, y.z, x[0][2]); x[0][3] = fmaf(g, y.w, x[0][3]);
                 }
             }
             if (at.whole) {
-                finish_four(p, w, row0 + rr, x, sum);
+                finish_row<bf16>(p, w, row0 + rr, x, sum);
                 continue;
             }
             const long long to = (2ll * cta + (at.begins ? 1 : 0)) * p.tile + rr;
-            if (lane * 4 < dv) *(float4*)(p.part + to * dv + lane * 4) = make_float4(x[0], x[1], x[2], x[3]);
+            if (lane * 4 < dv) store4(p.part + to * dv + lane * 4, x[0]);
             if (lane == 0) *(float2*)(p.ml + to * 2) = make_float2(top, sum);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");               // the places are loaded into again
@@ -411,41 +380,137 @@ struct TileParams {
     float scale_log2;
 };
 
+// The part of an item that a CTA takes: tiles of keys begin .. end - 1 in units of kTile positions (none: no part follows), those that query
+// tile g takes part in, and the rows of g.
+struct Part {
+    int begin, end, row0[2], rows[2], first[2], last[2];
+    int b, kv, token0, base;                   // sequence, key head, first token of the sequence, position of that
+    int begins, whole;
+};
+
+__device__ __forceinline__ Part part_of(const TileParams& t, const Walk& w, int taken)
+{
+    Part x;
+    const int all = w.n * t.p.group;
+    x.begin = w.begin(t.p);
+    x.end = w.end(t.p, taken);
+    x.begins = x.begin == 0;
+    x.whole = x.begins && x.end == w.count;
+    x.begin += w.first;
+    x.end += w.first;
+    x.b = w.b;
+    x.kv = w.kv;
+    x.token0 = w.row0;
+    x.base = w.len - w.n;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        x.row0[g] = w.t * t.p.tile + g * t.rows;
+        x.rows[g] = max(0, min(t.rows, all - x.row0[g]));
+        const int i0 = x.base + by_group(t.p, x.row0[g]), i1 = x.rows[g] > 0 ? x.base + by_group(t.p, x.row0[g] + x.rows[g] - 1) : -1;
+        const int lo = t.p.a.window > 0 ? max(i0 - t.p.a.window + 1, 0) / kTile : 0;
+        x.first[g] = max(x.begin, lo);
+        x.last[g] = i1 >= 0 ? min(x.end - 1, i1 / kTile) : x.first[g] - 1;
+    }
+    return x;
+}
+
 struct TileShared {
-    uint64_t q_full, q_empty, k_full[kMaxKeySlots], k_empty[kMaxKeySlots], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2];
-    float row_max[2][2][kTile];                // [query tile][column half][row]; at the end of an item the row sums
+    uint64_t q_full, q_empty, k_full[kMaxKeySlots], k_empty[kMaxKeySlots], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full[2], o_empty[2];
+    uint64_t part_full[2], part_empty[2];
+    __align__(16) uint8_t stage[16][1024];     // 32 bytes of the 32 rows of a warp
+    float most[4][2][2][kTile];                // [use][query tile][half][row], see below
+    Part part[2];
     uint32_t tmem;
     int abort;
 };
 
-// The part of an item that a CTA takes: tiles of keys begin .. end - 1 in units of kTile positions, those that query tile g
-// takes part in, and the rows of g.
-struct Part {
-    int begin, end, row0[2], rows[2], first[2], last[2];
-    int taken;                                 // units of the item, those for itself among them
-    bool begins, whole;
-    __device__ __forceinline__ Part(const TileParams& t, const Walk& w, long long left)
-    {
-        const int all = w.n * t.p.group, base = w.len - w.n;
-        taken = (int)min((long long)w.left(t.p), left);
-        begin = w.begin(t.p);
-        end = w.end(t.p, taken);
-        begins = begin == 0;
-        whole = begins && end == w.count;
-        begin += w.first;
-        end += w.first;
+// ---- the scores of a row -----------------------------------------------------------------------------------------
+// A thread has a row: 128 scores in tensor memory, 32 at a time in registers, the next 32 on their way.
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// largest score of 64 columns from c0 on
+template <bool MASKED>
+__device__ __forceinline__ float tile_max(uint32_t tS, int c0, int c_lo, int c_hi)
+{
+    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            row0[g] = w.t * t.p.tile + g * t.rows;
-            rows[g] = max(0, min(t.rows, all - row0[g]));
-            const int i0 = base + by_group(t.p, row0[g]), i1 = rows[g] > 0 ? base + by_group(t.p, row0[g] + rows[g] - 1) : -1;
-            const int lo = t.p.a.window > 0 ? max(i0 - t.p.a.window + 1, 0) / kTile : 0;
-            first[g] = max(begin, lo);
-            last[g] = i1 >= 0 ? min(end - 1, i1 / kTile) : first[g] - 1;
+    for (int q = 0; q < 2; ++q) {
+        float v[32];
+        tmem_ld32(tS + q * 32u, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const int c = c0 + q * 32 + i;
+            if (MASKED) {
+                if (c < c_lo || c > c_hi) v[i] = -INFINITY;
+                if (c + 1 < c_lo || c + 1 > c_hi) v[i + 1] = -INFINITY;
+            }
+            top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], v[i], v[i + 1]);
         }
     }
-    __device__ __forceinline__ bool active(int g, int j) const { return g ? j >= first[1] && j <= last[1] : j >= first[0] && j <= last[0]; }
-};
+    return fmaxf(top[0], top[1]);
+}
+
+// bfloat16 weights 2^(score * scale - sub) of the visible ones of 64 columns from c0 on, over their scores.  Gives their sum, and in `top` the
+// largest score.
+template <bool MASKED>
+__device__ __forceinline__ float weigh(uint32_t tS, int c0, int c_lo, int c_hi, uint64_t scale, uint64_t sub, float& top)
+{
+    float most[2] = {-INFINITY, -INFINITY};
+    uint64_t add[2] = {0, 0};
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        float v[32];
+        uint32_t x[16];
+        tmem_ld32(tS + q * 32u, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const int c = c0 + q * 32 + i;
+            if (MASKED) {
+                if (c < c_lo || c > c_hi) v[i] = -INFINITY;
+                if (c + 1 < c_lo || c + 1 > c_hi) v[i + 1] = -INFINITY;
+            }
+            most[(i >> 1) & 1] = max3(most[(i >> 1) & 1], v[i], v[i + 1]);
+            const uint64_t y = fma_pair(pair_of(v[i], v[i + 1]), scale, sub);
+            float e, f;
+            unpair(y, e, f);
+            e = exp2_approx(e);
+            f = exp2_approx(f);
+            add[(i >> 1) & 1] = add_pair(add[(i >> 1) & 1], pair_of(e, f));
+            x[i / 2] = pack_bf16(e, f);
+        }
+        tmem_st16(tS + q * 16u, x);
+    }
+    float e, f;
+    unpair(add_pair(add[0], add[1]), e, f);
+    top = fmaxf(most[0], most[1]);
+    return e + f;
+}
 
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -475,9 +540,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             mbar_init(smem_u32(&s.v_full[i]), 1);
             mbar_init(smem_u32(&s.v_empty[i]), 1);
             mbar_init(smem_u32(&s.s_full[i]), 1);
-            mbar_init(smem_u32(&s.p_full[i]), 8);
+            mbar_init(smem_u32(&s.p_full[i][0]), 4);
+            mbar_init(smem_u32(&s.p_full[i][1]), 4);
             mbar_init(smem_u32(&s.o_full[i]), 1);
             mbar_init(smem_u32(&s.o_empty[i]), 8);
+            mbar_init(smem_u32(&s.part_full[i]), 1);
+            mbar_init(smem_u32(&s.part_empty[i]), 17);         // the warp of MMAs, sixteen of softmax
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -491,21 +559,36 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const long long units = plan.before[a.batch];
     const int ctas = sharing(p, units), cta = blockIdx.x;
     const bool works = cta < ctas && units > 0;
-    long long u = works ? range_begin(units, cta, ctas) : 0;
-    const long long u1 = works ? range_begin(units, cta + 1, ctas) : 0;
-    Walk w;
-    if (works) w.locate(p, plan, u);
 
     if (warp == 0) {
         const uint32_t one = elect_one();
         int ks = 0, vs = 0;
         uint32_t kp = 0, vp = 0, qp = 0;
         bool ok = true;
+        long long u = works ? range_begin(units, cta, ctas) : 0;
+        const long long u1 = works ? range_begin(units, cta + 1, ctas) : 0;
+        Walk w;
+        if (works) w.locate(p, plan, u);
         if (one) no_cut(p, cta);
+        int slot = 0;
+        uint32_t phase = 0;
+        Part part;
+        auto publish = [&] {
+            if (!mbar_wait_warp(smem_u32(&s.part_empty[slot]), phase ^ 1u, abort_flag)) return false;
+            if (one) {
+                s.part[slot] = part;
+                mbar_arrive(smem_u32(&s.part_full[slot]));
+            }
+            slot ^= 1;
+            phase ^= slot == 0 ? 1u : 0u;
+            return true;
+        };
         while (u < u1 && ok) {
-            const Part part(t, w, u1 - u);
+            const int taken = (int)min((long long)w.left(p), u1 - u);
+            part = part_of(t, w, taken);
             if (part.begin == part.end) break;                 // units of an item that others take
             if (one && part.begins && !part.whole) write_cut(p, cta, units, ctas, w, u + w.left(p));
+            if (!(ok = publish())) break;
             if (!(ok = mbar_wait_warp(smem_u32(&s.q_empty), qp ^ 1u, abort_flag))) break;
             qp ^= 1u;
             const uint32_t row_bytes = (uint32_t)t.rows * 128u;
@@ -542,232 +625,258 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         tma_load_4d(dst + c * kSeg + i * t.box * 128, &tmV, c * 64, w.kv, line, __shfl_sync(0xffffffffu, mine, i), bar, one);
                 if (++vs == t.v_stages) { vs = 0; vp ^= 1u; }
             }
-            u += part.taken;
+            u += taken;
             if (u < u1) w.next(p, plan);
         }
+        part.begin = part.end = 0;
+        if (ok) publish();
     } else if (warp == 1) {
         const uint32_t one = elect_one(), tm = uniform(tmem);
         const uint32_t idesc_s = idesc_bf16(kTile, kTile), idesc_o = idesc_bf16(kTile, (a.dv + 15) & ~15, true);
-        uint32_t pp[2] = {0, 0}, op[2] = {0, 0}, kp = 0, vp = 0, qp = 0;
-        int ks = 0, vs = 0;
-        bool ok = true;
-        while (u < u1 && ok) {
-            Part part(t, w, u1 - u);
-            if (part.begin == part.end) break;
-            part.begin = (int)uniform(part.begin);
-            part.end = (int)uniform(part.end);
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                part.first[g] = (int)uniform(part.first[g]);
-                part.last[g] = (int)__reduce_max_sync(0xffffffffu, part.last[g]);
+        uint32_t pp[2] = {0, 0}, op[2] = {0, 0}, kp = 0, vp = 0, qp = 0, phase = 0;
+        int ks = 0, vs = 0, at = 0, begin = 0, end = 0, first[2] = {0, 0}, last[2] = {0, 0};
+        // the sums of query tile g over the keys that are there, and its scores with the tile of keys that follows
+        auto values = [&](const int g, int j) {
+            if (j == first[g]) {                               // the last part's sums have been read
+                if (!wait_awake(smem_u32(&s.o_empty[g]), op[g] ^ 1u, abort_flag)) return false;
+                op[g] ^= 1u;
             }
-            // the scores of query tile g with the keys at (ks, kp); `load` waits for their segments, `release` hands each back
-            auto scores = [&](int g, bool use, bool load, bool release) {
-                const uint32_t d = tm + (uint32_t)g * kTile;
-                int slot = ks;
-                uint32_t phase = kp;
-                for (int c = 0; c < t.seg; ++c) {
-                    if (load) {
-                        if (!mbar_wait_warp(smem_u32(&s.k_full[slot]), phase, abort_flag)) return false;
-                        tc_fence_after();
-                    }
-                    if (use) {
-                        const int cols = a.d - c * 64;
-                        const uint64_t ad = smem_desc_sw128(sQ + (uint32_t)g * bytesQ + (uint32_t)c * kSeg), bd = smem_desc_sw128(sK + (uint32_t)slot * kSeg);
+            const uint32_t ta = tm + g * kTile;
+            const uint64_t vd = smem_desc_mn_sw128(sV + (uint32_t)vs * bytesV, kSeg);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (k * 16 < cols) umma_bf16(d, ad + (uint64_t)(k * 2), bd + (uint64_t)(k * 2), idesc_s, (c | k) ? 1u : 0u, one);
-                    }
-                    if (release) umma_commit(smem_u32(&s.k_empty[slot]), one);
-                    if (++slot == t.k_slots) { slot = 0; phase ^= 1u; }
-                }
-                if (use) umma_commit(smem_u32(&s.s_full[g]), one);
-                if (release) { ks = slot; kp = phase; }
-                return true;
-            };
-            if (!(ok = mbar_wait_warp(smem_u32(&s.q_full), qp, abort_flag))) break;
-            qp ^= 1u;
-            for (int j = part.begin - 1; j < part.end && ok; ++j) {
-                if (j >= part.begin) {
-                    if (!(ok = mbar_wait_warp(smem_u32(&s.v_full[vs]), vp, abort_flag))) break;
+            for (int h = 0; h < 2; ++h) {
+                if (!wait_awake(smem_u32(&s.p_full[g][h]), pp[g], abort_flag)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < kTile / 32; ++k)
+                    umma_bf16_ts(ta + 256u, ta + (uint32_t)(h * 64 + k * 8), vd + (uint64_t)((h * kTile / 32 + k) * 128), idesc_o, (j != first[g] || h || k) ? 1u : 0u, one);
+            }
+            pp[g] ^= 1u;
+            if (j == last[g]) umma_commit(smem_u32(&s.o_full[g]), one);
+            return true;
+        };
+        // every segment is waited for once (by tile 0) and handed back once (by tile 1), also where neither has a use for it
+        auto scores = [&](const int g, int j) {
+            const bool use = j >= first[g] && j <= last[g];
+            int slot = ks;
+            uint32_t ph = kp;
+            for (int c = 0; c < t.seg; ++c) {
+                if (g == 0) {
+                    if (!wait_awake(smem_u32(&s.k_full[slot]), ph, abort_flag)) return false;
                     tc_fence_after();
                 }
-                for (int g = 0; g < 2 && ok; ++g) {
-                    if (j >= part.begin && part.active(g, j)) {
-                        const bool opens = j == (g ? part.first[1] : part.first[0]), closes = j == (g ? part.last[1] : part.last[0]);
-                        if (opens) {                           // the last item's sums have been read
-                            if (!(ok = mbar_wait_warp(smem_u32(&s.o_empty[g]), op[g] ^ 1u, abort_flag))) break;
-                            op[g] ^= 1u;
-                        }
-                        if (!(ok = mbar_wait_warp(smem_u32(&s.p_full[g]), pp[g], abort_flag))) break;
-                        pp[g] ^= 1u;
-                        tc_fence_after();
-                        const uint32_t ta = tm + (uint32_t)g * kTile, d = tm + 256u + (uint32_t)g * kTile;
-                        const uint64_t vd = smem_desc_mn_sw128(sV + (uint32_t)vs * bytesV, kSeg);
+                if (use) {
+                    const int cols = a.d - c * 64;
+                    const uint64_t ad = smem_desc_sw128(sQ + g * bytesQ + (uint32_t)c * kSeg), bd = smem_desc_sw128(sK + (uint32_t)slot * kSeg);
 #pragma unroll
-                        for (int k = 0; k < kTile / 16; ++k)
-                            umma_bf16_ts(d, ta + (uint32_t)k * 8u, vd + (uint64_t)(k * 128), idesc_o, (!opens || k) ? 1u : 0u, one);
-                        if (closes) umma_commit(smem_u32(&s.o_full[g]), one);
-                    }
-                    if (j >= part.begin && g == 1) umma_commit(smem_u32(&s.v_empty[vs]), one);
-                    // every segment is waited for once and handed back once, also when no query tile uses it
-                    if (j + 1 < part.end) {
-                        ok = scores(g, part.active(g, j + 1), g == 0, g == 1);
-                        if (ok && g == 1 && j + 2 == part.end) umma_commit(smem_u32(&s.q_empty), one);
-                    }
+                    for (int k = 0; k < 4; ++k)
+                        if (k * 16 < cols) umma_bf16(tm + g * kTile, ad + (uint64_t)(k * 2), bd + (uint64_t)(k * 2), idesc_s, (c | k) ? 1u : 0u, one);
                 }
-                if (!ok) break;
-                if (j >= part.begin && ++vs == t.v_stages) { vs = 0; vp ^= 1u; }
+                if (g == 1) umma_commit(smem_u32(&s.k_empty[slot]), one);
+                if (++slot == t.k_slots) { slot = 0; ph ^= 1u; }
             }
-            u += part.taken;
-            if (u < u1) w.next(p, plan);
+            if (use) umma_commit(smem_u32(&s.s_full[g]), one);
+            if (g == 1) { ks = slot; kp = ph; }
+            return true;
+        };
+        for (;;) {
+            if (!wait_awake(smem_u32(&s.part_full[at]), phase, abort_flag)) break;
+            begin = (int)uniform(s.part[at].begin);
+            end = (int)uniform(s.part[at].end);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                first[g] = (int)uniform(s.part[at].first[g]);
+                last[g] = __reduce_max_sync(0xffffffffu, s.part[at].last[g]);
+            }
+            if (one) mbar_arrive(smem_u32(&s.part_empty[at]));
+            __syncwarp();
+            at ^= 1;
+            phase ^= at == 0 ? 1u : 0u;
+            if (begin == end || !wait_awake(smem_u32(&s.q_full), qp, abort_flag)) break;
+            qp ^= 1u;
+            tc_fence_after();
+            bool ok = scores(0, begin) && scores(1, begin);
+            if (ok && begin + 1 == end) umma_commit(smem_u32(&s.q_empty), one);
+            for (int j = begin; j < end && ok; ++j) {
+                if (!(ok = wait_awake(smem_u32(&s.v_full[vs]), vp, abort_flag))) break;
+                tc_fence_after();
+                if (j >= first[0] && j <= last[0]) ok = values(0, j);
+                if (ok && j + 1 < end) ok = scores(0, j + 1);
+                if (ok && j >= first[1] && j <= last[1]) ok = values(1, j);
+                if (!ok) break;
+                umma_commit(smem_u32(&s.v_empty[vs]), one);
+                if (j + 1 < end) ok = scores(1, j + 1);
+                if (j + 2 == end) umma_commit(smem_u32(&s.q_empty), one);
+                if (++vs == t.v_stages) { vs = 0; vp ^= 1u; }
+            }
+            if (!ok) break;
         }
     } else {
         const int g = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane, c0 = half * 64;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const uint32_t tS = tmem + (uint32_t)g * kTile + lanes, tO = tmem + 256u + (uint32_t)g * kTile + lanes;
-        const int middle = (a.dv / 2 + 31) & ~31, o_begin = half ? middle : 0, o_end = half ? a.dv : min(a.dv, middle);
+        const uint32_t tS = tmem + (uint32_t)(g * kTile + c0) + lanes, tO = tmem + 256u + (uint32_t)g * kTile + lanes;
+        const int middle = (a.dv / 2 + 15) & ~15, o_begin = half ? middle : 0, o_end = half ? a.dv : min(a.dv, middle);
+        const uint64_t scale2 = twice(t.scale_log2);
         auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quarter) : "memory"); };
         uint32_t sp = 0, op = 0;
         bool ok = true;
-        while (u < u1 && ok) {
-            const Part part(t, w, u1 - u);
+        int at = 0;
+        uint32_t phase = 0;
+        for (;;) {
+            if (!(ok = mbar_wait_warp(smem_u32(&s.part_full[at]), phase, abort_flag))) break;
+            const Part& part = s.part[at];
             if (part.begin == part.end) break;
-            const int rows = part.rows[g], first_tile = part.first[g], last_tile = part.last[g], row_all = part.row0[g] + row;
-            const int in_seq = by_group(p, row_all), pos = row < rows ? w.len - w.n + in_seq : -1;
-            float m_used = -INFINITY, l = 0.f;
-            for (int j = first_tile; j <= last_tile && ok; ++j) {
+            const int rows = part.rows[g], first_tile = part.first[g], last_tile = part.last[g];
+            const int in_seq = by_group(p, part.row0[g] + row), pos = row < rows ? part.base + in_seq : -1;
+            // the maximum in use (in units of log2), the same in both threads of a row, and this one's sum of weights
+            float m = -INFINITY, l = 0.f;
+            for (int j = first_tile; j <= last_tile; ++j) {
                 if (!(ok = mbar_wait_warp(smem_u32(&s.s_full[g]), sp, abort_flag))) break;
                 sp ^= 1u;
                 tc_fence_after();
-                float v[2][32];
-                tmem_ld32(tS + (uint32_t)c0, v[0]);
-                tmem_ld32(tS + (uint32_t)c0 + 32u, v[1]);
-                // visible columns of this row: c_lo .. c_hi
-                const int c_hi = pos - j * kTile, c_lo = a.window > 0 ? c_hi - a.window + 1 : -1;
-                const bool masked = __any_sync(0xffffffffu, c_hi < kTile - 1 || c_lo > 0);
-                tmem_ld_wait();
-                if (masked) {
+                if (quarter * 32 < rows) {                // a warp without rows leaves the scores as weights that nothing reads
+                    // visible columns of this row: c_lo .. c_hi
+                    const int c_hi = pos - j * kTile, c_lo = a.window > 0 ? c_hi - a.window + 1 : -1;
+                    const bool masked = __any_sync(0xffffffffu, row < rows && (c_hi < kTile - 1 || c_lo > 0));
+                    // Both halves' largest scores of the tile in front: a thread leaves its own ahead of its weights, without which the next scores
+                    // are not made, in two places by turns.
+                    const float top = j == first_tile ? -INFINITY : fmaxf(s.most[j + 1 & 1][g][0][row], s.most[j + 1 & 1][g][1][row]) * t.scale_log2;
+                    if (__any_sync(0xffffffffu, top > m + 8.0f && m != -INFINITY)) {
+                        const float f = m == -INFINITY ? 1.f : exp2_approx(m - fmaxf(m, top));
+                        for (int c = o_begin; c < o_end; c += 8) {
+                            int32_t o[8];
+                            tmem_ld8(tO + (uint32_t)c, o);
+                            tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 64; ++c)
-                        if (c0 + c < c_lo || c0 + c > c_hi) v[c >> 5][c & 31] = -INFINITY;
-                }
-                float mp[8];                              // independent chains
-#pragma unroll
-                for (int i = 0; i < 8; ++i) mp[i] = v[0][i];
-#pragma unroll
-                for (int c = 8; c < 64; ++c) mp[c & 7] = fmaxf(mp[c & 7], v[c >> 5][c & 31]);
-                const float mine = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
-                                         fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
-                s.row_max[g][half][row] = mine;
-                // also: both threads of every row have read their scores before either overwrites any of them
-                pair_sync();
-                const float m_new = fmaxf(m_used, fmaxf(mine, s.row_max[g][half ^ 1][row]) * t.scale_log2);
-                if (j == first_tile) {
-                    m_used = m_new;
-                } else if (__any_sync(0xffffffffu, m_new > m_used + 8.0f)) {     // the same rows, so the same decision in both warps
-                    const float f = m_used == -INFINITY ? 0.f : exp2_approx(m_used - m_new);
-                    for (int c = o_begin; c < o_end; c += 8) {
-                        int32_t o[8];
-                        tmem_ld8(tO + (uint32_t)c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) o[i] = __float_as_int(__int_as_float(o[i]) * f);
-                        tmem_st8(tO + (uint32_t)c, o);
+                            for (int i = 0; i < 8; ++i) o[i] = __float_as_int(__int_as_float(o[i]) * f);
+                            tmem_st8(tO + (uint32_t)c, o);
+                        }
+                        l *= f;
+                        m = m == -INFINITY ? m : fmaxf(m, top);
                     }
-                    l *= f;
-                    m_used = m_new;
+                    if (__any_sync(0xffffffffu, m == -INFINITY)) {      // rows that have not seen a key yet
+                        s.most[2][g][half][row] = masked ? tile_max<true>(tS, c0, c_lo, c_hi) : tile_max<false>(tS, c0, 0, 0);
+                        pair_sync();
+                        if (m == -INFINITY) m = fmaxf(s.most[2][g][0][row], s.most[2][g][1][row]) * t.scale_log2;
+                    }
+                    const uint64_t sub = twice(m == -INFINITY ? 0.f : -m);
+                    float most;
+                    if (masked) l += weigh<true>(tS, c0, c_lo, c_hi, scale2, sub, most);
+                    else l += weigh<false>(tS, c0, 0, 0, scale2, sub, most);
+                    s.most[j & 1][g][half][row] = most;
+                    tmem_st_wait();
                 }
-                const float m_sub = m_used == -INFINITY ? 0.f : m_used;
-                float lp[4] = {};
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    uint32_t x[16];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[q][i] = exp2_approx(fmaf(v[q][i], t.scale_log2, -m_sub));
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) lp[i & 3] += v[q][i];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = pack_bf16(v[q][2 * i], v[q][2 * i + 1]);
-                    tmem_st16(tS + (uint32_t)(half * 32 + q * 16), x);
-                }
-                l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
-                tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&s.p_full[g]));
+                if (lane == 0) mbar_arrive(smem_u32(&s.p_full[g][half]));
             }
             if (!ok) break;
-            const bool any = first_tile <= last_tile;
+            const bool any = first_tile <= last_tile, writes = quarter * 32 < rows, whole = part.whole;
+            const int tok = part.token0 + in_seq, b = part.b, kv = part.kv, head = kv * p.group + part.row0[g] + row - in_seq * p.group;
+            const long long slot = (2ll * cta + (part.begins ? 1 : 0)) * p.tile + g * t.rows + row;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[at]));
+            at ^= 1;
+            phase ^= at == 0 ? 1u : 0u;
             if (any) {
-                pair_sync();                              // the last maxima have been read
-                s.row_max[g][half][row] = l;
-                pair_sync();
-                l += s.row_max[g][half ^ 1][row];
-                pair_sync();                              // the sums too, before the next item's maxima
                 if (!(ok = mbar_wait_warp(smem_u32(&s.o_full[g]), op, abort_flag))) break;
                 op ^= 1u;
                 tc_fence_after();
             }
-            const int head = w.kv * p.group + row_all - in_seq * p.group;
-            const long long token = w.row0 + in_seq;
-            if (part.whole) {
-                const float r = pos >= 0 ? 1.0f / l : 0.f;
-                bf16* out = (bf16*)a.out + token * a.o_tok + head * a.o_head;
-                const bf16* gate = a.gate ? (const bf16*)a.gate + token * a.gate_tok + head * a.gate_head : nullptr;
-                bool finite = true;
-                for (int c = o_begin; c < o_end; c += 8) {
-                    int32_t x[8] = {};
-                    if (any) {
-                        tmem_ld8(tO + (uint32_t)c, x);
-                        tmem_ld_wait();
-                    }
-                    if (row < rows) {
-                        float y[8];
+            if (writes) {
+                s.most[3][g][half][row] = l;
+                pair_sync();
+                l += s.most[3][g][half ^ 1][row];
+                // 32 bytes of every row pass through shared memory, so that a store meets 16 rows and not 32: lanes 2 r and 2 r + 1 take the
+                // halves of rows r and r + 16
+                uint8_t* stage = s.stage[warp - 2];
+                const int piece = lane & 1;
+                long long to[2], gate_at[2];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            y[k] = pos >= 0 ? __int_as_float(x[k]) * r : 0.f;
-                            finite = finite && isfinite(y[k]);
+                for (int k = 0; k < 2; ++k) {
+                    const int who = (lane >> 1) + 16 * k;
+                    const long long tk = __shfl_sync(0xffffffffu, tok, who), hd = __shfl_sync(0xffffffffu, head, who);
+                    to[k] = quarter * 32 + who >= rows ? -1 : whole ? tk * a.o_tok + hd * a.o_head : (slot - lane + who) * a.dv;
+                    gate_at[k] = tk * a.gate_tok + hd * a.gate_head;
+                }
+                auto at_stage = [&](int r, int i) { return (uint4*)(stage + r * 32 + ((i ^ (r >> 2)) & 1) * 16); };
+                if (whole) {
+                    const uint64_t r2 = twice(pos >= 0 ? 1.0f / l : 0.f);
+                    const bool blank = __any_sync(0xffffffffu, pos < 0);
+                    __nv_bfloat162 none = __float2bfloat162_rn(0.f);     // stays zero where everything is finite
+                    const __nv_bfloat162 zero = none;
+#pragma unroll 1
+                    for (int c = o_begin; c < o_end; c += 16) {
+                        float y[16] = {};
+                        if (any) {
+                            tmem_ldn(tO + (uint32_t)c, *reinterpret_cast<int32_t(*)[16]>(y));
+                            tmem_ld_wait();
                         }
-                        if (gate) {
-                            float z[8];
-                            load8(gate + c, z);
+                        const int col = c + 8 * piece;
+                        if (a.gate) {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) y[k] *= sigmoid_f(z[k]) * a.out_scale;
+                            for (int k = 0; k < 2; ++k)
+                                *at_stage((lane >> 1) + 16 * k, piece) = to[k] >= 0 && col < o_end ? *(const uint4*)((const bf16*)a.gate + gate_at[k] + col) : make_uint4(0, 0, 0, 0);
+                            __syncwarp();
                         }
-                        store8(out + c, y);
-                    }
-                    __syncwarp();
-                }
-                for (unsigned again = __ballot_sync(0xffffffffu, !finite); again; again &= again - 1) {
-                    const int who = __ffs(again) - 1, rr = part.row0[g] + quarter * 32 + who, tok = by_group(p, rr);
-                    finish_again(p, w.b, w.kv, w.row0 + tok, w.kv * p.group + rr - tok * p.group, w.len - w.n + tok, o_begin, o_end);
-                }
-            } else {
-                const long long at = (2ll * cta + (part.begins ? 1 : 0)) * p.tile + g * t.rows + row;
-                for (int c = o_begin; c < o_end; c += 8) {
-                    int32_t x[8] = {};
-                    if (any) {
-                        tmem_ld8(tO + (uint32_t)c, x);
-                        tmem_ld_wait();
-                    }
-                    if (row < rows) {
-                        float y[8];
+                        if (blank && pos < 0)
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) y[k] = __int_as_float(x[k]);
-                        store8(p.part + at * a.dv + c, y);
+                            for (int i = 0; i < 16; ++i) y[i] = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t x[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float e, f;
+                                unpair(fma_pair(pair_of(y[8 * k + 2 * i], y[8 * k + 2 * i + 1]), r2, 0), e, f);
+                                if (a.gate) {
+                                    const __nv_bfloat162 plain = __floats2bfloat162_rn(e, f);
+                                    if (c + 8 * k < o_end) none = __hfma2(plain, zero, none);
+                                    const uint32_t z = ((const uint32_t*)at_stage(lane, k))[i];
+                                    e *= sigmoid_for<bf16>(bf16_lo(z)) * a.out_scale;
+                                    f *= sigmoid_for<bf16>(bf16_hi(z)) * a.out_scale;
+                                }
+                                x[i] = pack_bf16(e, f);
+                                if (!a.gate && c + 8 * k < o_end) none = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&x[i]), zero, none);
+                            }
+                            *at_stage(lane, k) = make_uint4(x[0], x[1], x[2], x[3]);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            if (to[k] >= 0 && col < o_end) *(uint4*)((bf16*)a.out + to[k] + col) = *at_stage((lane >> 1) + 16 * k, piece);
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    const float2 bad = __bfloat1622float2(none);
+                    for (unsigned again = __ballot_sync(0xffffffffu, row < rows && !(bad.x == 0.f && bad.y == 0.f)); again; again &= again - 1) {
+                        const int who = __ffs(again) - 1;
+                        finish_again<bf16>(p, b, kv, __shfl_sync(0xffffffffu, tok, who), __shfl_sync(0xffffffffu, head, who), __shfl_sync(0xffffffffu, pos, who),
+                                           o_begin, o_end);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = o_begin; c < o_end; c += 8) {
+                        int32_t y[8] = {};
+                        if (any) {
+                            tmem_ld8(tO + (uint32_t)c, y);
+                            tmem_ld_wait();
+                        }
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) *at_stage(lane, k) = *reinterpret_cast<uint4*>(&y[4 * k]);
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            if (to[k] >= 0) *(uint4*)(p.part + to[k] + c + 4 * piece) = *at_stage((lane >> 1) + 16 * k, piece);
+                        __syncwarp();
+                    }
+                    if (row < rows) p.ml[slot * 2 + half] = half ? l : m;
                 }
-                if (row < rows) p.ml[at * 2 + half] = half ? l : m_used;
             }
             if (any) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s.o_empty[g]));
             }
-            u += part.taken;
-            if (u < u1) w.next(p, plan);
         }
     }
     tc_fence_before();
