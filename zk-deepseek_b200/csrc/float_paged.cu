@@ -1,4 +1,4 @@
-// Attention of new tokens over pages: the kernel of CUDA cores (float32, and sizes that the tensor cores do not take) and
+// Attention of new tokens over pages: the kernels of CUDA cores (float32, and sizes that the tensor cores do not take) and
 // the one that merges what the CTAs of a cut item leave.  How the work is shared is in float_paged.cuh.
 #include "float_paged.cuh"
 
@@ -6,7 +6,7 @@ namespace zkds {
 
 namespace {
 
-// ---- CUDA cores --------------------------------------------------------------------------------------------------
+// ---- CUDA cores, few rows ----------------------------------------------------------------------------------------
 // Tiles of 16 rows over blocks of 64 keys, all in shared memory, sums of a row in registers: a thread holds eight columns of
 // up to four rows.
 constexpr int kPlainRows = 16, kPlainKeys = 64, kPlainThreads = 128, kPlainMost = 256;
@@ -171,6 +171,199 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
     }
 }
 
+// ---- CUDA cores, more rows -----------------------------------------------------------------------------------------
+// Tiles of 32 rows over blocks of 64 keys, which bound it by multiply-adds: sixteen lanes own four rows.  Scores: four rows times four keys (16
+// apart) a thread, two products an instruction along the head, so that eight 16-byte loads feed 64 products; rows of keys are shifted by one
+// 16-byte piece against each other, which meets no bank twice.  The rows' maxima and sums are these lanes' own, and so are the weights, which pass through shared memory to the second product: four rows times every
+// sixteenth pair of columns.  Only the keys and values need the whole block to meet.
+constexpr int kBlockRows = 32, kBlockKeys = 64, kBlockThreads = 128, kWeightPitch = kBlockKeys + 4;
+
+struct BlockShape {
+    size_t smem;
+    int pairs;                                         // of columns a thread
+    BlockShape(const zkfp_paged_attention_args& a)
+    {
+        pairs = (a.dv + 31) / 32;
+        pairs = pairs <= 2 ? 2 : pairs <= 4 ? pairs : 8;
+        smem = plan_bytes(a.batch) + sizeof(float) * ((size_t)kBlockKeys * (a.d + 4 + a.dv) + (size_t)kBlockRows * a.d + kBlockRows * kWeightPitch);
+    }
+};
+
+template <typename T, int PAIRS>
+__global__ void __launch_bounds__(kBlockThreads)
+paged_block_kernel(const __grid_constant__ Paged p)
+{
+    chain_enter();
+    extern __shared__ __align__(16) uint8_t sm[];
+    const zkfp_paged_attention_args& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 31, d = a.d, dv = a.dv, vd = d / 8, pieces = vd + dv / 8, kpitch = d + 4, batch = (int)a.batch;
+    const Plan plan(sm, batch);
+    float* K = (float*)(sm + (((size_t)(batch + 1) * 8 + (size_t)batch * 12 + 15) & ~(size_t)15));            // [key][kpitch]
+    float* Q = K + kBlockKeys * kpitch;                                                                        // [row][d]
+    float* V = Q + kBlockRows * d;                                                                             // [key][dv]; at the end [row][dv]
+    float* P = V + kBlockKeys * dv;                                                                            // [row][key]
+    make_plan(p, plan);
+    const long long units = plan.before[batch];
+    const int ctas = sharing(p, units), cta = blockIdx.x;
+    if (tid == 0) no_cut(p, cta);
+    if (cta >= ctas || units == 0) return;
+    const long long u1 = range_begin(units, cta + 1, ctas);
+    long long u = range_begin(units, cta, ctas);
+    const int r4 = tid >> 4, at = tid & 15;            // which four rows, which of the sixteen
+    Walk w;
+    for (w.locate(p, plan, u); u < u1; w.next(p, plan)) {
+        const int taken = (int)min((long long)w.left(p), u1 - u), j_begin = w.begin(p), j_end = w.end(p, taken);
+        const long long end = u + w.left(p);
+        u += taken;
+        if (j_begin == j_end) continue;
+        const bool whole = j_begin == 0 && j_end == w.count;
+        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, units, ctas, w, end);
+        const int slot = 2 * cta + (j_begin == 0 ? 1 : 0), row0 = w.t * kBlockRows, rows = min(kBlockRows, w.n * p.group - row0);
+        __syncthreads();
+        for (int i = tid; i < kBlockRows * vd; i += kBlockThreads) {
+            const int r = i / vd, c = (i - r * vd) * 8;
+            float x[8] = {};
+            if (r < rows) {
+                const int t = by_group(p, row0 + r), h = w.kv * p.group + row0 + r - t * p.group;
+                load8((const T*)a.q + (long long)(w.row0 + t) * a.q_tok + h * a.q_head + c, x);
+            }
+            store8(Q + r * d + c, x);
+        }
+        int pos[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pos[i] = 4 * r4 + i < rows ? w.len - w.n + by_group(p, row0 + 4 * r4 + i) : -1;
+        int column[PAIRS];                             // behind the last one: that one again, without a branch, and not stored
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) column[k] = min(32 * k + 2 * at, dv - 2);
+        float m[4], l[4];
+        uint64_t acc[4][PAIRS];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) acc[i][k] = 0;
+        }
+        for (int j = j_begin; j < j_end; ++j) {
+            const int k0 = (w.first + j) * kBlockKeys;
+            __syncthreads();                           // the block in front is done with keys and values
+            {
+                // a warp takes every fourth key with its value, a lane a piece; lane i knows the page of the i-th
+                const int warp = tid >> 5, of = k0 + warp + 4 * (lane & 15);
+                const long long held = of < w.len ? page_of(p, w.b, of) : -1;
+                if (of < w.len && held < 0) *(volatile int*)p.error_flag = 1;
+                __syncwarp();
+                for (int c = lane; c < (pieces + 31) / 32 * 32; c += 32) {
+                    const bool key = c < vd;
+                    const T* base = key ? (const T*)a.k + w.kv * a.k_head + 8 * c : (const T*)a.v + w.kv * a.v_head + 8 * (c - vd);
+                    const long long page_step = key ? a.k_page : a.v_page, line_step = key ? a.k_pos : a.v_pos;
+                    float* to = key ? K + 8 * c : V + 8 * (c - vd);
+                    const int to_step = key ? kpitch : dv;
+#pragma unroll 8
+                    for (int i = 0; i < kBlockKeys / 4; ++i) {
+                        const int r = warp + 4 * i;
+                        const long long page = __shfl_sync(0xffffffffu, held, i);
+                        float x[8] = {};
+                        if (page >= 0 && c < pieces) load8(base + page * page_step + ((k0 + r) & (a.page - 1)) * line_step, x);
+                        if (c < pieces) store8(to + r * to_step, x);
+                    }
+                }
+            }
+            __syncthreads();
+            if (4 * r4 >= rows) continue;              // sixteen lanes without rows
+            uint64_t s[4][4] = {};                     // even and odd elements apart
+#pragma unroll 2
+            for (int c = 0; c < d; c += 4) {
+                ulonglong2 q[4], k[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    q[i] = *(const ulonglong2*)(Q + (4 * r4 + i) * d + c);
+                    k[i] = *(const ulonglong2*)(K + (at + 16 * i) * kpitch + c);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        fma2(s[i][e], q[i].x, k[e].x);
+                        fma2(s[i][e], q[i].y, k[e].y);
+                    }
+            }
+            const unsigned half = 0xffffu << (lane & 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[4], top = m[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = k0 + at + 16 * e;
+                    const bool seen = key <= pos[i] && (a.window <= 0 || pos[i] - key < a.window);
+                    v[e] = seen ? (__uint_as_float((uint32_t)s[i][e]) + __uint_as_float((uint32_t)(s[i][e] >> 32))) * a.scale : -INFINITY;
+                    top = fmaxf(top, v[e]);
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(half, top, o));
+                const float f = m[i] == -INFINITY ? 0.f : expf(m[i] - top);
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = v[e] == -INFINITY ? 0.f : expf(v[e] - top);
+                    sum += v[e];
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(half, sum, o);
+                l[i] = l[i] * f + sum;
+                m[i] = top;
+                const uint64_t f2 = twice(f);
+                uint64_t none = 0;
+#pragma unroll
+                for (int k = 0; k < PAIRS; ++k) {
+                    uint64_t y = none;
+                    fma2(y, acc[i][k], f2);
+                    acc[i][k] = y;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) P[(4 * r4 + i) * kWeightPitch + at + 16 * e] = v[e];
+            }
+            __syncwarp(half);
+            for (int key = 0; key < kBlockKeys; key += 4) {
+                float x[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) load4(P + (4 * r4 + i) * kWeightPitch + key, x[i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) {
+                        const uint64_t v = *(const uint64_t*)(V + (key + e) * dv + column[k]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) fma2(acc[i][k], v, twice(x[i][e]));
+                    }
+            }
+        }
+        __syncthreads();                               // the values make room for the sums
+        float* to = whole ? V : p.part + (long long)slot * p.tile * dv;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (4 * r4 + i >= rows) break;
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k)
+                if (32 * k + 2 * at < dv) *(uint64_t*)(to + (4 * r4 + i) * dv + 32 * k + 2 * at) = acc[i][k];
+            if (at == 0) {
+                if (whole) P[4 * r4 + i] = l[i];
+                else *(float2*)(p.ml + ((long long)slot * p.tile + 4 * r4 + i) * 2) = make_float2(m[i], l[i]);
+            }
+        }
+        if (whole) {
+            __syncthreads();
+            for (int r = tid >> 5; r < rows; r += kBlockThreads / 32) {
+                float x[2][4];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (4 * lane + 128 * k < dv) load4(V + r * dv + 4 * lane + 128 * k, x[k]);
+                finish_row<T>(p, w, row0 + r, x, P[r]);
+            }
+        }
+    }
+}
+
 // ---- cut items ---------------------------------------------------------------------------------------------------
 // Block x merges the item that CTA x began and did not end, a warp per row.  Maxima are in units of log2 where base2.  Lanes take the
 // parts' maxima and sums, 32 at a time, then all of them the columns of eight parts at a time.
@@ -259,6 +452,29 @@ int launch_plain(Paged& p, cudaStream_t st)
     return rc != ZKDS_OK ? rc : launch_combine<T>(p, 0, st);
 }
 
+template <typename T, int PAIRS>
+int launch_block(Paged& p, size_t smem, cudaStream_t st)
+{
+    ZKDS_CUDA(cudaFuncSetAttribute(paged_block_kernel<T, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax));
+    fp_launch(paged_block_kernel<T, PAIRS>, dim3((unsigned)p.grid), dim3(kBlockThreads), smem, st, p);
+    const int rc = fp_launched();
+    return rc != ZKDS_OK ? rc : launch_combine<T>(p, 0, st);
+}
+
+template <typename T>
+int launch_cores(Paged& p, cudaStream_t st)
+{
+    if (p.tile == kPlainRows) return launch_plain<T>(p, st);
+    const BlockShape s(p.a);
+    if (s.smem > (size_t)kSharedMax) return ZKDS_ERR_UNSUPPORTED;
+    switch (s.pairs) {
+    case 2: return launch_block<T, 2>(p, s.smem, st);
+    case 3: return launch_block<T, 3>(p, s.smem, st);
+    case 4: return launch_block<T, 4>(p, s.smem, st);
+    default: return launch_block<T, 8>(p, s.smem, st);
+    }
+}
+
 // grid and tile of the kernel that a call takes
 void choose(Paged& p)
 {
@@ -267,10 +483,16 @@ void choose(Paged& p)
     const int path = zkfp_paged_path(&p.a);
     if (path == 2) return paged_stream_shape(p);
     if (path == 1) return paged_tile_shape(p);
-    p.tile = kPlainRows;
     p.block = kPlainKeys;
-    p.over = 0;
-    p.least = 1;
+    p.over = 1;
+    p.least = 2;
+    if (p.a.max_tokens * p.group > kPlainRows) {
+        p.tile = kBlockRows;
+        const int per_sm = (int)(220 * 1024 / BlockShape(p.a).smem);
+        p.grid = fp_sm_count() * (per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm);
+        return;
+    }
+    p.tile = kPlainRows;
     p.grid = p.a.dtype == ZKFP_BF16 ? plain_grid<bf16>(p.a) : plain_grid<float>(p.a);
 }
 
@@ -332,7 +554,7 @@ int zkfp_paged_attention(const zkfp_paged_attention_args* a, void* stream)
         const int rc = path == 2 ? launch_paged_stream(p, st) : launch_paged_tile(p, st);
         return rc != ZKDS_OK ? rc : launch_combine<bf16>(p, 1, st);
     }
-    return a->dtype == ZKFP_BF16 ? launch_plain<bf16>(p, st) : launch_plain<float>(p, st);
+    return a->dtype == ZKFP_BF16 ? launch_cores<bf16>(p, st) : launch_cores<float>(p, st);
 }
 
 }  // extern "C"

@@ -189,10 +189,10 @@ struct Walk {
         }
         b = lo;
         sequence(p, s);
-        const long long per = (s.before[b + 1] - s.before[b]) / p.a.kv_heads;
-        long long rest = u - s.before[b];
-        kv = (int)(rest / per);
-        rest -= kv * per;
+        const long long mine = s.before[b + 1] - s.before[b], in = u - s.before[b];
+        const long long per = mine < 0x80000000ll ? (uint32_t)mine / (uint32_t)p.a.kv_heads : mine / p.a.kv_heads;
+        kv = (int)(in < 0x80000000ll && per < 0x80000000ll ? (uint32_t)in / (uint32_t)per : in / per);
+        long long rest = in - kv * per;
         const int lane = threadIdx.x & 31;
         for (int t0 = 0;; t0 += 32) {                  // ends: rest < per, the sum of all tiles
             int f = 0, c = -p.over;
@@ -242,7 +242,9 @@ struct Walk {
 __device__ __forceinline__ void no_cut(const Paged& p, int cta) { p.cut[cta * 8] = 0; }
 __device__ __forceinline__ void write_cut(const Paged& p, int cta, long long units, int ctas, const Walk& w, long long end)
 {
-    const long long behind = min((end * ctas + units - 1) / units, (long long)ctas);      // the first CTA whose range begins behind it
+    // the first CTA whose range begins behind it
+    const long long behind = end >= units ? ctas : units < 0x100000 ? ((uint32_t)end * (uint32_t)ctas + (uint32_t)units - 1) / (uint32_t)units
+                                                                    : (end * ctas + units - 1) / units;
     int4* to = (int4*)(p.cut + cta * 8);
     to[0] = make_int4((int)behind - cta, w.b, w.kv, w.t);
     to[1] = make_int4(w.row0, w.n, w.len, 0);
