@@ -599,10 +599,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     for (int c = 0; c < t.seg; ++c)
                         tma_load_4d(sQ + g * bytesQ + c * kSeg, &tmQ, c * 64, 0, w.kv, w.row0 + by_group(p, part.row0[g]), smem_u32(&s.q_full), one);
             for (int j = part.begin; j < part.end && ok; ++j) {
-                // pages of this tile of keys: lane i holds that of its i-th box
+                // pages of this tile of keys: lane i holds that of its i-th box, and asks for it
                 int mine = (int)a.pages;                       // beyond the tensor: zeros
                 const int at = j * kTile + lane * t.box;
-                if (lane * t.box < kTile && at < w.len) {
+                const uint32_t loads = lane * t.box < kTile;
+                if (loads && at < w.len) {
                     const long long page = page_of(p, w.b, at);
                     if (page >= 0) mine = (int)page;
                     else *(volatile int*)p.error_flag = 1;
@@ -613,16 +614,13 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     if (!(ok = mbar_wait_warp(smem_u32(&s.k_empty[ks]), kp ^ 1u, abort_flag))) break;
                     const uint32_t bar = smem_u32(&s.k_full[ks]), dst = sK + (uint32_t)ks * kSeg;
                     mbar_expect_tx(bar, kSeg, one);
-                    for (int i = 0; i * t.box < kTile; ++i)
-                        tma_load_4d(dst + i * t.box * 128, &tmK, c * 64, w.kv, line, __shfl_sync(0xffffffffu, mine, i), bar, one);
+                    tma_load_4d(dst + lane * t.box * 128, &tmK, c * 64, w.kv, line, mine, bar, loads);
                     if (++ks == t.k_slots) { ks = 0; kp ^= 1u; }
                 }
                 if (!ok || !(ok = mbar_wait_warp(smem_u32(&s.v_empty[vs]), vp ^ 1u, abort_flag))) break;
                 const uint32_t bar = smem_u32(&s.v_full[vs]), dst = sV + (uint32_t)vs * bytesV;
                 mbar_expect_tx(bar, bytesV, one);
-                for (int c = 0; c < t.segv; ++c)
-                    for (int i = 0; i * t.box < kTile; ++i)
-                        tma_load_4d(dst + c * kSeg + i * t.box * 128, &tmV, c * 64, w.kv, line, __shfl_sync(0xffffffffu, mine, i), bar, one);
+                for (int c = 0; c < t.segv; ++c) tma_load_4d(dst + c * kSeg + lane * t.box * 128, &tmV, c * 64, w.kv, line, mine, bar, loads);
                 if (++vs == t.v_stages) { vs = 0; vp ^= 1u; }
             }
             u += taken;

@@ -471,29 +471,40 @@ def copy_pages(buffers, source, target, positions=None):
     if not buffers or not n:
         return
     dev = _device(what, "a buffer", buffers[0])
-    list_ = (PageBuffer * len(buffers))()
+    layout, words = None, []                   # four words of a PageBuffer each; layers are mostly alike
     for i, t in enumerate(buffers):
-        if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dim() < 2:
-            _refuse(what, "buffer %d is no [pages, page, ...] tensor on cuda:%d" % (i, dev))
-        pages, lines, *rest = t.shape
-        stride, line, *inner = t.stride()
-        size = t.element_size()
-        row = math.prod(rest) * size
-        if positions is not None and not 0 <= positions <= lines:
-            _refuse(what, "%d positions of pages of %d" % (positions, lines))
-        if not pages or not lines or not row:
-            if pages <= max(max(source), max(target)):
-                _refuse(what, "buffer %d has %d pages" % (i, pages))
-            continue
-        dense = len(rest) == 1 and inner[0] == 1 and (line == rest[0] or lines == 1)
-        if not dense and not t[0].is_contiguous():
-            _refuse(what, "pages of buffer %d are not contiguous: strides %s" % (i, list(t.stride())))
-        at, whole, some = t.data_ptr(), row * lines, row * (lines if positions is None else positions)
-        stride = stride * size if pages > 1 else whole
-        if (at | stride | some) & 15:
-            _refuse(what, "pages of buffer %d, or the part of them that is copied, do not lie on 16-byte pieces" % i)
-        list_[i] = (at, stride, some, pages)
+        if not isinstance(t, torch.Tensor) or t.get_device() != dev:
+            _refuse(what, "buffer %d is no tensor on cuda:%d" % (i, dev))
+        this = t.shape, t.stride(), t.dtype
+        if this != layout:
+            layout, (stride, some, pages) = this, _page_layout(what, i, t, n, source, target, positions)
+        at = t.data_ptr()
+        if at & 15:
+            _refuse(what, "buffer %d does not lie on 16-byte pieces" % i)
+        words += (at, stride, some, pages)
+    list_ = ctypes.cast((_ll * len(words))(*words), ctypes.POINTER(PageBuffer))
     _call(_copy_pages, (list_, len(buffers), (_i * n)(*source), (_i * n)(*target), n), what, *buffers)
+
+
+def _page_layout(what, i, t, n, source, target, positions):
+    """bytes between pages, bytes of one that are copied, pages"""
+    if t.dim() < 2:
+        _refuse(what, "buffer %d is no [pages, page, ...] tensor" % i)
+    pages, lines = t.shape[:2]
+    if positions is not None and not 0 <= positions <= lines:
+        _refuse(what, "%d positions of pages of %d" % (positions, lines))
+    if pages <= max(max(source), max(target)) or min(min(source), min(target)) < 0:
+        _refuse(what, "pages that buffer %d of %d does not have" % (i, pages))
+    if t.numel() == 0:
+        return 0, 0, pages
+    if not t[0].is_contiguous():
+        _refuse(what, "pages of buffer %d are not contiguous: strides %s" % (i, list(t.stride())))
+    whole = t[0].numel() * t.element_size()
+    some = whole if positions is None else whole // lines * positions
+    stride = t.stride(0) * t.element_size() if pages > 1 else whole
+    if (stride | some) & 15 or stride < whole:
+        _refuse(what, "pages of buffer %d, or the part of them that is copied, do not lie on 16-byte pieces of their own" % i)
+    return stride, some, pages
 
 
 def sample(logits, random, out=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
