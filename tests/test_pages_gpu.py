@@ -438,3 +438,237 @@ def test_the_program_draws_tokens_on_pages(float_libpath, tmp_path, capsys):
         lines.append([json.loads(x) for x in capsys.readouterr().out.splitlines()])
         assert [len(x) for x in lines[-1]] == [6] * 3
     assert lines[0] == lines[1] and lines[2][0] == lines[2][1] == lines[2][2]
+
+
+# ---- calls that the documentation allows -------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 40])
+def test_captured_calls_follow_their_inputs(K, dtype, new):
+    """one graph of write, attention and sampling; rows, lengths, table and values change between replays; a second graph of the same
+    calls in between"""
+    B, page, H, G, d = 3, 16, 4, 2, 64
+    a, b = (pool(dtype, [new] * B, lengths, page, H, G, d, d, seed=s) for s, lengths in ((1, [200, 90, 64]), (2, [41, 230, 77])))
+    cols = max(a["table"].shape[1], b["table"].shape[1])
+    pages = max(a["k"].shape[0], b["k"].shape[0])
+    st = dict(q=a["q"].clone(), table=torch.zeros(B, cols, dtype=torch.int32, device="cuda"), rows=a["rows"].clone(), lengths=a["lengths"].clone(),
+              pool=torch.zeros(pages, page, 2 * G * d, dtype=a["q"].dtype, device="cuda"), out=torch.empty_like(a["q"]),
+              u=torch.rand(B * new, device="cuda"), token=torch.empty(B * new, dtype=torch.int64, device="cuda"), nk=rnd((B * new, G, d), dtype, 7))
+    kp, vp = st["pool"][..., :G * d].unflatten(2, (G, d)), st["pool"][..., G * d:].unflatten(2, (G, d))
+
+    def put(s):
+        st["q"].copy_(s["q"])
+        st["table"][:, :s["table"].shape[1]].copy_(s["table"])
+        st["rows"].copy_(s["rows"])
+        st["lengths"].copy_(s["lengths"])
+        kp[:s["k"].shape[0]].copy_(s["k"].nan_to_num(0.0))
+        vp[:s["v"].shape[0]].copy_(s["v"].nan_to_num(0.0))
+
+    def calls():
+        K.write_pages(st["nk"], st["nk"], kp, vp, st["table"], st["rows"], st["lengths"])
+        K.paged_attention(st["q"], kp, vp, st["table"], st["rows"], st["lengths"], st["out"], 0.1, window=120, max_tokens=new)
+        K.sample(st["out"].flatten(1), st["u"], st["token"], temperature=0.7, top_k=30, top_p=0.9)
+
+    def plain(s):
+        put(s)
+        calls()
+        return st["out"].clone(), st["token"].clone()
+
+    want = [plain(s) for s in (a, b)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g in graphs:
+        with torch.cuda.graph(g):
+            calls()
+    for i in (0, 1, 0):
+        for g in graphs:
+            put((a, b)[i])
+            st["out"].zero_()
+            st["token"].zero_()
+            g.replay()
+            # the same bits: nothing depends on the timing of a run
+            assert torch.equal(st["out"], want[i][0]) and torch.equal(st["token"], want[i][1])
+    K.device_status(sync=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_calls_at_once_on_streams_of_their_own(K, dtype):
+    s = [pool(dtype, [1 + 60 * (i % 2)] * 2, [700, 300], 32, 8, 2, 64, 64, seed=i, fill=0.0) for i in range(4)]
+    logits = [rnd((40, 5000), dtype, i, 2.0) for i in range(4)]
+    u = torch.rand(40, generator=torch.Generator().manual_seed(3)).cuda()
+    want = [(attend(K, x, dtype, 0.1).clone(), K.sample(l, u, top_p=0.9)) for x, l in zip(s, logits)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in s]
+    for _ in range(5):
+        got = []
+        for x, l, stream in zip(s, logits, streams):
+            with torch.cuda.stream(stream):
+                got.append((attend_quietly(K, x, dtype), K.sample(l, u, top_p=0.9)))
+        torch.cuda.synchronize()
+        for (o, t), (wo, wt) in zip(got, want):
+            assert torch.equal(o, wo) and torch.equal(t, wt)
+
+
+def attend_quietly(K, s, dtype):
+    """attend without its host checks, which wait"""
+    out = torch.empty(s["q"].shape[:2] + s["v"].shape[3:], dtype=s["q"].dtype, device="cuda")
+    return K.paged_attention(s["q"], s["k"], s["v"], s["table"], s["rows"], s["lengths"], out, 0.1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 3, 80])
+def test_strided_heads(K, dtype, new):
+    """queries, gate and result as parts of wider rows, in another order of heads and tokens"""
+    s = pool(dtype, [new, 2], [150, 40], 16, 6, 3, 40, 24, fill=0.0, pad=24)
+    n, gate = new + 2, rnd((new + 2, 6, 24), dtype, 9)
+    want = attend(K, s, dtype, 0.2, 33, gate, 0.9)
+    wide = rnd((n, 6 * 40 + 6 * 24 + 16), dtype, 4)
+    q, g = wide[:, :240].unflatten(1, (6, 40)), wide[:, 240:384].unflatten(1, (6, 24))
+    q.copy_(s["q"])
+    g.copy_(gate)
+    out = torch.zeros(6, n, 32, dtype=q.dtype, device="cuda").transpose(0, 1)[..., :24]         # heads first
+    K.paged_attention(q, s["k"], s["v"], s["table"], s["rows"], s["lengths"], out, 0.2, window=33, gate=g, out_scale=0.9, max_tokens=new)
+    assert torch.equal(out, attend(K, s, dtype, 0.2, 33, gate, 0.9, max_tokens=new))
+    assert (out.double() - want.double()).abs().max() <= 6 * HALF[dtype] * float(want.abs().max()) + 1e-5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pages_beyond_32_bit_offsets(K, dtype):
+    """the last pages of a pool of more than 2^32 bytes, and of 2^31 elements"""
+    G, d, page, pages = 8, 128, 64, 16500
+    small = pool(dtype, [2, 70], [100, 70], page, 16, G, d, d, fill=0.0)
+    big = torch.empty(pages, page, 2 * G * d, dtype=getattr(torch, dtype), device="cuda")
+    assert big.numel() > 2 ** 31 and big.numel() * big.element_size() > 2 ** 32
+    n = small["k"].shape[0]
+    kp, vp = big[..., :G * d].unflatten(2, (G, d)), big[..., G * d:].unflatten(2, (G, d))
+    kp[-n:], vp[-n:] = small["k"], small["v"]
+    table = torch.where(small["table"] >= 0, small["table"] + (pages - n), small["table"])
+    for kw in (dict(max_tokens=1), dict()):
+        out, want = torch.empty_like(small["q"]), torch.empty_like(small["q"])
+        K.paged_attention(small["q"], kp, vp, table, small["rows"], small["lengths"], out, 0.09, **kw)
+        K.paged_attention(small["q"], small["k"], small["v"], small["table"], small["rows"], small["lengths"], want, 0.09, **kw)
+        assert torch.equal(out, want)
+    new = rnd((72, G, d), dtype, 5)
+    K.write_pages(new, new, kp, vp, table, small["rows"], small["lengths"])
+    last = small["host"][0][1][1] + pages - n
+    assert torch.equal(kp[last, 5], new[-1]) and torch.equal(vp[last, 5], new[-1])
+    K.copy_pages([big], [int(last)], [7])
+    assert torch.equal(big[7], big[int(last)])
+    K.device_status(sync=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,heads,kv", [(1024, 2, 1), (1, 130, 1), (2, 128, 1), (300, 12, 12)])
+def test_many_sequences_and_many_heads_of_a_group(K, dtype, batch, heads, kv):
+    g = np.random.default_rng(batch)
+    lengths = g.integers(1, 30, batch).tolist()
+    for new in ([1] * batch, [min(n, int(k)) for n, k in zip(lengths, g.integers(0, 4, batch))]):
+        check(K, pool(dtype, new, lengths, 8, heads, kv, 16, 16, fill=0.0), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 40])
+def test_what_does_not_fit_is_reported(K, dtype, new):
+    """page numbers outside the pool, more positions than the table has columns for, rows outside the batch: nothing of it is read or
+    written, the other sequences come out right, and the status says so"""
+    s = pool(dtype, [new, new, new], [100, 90, 60], 16, 4, 2, 64, 64, fill=0.0)
+    want = attend(K, s, dtype, 0.1)
+    K.device_status(sync=True)
+
+    def wrong(name, edit, whole):
+        kept = s[name].clone()
+        edit(s[name])
+        out = attend(K, s, dtype, 0.1)
+        torch.cuda.synchronize()
+        with pytest.raises(K.FloatOpsError):
+            K.device_status(sync=True)
+        for b in whole:                        # other lengths are cut elsewhere, so that sums come in another order
+            mine = (out - want)[b * new:(b + 1) * new].double().abs().max()
+            assert mine <= 4 * HALF[dtype] * float(want.abs().max()) + 1e-5
+        before = s["k"].clone()
+        K.write_pages(torch.ones_like(s["q"][:, :2]), torch.ones_like(s["q"][:, :2]), s["k"], s["v"], s["table"], s["rows"], s["lengths"])
+        torch.cuda.synchronize()
+        s["k"].copy_(before)
+        try:
+            K.device_status(sync=True)
+        except K.FloatOpsError:
+            pass
+        s[name].copy_(kept)
+
+    def page(value):
+        def edit(t):
+            t[1, 3] = value
+        return edit
+    values = s["v"].clone()
+    for value in (-1, s["k"].shape[0], 2 ** 31 - 1, -2 ** 31):
+        wrong("table", page(value), [0, 2])
+        s["v"].copy_(values)
+    for value in (16 * s["table"].shape[1] + 1, 2 ** 31 - 1, -5, -2 ** 31):
+        wrong("lengths", lambda t: t[1:2].fill_(value), [0, 2])
+        s["v"].copy_(values)
+    wrong("rows", lambda t: t[3:].fill_(3 * new + 50), [0, 1])
+    s["v"].copy_(values)
+    wrong("rows", lambda t: t[2:3].fill_(-7), [0])
+    s["v"].copy_(values)
+    wrong("rows", lambda t: t[1:2].fill_(2 ** 31 - 1), [2])
+    s["v"].copy_(values)
+    assert torch.equal(attend(K, s, dtype, 0.1), want)
+    K.device_status(sync=True)
+
+
+def test_sampling_takes_any_number(K):
+    """random numbers outside [0, 1) and settings that no row should have name a kept token all the same"""
+    l = rnd((1, 300), "float32", 2, 2.0)
+    kept = set(fo.kept_tokens(np64(l)[0], 1.0, 5, 1.0, 0.0)[0].tolist())
+    for u in (1.0, -1.0, 7.0, float("nan"), float("inf"), -float("inf")):
+        assert int(K.sample(l, torch.tensor([u], device="cuda"), top_k=5)) in kept
+    f = lambda x: torch.tensor([x], dtype=torch.float32, device="cuda")
+    best = int(l.argmax())
+    half = f(0.5)
+    assert int(K.sample(l, half, temperature=f(float("nan")))) == best and int(K.sample(l, half, temperature=f(-1.0))) == best
+    assert int(K.sample(l, half, temperature=f(1e-30))) == best and int(K.sample(l, half, min_p=f(5.0))) == best
+    assert int(K.sample(l, half, top_k=torch.tensor([-3], dtype=torch.int32, device="cuda"))) == fo.sample(np64(l)[0], 0.5)
+    assert int(K.sample(l, half, temperature=float("inf"))) == 150 and int(K.sample(l, half, top_p=f(float("nan")))) == fo.sample(np64(l)[0], 0.5)
+
+
+def test_calls_refuse_what_does_not_belong_together(K):
+    s = pool("bfloat16", [2, 1], [30, 9], 16, 4, 2, 64, 64, fill=0.0)
+    q, out, half = s["q"], torch.empty_like(s["q"]), s["q"].half()
+    base = dict(q=q, k_pages=s["k"], v_pages=s["v"], table=s["table"], rows=s["rows"], lengths=s["lengths"], out=out, scale=0.1)
+    K.paged_attention(**base)
+    for bad in (dict(q=half), dict(q=q.float()), dict(out=out.float()), dict(q=q[:, :3]), dict(q=q[:2]), dict(q=q[..., :32]), dict(q=q.cpu()), dict(out=q),
+                dict(table=s["table"].long()), dict(table=s["table"][0]), dict(rows=s["rows"][:2]), dict(lengths=s["lengths"][:1]), dict(scale=-0.1),
+                dict(window=-1), dict(max_tokens=-1), dict(k_pages=s["k"][:, :12]), dict(v_pages=s["v"][:, :8]), dict(v_pages=s["v"].float()),
+                dict(gate=q[..., :32]), dict(q=torch.empty(3, 4, 68, device="cuda", dtype=q.dtype)[..., 4:]), dict(k_pages=s["k"][:0], v_pages=s["v"][:0]),
+                dict(table=s["table"].t().contiguous().t()), dict(q=[1.0])):
+        with pytest.raises(ValueError):
+            K.paged_attention(**{**base, **bad})
+    with pytest.raises(K.FloatOpsError):
+        big = torch.zeros(2, 16, 1, 264, dtype=q.dtype, device="cuda")
+        x = torch.zeros(3, 1, 264, dtype=q.dtype, device="cuda")
+        K.paged_attention(x, big, big, s["table"], s["rows"], s["lengths"], torch.empty_like(x), 0.1)
+    k, cs = rnd((3, 2, 64), "bfloat16"), torch.zeros(9, 32, 2, device="cuda")
+    base = dict(k=k, v=k, k_pages=s["k"], v_pages=s["v"], table=s["table"], rows=s["rows"], lengths=s["lengths"], q=q, q_out=out, cos_sin=cs)
+    K.write_pages(**base)
+    for bad in (dict(k=k[:2]), dict(v=k[:, :1]), dict(q=None), dict(q_out=None), dict(q=q[:2]), dict(q_out=out[:, :2]), dict(layout="other"),
+                dict(cos_sin=cs.double()), dict(cos_sin=cs[..., :1]), dict(cos_sin=torch.zeros(9, 33, 2, device="cuda")), dict(cos_sin=cs[:, ::2]), dict(k=k.float())):
+        with pytest.raises(ValueError):
+            K.write_pages(**{**base, **bad})
+    b = torch.zeros(6, 16, 8, dtype=q.dtype, device="cuda")
+    for bufs, src, dst, n in (([b], [0], [6], None), ([b], [0], [-1], None), ([b], [6], [0], None), ([b], [0], [1], 17), ([b], [0], [1], -1), ([b.cpu()], [0], [1], None),
+                              ([b[:, :, :4]], [0], [1], None), ([b[0, 0]], [0], [1], None), ([b[:1].expand(6, 16, 8)], [0], [1], None), ([b, b[:3]], [0], [5], None),
+                              ([torch.zeros(6, 16, 9, device="cuda", dtype=q.dtype)], [0], [1], 1)):
+        with pytest.raises(ValueError):
+            K.copy_pages(bufs, src, dst, positions=n)
+    for src, dst in (([0, 1], [2, 2]), ([0, 2], [2, 3])):
+        with pytest.raises(K.FloatOpsError):
+            K.copy_pages([b], src, dst)
+    l, u = rnd((3, 50), "float32"), torch.zeros(3, device="cuda")
+    for bad in (dict(random=u[:2]), dict(random=u.double()), dict(logits=l.double()), dict(logits=l.t()), dict(logits=l[0]), dict(out=u), dict(temperature=-1.0),
+                dict(top_k=1.5), dict(top_k=torch.zeros(3, device="cuda")), dict(top_p=torch.zeros(2, device="cuda")), dict(min_p=float("nan")),
+                dict(random=torch.zeros(6, device="cuda")[::2])):
+        with pytest.raises(ValueError):
+            K.sample(**{**dict(logits=l, random=u), **bad})
+    # nothing to do
+    none = torch.empty(0, 4, 64, dtype=q.dtype, device="cuda")
+    assert K.paged_attention(none, s["k"], s["v"], s["table"], s["rows"], s["lengths"], none.clone(), 0.1).shape == (0, 4, 64)
+    assert K.sample(l[:0], u[:0]).shape == (0,)
+    K.device_status(sync=True)

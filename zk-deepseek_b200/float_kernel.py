@@ -404,7 +404,8 @@ def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, windo
     the positions up to its own, with window > 0 the last `window` of them.  A row at a negative position (a sequence
     with more rows than positions) sees none and gives zeros; rows behind the last sequence are left as they were.
     max_tokens: most rows that a sequence brings (default: all), which chooses the kernel.  gate [tokens, heads, dv]: out is
-    multiplied by sigmoid(gate) * out_scale."""
+    multiplied by sigmoid(gate) * out_scale.  Head sizes up to 256, up to 1024 sequences; scale is not negative; out lies on no
+    input."""
     what = "paged_attention"
     dev, dt, kp, ks, vp, vs, tp, rp, lp, ld, batch, cols, pages, page, kv, d, dv = _pool(what, k_pages, v_pages, table, rows, lengths)
     qp, qs = _heads(what, "q", q, dt, 3, dev)
@@ -418,6 +419,8 @@ def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, windo
         max_tokens = tokens
     if window < 0 or max_tokens < 0 or not 0 <= scale < 3e38:
         _refuse(what, "a negative window, bound or scale")
+    if tokens and op in (qp, gp, kp, vp):
+        _refuse(what, "out lies on an input")
     if tokens:
         a = PagedAttentionArgs(qp, kp, vp, op, gp, tp, rp, lp, None, *qs, *ks, *vs, *os, *gs, tokens, pages, cols, ld, batch, max_tokens, heads,
                                kv, d, dv, page, min(window, 0x7fffffff), code(dt), scale, out_scale)
