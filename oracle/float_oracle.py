@@ -242,7 +242,7 @@ def paged_attention(q, k_pages, v_pages, table, rows, lengths, scale, window=0, 
     size, score = np.zeros_like(out), np.zeros(q.shape[:2])
     for b, length in enumerate(lengths):
         k, v = gather_pages(k_pages, table[b], length), gather_pages(v_pages, table[b], length)
-        n = rows[b + 1] - rows[b]
+        n = int(rows[b + 1] - rows[b])
         for t in range(n):
             i, r = length - n + t, rows[b] + t
             lo = max(0, i - window + 1) if window else 0

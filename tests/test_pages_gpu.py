@@ -672,3 +672,61 @@ def test_calls_refuse_what_does_not_belong_together(K):
     assert K.paged_attention(none, s["k"], s["v"], s["table"], s["rows"], s["lengths"], none.clone(), 0.1).shape == (0, 4, 64)
     assert K.sample(l[:0], u[:0]).shape == (0,)
     K.device_status(sync=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,lengths", [([5], [3]), ([40, 2], [7, 0]), ([200], [130]), ([1, 70], [90, 300])])
+def test_a_window_of_any_size(K, dtype, new, lengths):
+    """windows as long as the cache and longer, up to beyond 32 bits, see what no window sees, rows at negative positions among them"""
+    s = pool(dtype, new, lengths, 16, 4, 2, 64, 64, fill=0.0)
+    want = attend(K, s, dtype, 0.1)
+    for window in (max(lengths), 2 ** 31 - 1, 2 ** 40):
+        assert torch.equal(attend(K, s, dtype, 0.1, window), want)
+    check(K, s, dtype, 0.1, 2 ** 31 - 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 2, 90])
+def test_expanded_heads(K, dtype, new):
+    """keys and values that all heads share, queries that all tokens or all heads share, none of them copied"""
+    s = pool(dtype, [new, 1], [150, 40], 16, 4, 2, 64, 64, fill=0.0)
+    s["k"], s["v"] = s["k"][:, :, :1].expand(-1, -1, 2, -1), s["v"][:, :, :1].expand(-1, -1, 2, -1)
+    check(K, s, dtype)
+    s = pool(dtype, [new, 1], [150, 40], 16, 4, 2, 64, 64, seed=3, fill=0.0)
+    table, rows, lengths = s["host"]
+    for q in (s["q"][:1].expand(new + 1, -1, -1), s["q"][:, :1].expand(-1, 4, -1)):
+        out = K.paged_attention(q, s["k"], s["v"], s["table"], s["rows"], s["lengths"], torch.empty_like(s["q"]), 0.125)
+        want, size, score = fo.paged_attention(np64(q), np64(s["k"]), np64(s["v"]), table, rows, lengths, 0.125)
+        assert (np.abs(np64(out) - want) <= limit(dtype, size, score, 64, 150) + HALF[dtype] * np.abs(want)).all()
+    q = s["q"]
+    with pytest.raises(ValueError):
+        K.paged_attention(q, s["k"], s["v"], s["table"], s["rows"], s["lengths"], q[:, :1].clone().expand(-1, 4, -1), 0.125)
+    new_k = q[:, :2].contiguous()
+    for bad in (dict(k_pages=s["k"][:, :, :1].expand(-1, -1, 2, -1)), dict(v_pages=s["v"][:1].expand(s["v"].shape)),
+                dict(q_out=q[:, :1].clone().expand(-1, 4, -1))):
+        with pytest.raises(ValueError):
+            K.write_pages(**{**dict(k=new_k, v=new_k, k_pages=s["k"], v_pages=s["v"], table=s["table"], rows=s["rows"], lengths=s["lengths"], q=q, q_out=q), **bad})
+    K.device_status(sync=True)
+
+
+@pytest.mark.parametrize("rows,lengths", [([0, 3, 9], [20, 20]), ([-2, 3, 6], [20, 20]), ([0, 3, 6], [-1, 20])])
+def test_rows_that_do_not_fit_are_reported_when_written(K, rows, lengths):
+    s = pool("float32", [3, 3], [20, 20], 16, 2, 2, 32, 32, fill=0.0)
+    before, x = s["k"].clone(), torch.ones(6, 2, 32, device="cuda")
+    K.write_pages(x, x, s["k"], s["v"], s["table"], i32(*rows), i32(*lengths))
+    torch.cuda.synchronize()
+    with pytest.raises(K.FloatOpsError):
+        K.device_status(sync=True)
+    # the sequence that fits is written, the other one is not
+    b = 0 if rows[2] == 9 else 1
+    table = s["host"][0]
+    page = int(table[b][1])
+    assert (s["k"][page, 1:4] == 1).all()
+    s["k"][page, 1:4] = before[page, 1:4]
+    assert torch.equal(s["k"], before)
+
+
+def test_the_path_of_a_call_without_heads(K):
+    import ctypes
+    a = K.PagedAttentionArgs()
+    assert K.paged_path(ctypes.byref(a)) == 0

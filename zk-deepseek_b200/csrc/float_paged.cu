@@ -521,6 +521,7 @@ extern "C" {
 
 int zkfp_paged_path(const zkfp_paged_attention_args* a)
 {
+    if (!a || a->heads <= 0 || a->kv_heads <= 0 || a->heads < a->kv_heads || a->d <= 0 || a->dv <= 0 || a->batch <= 0) return 0;
     if (paged_stream_takes(*a)) return 2;
     return paged_tile_takes(*a) ? 1 : 0;
 }

@@ -12,7 +12,7 @@ inline int page_shift(int page)
     return -1;
 }
 
-// the sequence that row r belongs to, the same in every thread of the block, or -1 (all threads call it)
+// the sequence whose rows end behind row r, the same in every thread of the block, or -1 (all threads call it)
 __device__ __forceinline__ int sequence_of_row(const int* rows, int batch, long long r)
 {
     int b = 0;
@@ -20,7 +20,7 @@ __device__ __forceinline__ int sequence_of_row(const int* rows, int batch, long 
         const int i = base + (int)threadIdx.x;
         b += __syncthreads_count(i < batch && rows[i + 1] <= r);
     }
-    return b < batch && rows[b] >= 0 && rows[b] <= r ? b : -1;
+    return b < batch ? b : -1;
 }
 
 // ---- attention over pages: how the work is shared ----------------------------------------------------------------
@@ -69,14 +69,16 @@ inline void set_group(Paged& p, int group)
 }
 __device__ __forceinline__ int by_group(const Paged& p, int x) { return (int)(((uint64_t)(uint32_t)x * p.group_mul) >> p.group_shift); }
 
+// the first position that a row at position i (which may be negative) sees
+__device__ __forceinline__ int first_seen(const Paged& p, int i) { return p.a.window > 0 && i >= p.a.window ? i - p.a.window + 1 : 0; }
+
 // blocks of keys that tile t of a sequence with n rows and len positions visits: first .. first + count - 1, one at least
 __device__ __forceinline__ void tile_blocks(const Paged& p, int n, int len, int t, int& first, int& count)
 {
     const int last_row = min((t + 1) * p.tile, n * p.group) - 1;
     const int i0 = len - n + by_group(p, t * p.tile), i1 = len - n + by_group(p, last_row);
     if (i1 < 0) { first = 0; count = 1; return; }
-    const int lo = p.a.window > 0 ? max(i0 - p.a.window + 1, 0) : 0;
-    first = lo / p.block;
+    first = first_seen(p, i0) / p.block;
     count = i1 / p.block - first + 1;
 }
 
@@ -270,7 +272,7 @@ __device__ __noinline__ void attend_row(const Paged& p, int b, int kv, int token
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) o[k] = 0.f;
-    for (int j0 = p.a.window > 0 ? max(pos - p.a.window + 1, 0) : 0; j0 <= pos; j0 += 32) {
+    for (int j0 = first_seen(p, pos); j0 <= pos; j0 += 32) {
         const int j = j0 + lane;
         const long long page = j <= pos ? page_of(p, b, j) : -1;
         float s = 0.f;

@@ -114,7 +114,7 @@ struct Cursor {
         whole = begins && j_end == w.count;
         const int base = w.len - w.n, last_row = min((w.t + 1) * p.tile, w.n * p.group) - 1;
         hi = base + by_group(p, last_row);
-        lo = p.a.window > 0 ? base + by_group(p, w.t * p.tile) - p.a.window + 1 : 0;
+        lo = first_seen(p, base + by_group(p, w.t * p.tile));
         return true;
     }
     __device__ __forceinline__ bool next(const Paged& p, const Plan& plan, long long u1)
@@ -407,8 +407,7 @@ __device__ __forceinline__ Part part_of(const TileParams& t, const Walk& w, int 
         x.row0[g] = w.t * t.p.tile + g * t.rows;
         x.rows[g] = max(0, min(t.rows, all - x.row0[g]));
         const int i0 = x.base + by_group(t.p, x.row0[g]), i1 = x.rows[g] > 0 ? x.base + by_group(t.p, x.row0[g] + x.rows[g] - 1) : -1;
-        const int lo = t.p.a.window > 0 ? max(i0 - t.p.a.window + 1, 0) / kTile : 0;
-        x.first[g] = max(x.begin, lo);
+        x.first[g] = max(x.begin, first_seen(t.p, i0) / kTile);
         x.last[g] = i1 >= 0 ? min(x.end - 1, i1 / kTile) : x.first[g] - 1;
     }
     return x;
@@ -782,9 +781,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 tc_fence_after();
             }
             if (writes) {
-                s.most[3][g][half][row] = l;
-                pair_sync();
-                l += s.most[3][g][half ^ 1][row];
+                if (any) {                                // (without a tile nothing keeps the halves from the next part's place)
+                    s.most[3][g][half][row] = l;
+                    pair_sync();
+                    l += s.most[3][g][half ^ 1][row];
+                }
                 // 32 bytes of every row pass through shared memory, so that a store meets 16 rows and not 32: lanes 2 r and 2 r + 1 take the
                 // halves of rows r and r + 16
                 uint8_t* stage = s.stage[warp - 2];
@@ -919,11 +920,19 @@ bool key_maps(CUtensorMap* k, CUtensorMap* v, const zkfp_paged_attention_args& a
            pages_map(v, a.v, a.dv, a.kv_heads, a.page, a.pages, a.v_head, a.v_pos, a.v_page, rows);
 }
 
+// Tensor maps have no dimension that does not move on (a tensor expanded over heads, pages or tokens): the CUDA cores take those.
+bool moves(long long n, long long stride) { return n == 1 || stride > 0; }
+bool pages_move(const zkfp_paged_attention_args& a)
+{
+    return moves(a.kv_heads, a.k_head) && moves(a.kv_heads, a.v_head) && moves(a.page, a.k_pos) && moves(a.page, a.v_pos) && moves(a.pages, a.k_page) &&
+           moves(a.pages, a.v_page);
+}
+
 }  // namespace
 
 bool paged_stream_takes(const zkfp_paged_attention_args& a)
 {
-    return a.dtype == ZKFP_BF16 && a.d <= kStreamMost && a.dv <= kStreamMost && a.max_tokens * (a.heads / a.kv_heads) <= kStreamRows &&
+    return pages_move(a) && a.dtype == ZKFP_BF16 && a.d <= kStreamMost && a.dv <= kStreamMost && a.max_tokens * (a.heads / a.kv_heads) <= kStreamRows &&
            StreamShape(a).stages >= 2;
 }
 
@@ -946,7 +955,7 @@ static int launch_stream(const Paged& p, const CUtensorMap& k, const CUtensorMap
 
 bool paged_tile_takes(const zkfp_paged_attention_args& a)
 {
-    if (a.dtype != ZKFP_BF16 || a.d > kTileMost || a.dv > kTileMost) return false;
+    if (a.dtype != ZKFP_BF16 || a.d > kTileMost || a.dv > kTileMost || !pages_move(a) || !moves(a.heads, a.q_head) || !moves(a.tokens, a.q_tok)) return false;
     const TileShape s(a);
     return s.rows > 0 && s.k_slots >= s.seg;
 }

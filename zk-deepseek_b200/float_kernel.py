@@ -164,7 +164,7 @@ class FloatOpsError(RuntimeError):
 
 def _check(status, what):
     if status:
-        text = {1: "bad argument", 3: "CUDA error %d" % lib.zkfp_cuda_error(), 5: "a bounded wait ran out",
+        text = {1: "bad argument", 3: "CUDA error %d" % lib.zkfp_cuda_error(), 5: "a bounded wait ran out, or pages, rows or lengths do not fit",
                 6: "unsupported shape"}.get(status, "status %d" % status)
         raise FloatOpsError("%s: %s" % (what, text), status)
 
@@ -180,7 +180,7 @@ def _stream():
 
 
 def device_status(sync=False):
-    """raises if a finished kernel gave up a bounded wait"""
+    """raises if a finished kernel gave up a bounded wait, or met pages, rows or lengths that do not fit"""
     if sync:
         torch.cuda.current_stream().synchronize()
     _check(lib.zkfp_device_status(), "device status")
@@ -327,7 +327,8 @@ def gated_norm(args, *tensors):
 # Shared by the calls below: k_pages and v_pages [pages, page, kv_heads, size] (views with contiguous heads, the page size a
 # power of two from 8 to 1024), table [batch, columns] int32 (page numbers), rows [batch + 1] int32 (sequence b owns the
 # rows rows[b] .. rows[b + 1] - 1 of the batch), lengths [batch] int32 (positions that a sequence holds, its new rows
-# among them).  The device checks what they hold; `device_status` raises for what did not fit.
+# among them).  The device checks what they hold; `device_status` raises for what did not fit.  Pages may be shared by sequences
+# that read them; one that takes new rows is one sequence's.
 
 def _refuse(what, why):
     raise ValueError("%s: %s" % (what, why))
@@ -366,6 +367,12 @@ def _heads(what, name, t, dtype, dims, device, shape=None):
             _refuse(what, "%s has strides %s: heads must be contiguous, all else multiples of 8 elements" % (name, list(strides)))
         strides = [s if k > 1 else 0 for s, k in zip(strides, n)]
     return at, strides[:-1]
+
+
+def _apart(what, name, t, strides):
+    """refuses a result whose heads lie on one another (a tensor that was expanded)"""
+    if 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, t.shape)):
+        _refuse(what, "the heads of %s lie on one another" % name)
 
 
 def _pool(what, k, v, table, rows, lengths):
@@ -414,6 +421,7 @@ def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, windo
         _refuse(what, "%d query heads of %d over %d key heads of %d" % (heads, size, kv, d))
     shape = (tokens, heads, dv)
     op, os = _heads(what, "out", out, dt, 3, dev, shape)
+    _apart(what, "out", out, os)
     gp, gs = _heads(what, "gate", gate, dt, 3, dev, shape) if gate is not None else (None, (0, 0))
     if max_tokens is None:
         max_tokens = tokens
@@ -451,6 +459,9 @@ def write_pages(k, v, k_pages, v_pages, table, rows, lengths, q=None, q_out=None
         if not heads or q.shape != (tokens, heads, d):
             _refuse(what, "q is %s beside %d keys of %d" % (list(q.shape), tokens, d))
         oa, os = _heads(what, "q_out", q_out, dt, 3, dev, q.shape)
+        _apart(what, "q_out", q_out, os)
+    _apart(what, "k_pages", k_pages, ks)
+    _apart(what, "v_pages", v_pages, vs)
     ca, positions, pairs = None, 0, 0
     if cos_sin is not None:
         ca = _tensor(what, "cos_sin", cos_sin, torch.float32, 3, dev)
@@ -516,7 +527,7 @@ def sample(logits, random, out=None, temperature=1.0, top_k=0, top_p=1.0, min_p=
     A row keeps its top_k largest logits (0: all), of those the likeliest tokens until top_p of their weight lies in front
     (1: all), of those the tokens at least min_p as likely as the likeliest; of equal logits the lower indices.  Kept tokens lie in
     the order of their indices on [0, 1), as wide as they are likely, and random names the one.  temperature 0 takes the first of
-    the largest.  Each of the four is a number or a tensor [rows] (float32; top_k int32).  A row of nothing but -infinity and
+    the largest.  Each of the four is a number or a tensor [rows] (float32; top_k int32).  Up to 262144 tokens a row.  A row of nothing but -infinity and
     NaN gives -1."""
     what = "sample"
     dev = _device(what, "logits", logits)
