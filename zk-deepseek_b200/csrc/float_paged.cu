@@ -1,6 +1,7 @@
 // Attention of new tokens over pages: the kernels of CUDA cores (float32, and sizes that the tensor cores do not take) and
 // the one that merges what the CTAs of a cut item leave.  How the work is shared is in float_paged.cuh.
 #include "float_paged.cuh"
+#include "tcgen05.cuh"
 
 namespace zkds {
 
@@ -172,11 +173,22 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
 }
 
 // ---- CUDA cores, more rows -----------------------------------------------------------------------------------------
-// Tiles of 32 rows over blocks of 64 keys, which bound it by multiply-adds: sixteen lanes own four rows.  Scores: four rows times four keys (16
-// apart) a thread, two products an instruction along the head, so that eight 16-byte loads feed 64 products; rows of keys are shifted by one
-// 16-byte piece against each other, which meets no bank twice.  The rows' maxima and sums are these lanes' own, and so are the weights, which pass through shared memory to the second product: four rows times every
-// sixteenth pair of columns.  Only the keys and values need the whole block to meet.
-constexpr int kBlockRows = 32, kBlockKeys = 64, kBlockThreads = 128, kWeightPitch = kBlockKeys + 4;
+// Tiles of 32 rows over blocks of 48 keys.  What bounds it next to multiply-adds is what shared memory can hand to the registers, 128 bytes a
+// cycle, so a thread multiplies eight rows by six keys (eight apart), fourteen loads of 8 bytes for 96 products, and the head is dealt out in
+// pairs of elements to the four lanes that have the same forty-eight; they hand each other their sums, so that each is left with two rows.  Weights pass
+// through shared memory to the second product, eight rows times every sixteenth pair of columns over half of the keys a thread.  A warp owns its
+// eight rows; only keys and values need all of them to meet.  They have one place each: the next block's keys are on their way under the
+// softmax and the second product of this one, its values under the next scores.  Rows of keys are shifted by one 16-byte piece against each other,
+// which meets no bank twice.
+// Chunks of 100 tokens of three sequences, 16 heads of 72 over 4, the last 300 of up to 777 positions: 38 us, 6 of them to the first scores, 5 for the cut
+// items.  128 tokens of four sequences up to 1024, heads of 128: 96.  (Blocks of 64 keys 44 and 92, of 32 keys 40 and 109; four rows by two
+// keys a thread 42 and 116.)
+constexpr int kBlockRows = 32, kBlockKeys = 48, kKeysEach = kBlockKeys / 8, kBlockThreads = 128, kWarpRows = 8, kWeightPitch = kBlockKeys + 4;
+
+struct BlockShared {
+    uint64_t k_full, v_full, q_full;
+    int gave_up;
+};
 
 struct BlockShape {
     size_t smem;
@@ -185,23 +197,40 @@ struct BlockShape {
     {
         pairs = (a.dv + 31) / 32;
         pairs = pairs <= 2 ? 2 : pairs <= 4 ? pairs : 8;
-        smem = plan_bytes(a.batch) + sizeof(float) * ((size_t)kBlockKeys * (a.d + 4 + a.dv) + (size_t)kBlockRows * a.d + kBlockRows * kWeightPitch);
+        smem = plan_bytes(a.batch) + sizeof(float) * ((size_t)kBlockKeys * (a.d + 4 + a.dv) + (size_t)kBlockRows * a.d + kBlockRows * kWeightPitch) +
+               sizeof(BlockShared);
     }
 };
 
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <typename T, int PAIRS>
-__global__ void __launch_bounds__(kBlockThreads)
+__global__ void __launch_bounds__(kBlockThreads, PAIRS <= 3 ? 3 : 2)
 paged_block_kernel(const __grid_constant__ Paged p)
 {
     chain_enter();
     extern __shared__ __align__(16) uint8_t sm[];
     const zkfp_paged_attention_args& a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, d = a.d, dv = a.dv, vd = d / 8, pieces = vd + dv / 8, kpitch = d + 4, batch = (int)a.batch;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = a.d, dv = a.dv, kpitch = d + 4, batch = (int)a.batch;
     const Plan plan(sm, batch);
     float* K = (float*)(sm + (((size_t)(batch + 1) * 8 + (size_t)batch * 12 + 15) & ~(size_t)15));            // [key][kpitch]
-    float* Q = K + kBlockKeys * kpitch;                                                                        // [row][d]
-    float* V = Q + kBlockRows * d;                                                                             // [key][dv]; at the end [row][dv]
-    float* P = V + kBlockKeys * dv;                                                                            // [row][key]
+    float* V = K + kBlockKeys * kpitch;                                                                        // [key][dv]; at the end [row][dv]
+    float* Q = V + kBlockKeys * dv;                                                                            // [row][d]
+    float* P = Q + kBlockRows * d;                                                                             // [row][key]
+    BlockShared& sh = *(BlockShared*)(P + kBlockRows * kWeightPitch);
+    constexpr bool kBulk = sizeof(T) == 4;             // lines of keys and values go to shared memory as they are
+    if (tid == 0) {
+        mbar_init(smem_u32(&sh.k_full), kBlockKeys);
+        mbar_init(smem_u32(&sh.v_full), kBlockKeys);
+        mbar_init(smem_u32(&sh.q_full), kBlockRows);
+        sh.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     make_plan(p, plan);
     const long long units = plan.before[batch];
     const int ctas = sharing(p, units), cta = blockIdx.x;
@@ -209,7 +238,11 @@ paged_block_kernel(const __grid_constant__ Paged p)
     if (cta >= ctas || units == 0) return;
     const long long u1 = range_begin(units, cta + 1, ctas);
     long long u = range_begin(units, cta, ctas);
-    const int r4 = tid >> 4, at = tid & 15;            // which four rows, which of the sixteen
+    // scores: keys kg + 8 e, pairs sp, sp + 4, ... of the head; then rows r0 and r0 + 1 of the warp's.  Values: column pairs cl + 16 k, keys 8 i + 4 kh + 0 .. 3.
+    const int kg = lane & 7, sp = lane >> 3, r0 = 4 * (sp & 1) + 2 * (sp >> 1), cl = lane & 15, kh = lane >> 4;
+    const float scale = a.scale * 1.4426950408889634f;
+    uint32_t phase = 0, q_phase = 0;
+    bool ok = true;
     Walk w;
     for (w.locate(p, plan, u); u < u1; w.next(p, plan)) {
         const int taken = (int)min((long long)w.left(p), u1 - u), j_begin = w.begin(p), j_end = w.end(p, taken);
@@ -219,149 +252,213 @@ paged_block_kernel(const __grid_constant__ Paged p)
         const bool whole = j_begin == 0 && j_end == w.count;
         if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, units, ctas, w, end);
         const int slot = 2 * cta + (j_begin == 0 ? 1 : 0), row0 = w.t * kBlockRows, rows = min(kBlockRows, w.n * p.group - row0);
-        __syncthreads();
-        for (int i = tid; i < kBlockRows * vd; i += kBlockThreads) {
-            const int r = i / vd, c = (i - r * vd) * 8;
-            float x[8] = {};
-            if (r < rows) {
-                const int t = by_group(p, row0 + r), h = w.kv * p.group + row0 + r - t * p.group;
-                load8((const T*)a.q + (long long)(w.row0 + t) * a.q_tok + h * a.q_head + c, x);
+        const T *kb = (const T*)a.k + w.kv * a.k_head, *vb = (const T*)a.v + w.kv * a.v_head;
+        // A thread asks for one line of a block, keys or values; its page is looked up a block ahead, and looked at when it is needed.
+        auto find = [&](int j) {
+            const int k = (w.first + j) * kBlockKeys + tid;
+            return tid < kBlockKeys && j < j_end && k < w.len ? a.table[w.b * a.table_ld + (k >> p.shift)] : 0;
+        };
+        auto request = [&](int j, int page, bool values) {
+            const int k0 = (w.first + j) * kBlockKeys;
+            const T* from = values ? vb : kb;
+            const long long page_step = values ? a.v_page : a.k_page, line_step = values ? a.v_pos : a.k_pos;
+            float* to = values ? V : K;
+            const int size = values ? dv : d, pitch = values ? dv : kpitch;
+            if (kBulk) {
+                if (tid >= kBlockKeys) return;
+                const int k = k0 + tid;
+                const bool there = k < w.len && page >= 0 && page < a.pages;
+                if (k < w.len && !there) *(volatile int*)p.error_flag = 1;
+                const uint32_t bar = values ? smem_u32(&sh.v_full) : smem_u32(&sh.k_full);
+                if (there) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // zeros that the line held
+                    mbar_expect_tx(bar, size * 4);
+                    bulk_load(smem_u32(to + tid * pitch), from + page * page_step + (k & (a.page - 1)) * line_step, size * 4, bar);
+                } else {
+                    for (int c = 0; c < size; c += 4) *(float4*)(to + tid * pitch + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+                    mbar_arrive(bar);
+                }
+            } else {
+                for (int i = tid; i < kBlockKeys * (size / 4); i += kBlockThreads) {
+                    const int n = i / (size / 4), c = 4 * (i - n * (size / 4)), k = k0 + n;
+                    const long long at = k < w.len ? page_of(p, w.b, k) : -1;
+                    if (k < w.len && at < 0) *(volatile int*)p.error_flag = 1;
+                    float x[4] = {};
+                    if (at >= 0) load4(from + at * page_step + (k & (a.page - 1)) * line_step + c, x);
+                    store4(to + n * pitch + c, x);
+                }
             }
-            store8(Q + r * d + c, x);
+        };
+        const int here = kBulk ? find(j_begin) : 0;
+        int ahead = kBulk ? find(j_begin + 1) : 0;
+        if (kBulk) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();                               // the item in front is done with all of it
+        if (kBulk) {
+            // rows behind the last hold what they held, and nothing reads their results
+            if (tid >= kBlockThreads - kBlockRows) {
+                const int n = tid - (kBlockThreads - kBlockRows), t = by_group(p, row0 + n), h = w.kv * p.group + row0 + n - t * p.group;
+                mbar_expect_tx(smem_u32(&sh.q_full), n < rows ? d * 4 : 0);
+                if (n < rows) bulk_load(smem_u32(Q + n * d), (const T*)a.q + (long long)(w.row0 + t) * a.q_tok + h * a.q_head, d * 4, smem_u32(&sh.q_full));
+            }
+        } else {
+            for (int i = tid; i < rows * (d / 4); i += kBlockThreads) {
+                const int n = i / (d / 4), c = (i - n * (d / 4)) * 4, t = by_group(p, row0 + n), h = w.kv * p.group + row0 + n - t * p.group;
+                float x[4];
+                load4((const T*)a.q + (long long)(w.row0 + t) * a.q_tok + h * a.q_head + c, x);
+                store4(Q + n * d + c, x);
+            }
         }
-        int pos[4];
+        request(j_begin, here, false);
+        request(j_begin, here, true);
+        if (kBulk) {
+            if (ok) ok = mbar_wait_warp(smem_u32(&sh.q_full), q_phase, &sh.gave_up);
+            q_phase ^= 1u;
+        } else {
+            __syncthreads();
+        }
+        const int row = kWarpRows * warp;              // the first of this warp's
+        int pos[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pos[i] = 4 * r4 + i < rows ? w.len - w.n + by_group(p, row0 + 4 * r4 + i) : -1;
+        for (int i = 0; i < 2; ++i) pos[i] = row + r0 + i < rows ? w.len - w.n + by_group(p, row0 + row + r0 + i) : -1;
+        const int all_lo = first_seen(p, pos[1]);
         int column[PAIRS];                             // behind the last one: that one again, without a branch, and not stored
 #pragma unroll
-        for (int k = 0; k < PAIRS; ++k) column[k] = min(32 * k + 2 * at, dv - 2);
-        float m[4], l[4];
-        uint64_t acc[4][PAIRS];
+        for (int k = 0; k < PAIRS; ++k) column[k] = min(32 * k + 2 * cl, dv - 2);
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+        uint64_t acc[kWarpRows][PAIRS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.f;
+        for (int i = 0; i < kWarpRows; ++i)
 #pragma unroll
             for (int k = 0; k < PAIRS; ++k) acc[i][k] = 0;
-        }
         for (int j = j_begin; j < j_end; ++j) {
             const int k0 = (w.first + j) * kBlockKeys;
-            __syncthreads();                           // the block in front is done with keys and values
-            {
-                // a warp takes every fourth key with its value, a lane a piece; lane i knows the page of the i-th
-                const int warp = tid >> 5, of = k0 + warp + 4 * (lane & 15);
-                const long long held = of < w.len ? page_of(p, w.b, of) : -1;
-                if (of < w.len && held < 0) *(volatile int*)p.error_flag = 1;
-                __syncwarp();
-                for (int c = lane; c < (pieces + 31) / 32 * 32; c += 32) {
-                    const bool key = c < vd;
-                    const T* base = key ? (const T*)a.k + w.kv * a.k_head + 8 * c : (const T*)a.v + w.kv * a.v_head + 8 * (c - vd);
-                    const long long page_step = key ? a.k_page : a.v_page, line_step = key ? a.k_pos : a.v_pos;
-                    float* to = key ? K + 8 * c : V + 8 * (c - vd);
-                    const int to_step = key ? kpitch : dv;
-#pragma unroll 8
-                    for (int i = 0; i < kBlockKeys / 4; ++i) {
-                        const int r = warp + 4 * i;
-                        const long long page = __shfl_sync(0xffffffffu, held, i);
-                        float x[8] = {};
-                        if (page >= 0 && c < pieces) load8(base + page * page_step + ((k0 + r) & (a.page - 1)) * line_step, x);
-                        if (c < pieces) store8(to + r * to_step, x);
+            const bool works = row < rows;             // this warp
+            float s[kWarpRows][kKeysEach] = {};
+            if (kBulk && ok) ok = mbar_wait_warp(smem_u32(&sh.k_full), phase, &sh.gave_up);
+            if (works)
+#pragma unroll 1
+                for (int c = 2 * sp; c < d; c += 8) {
+                    float2 q[kWarpRows];
+#pragma unroll
+                    for (int i = 0; i < kWarpRows; ++i) q[i] = *(const float2*)(Q + (row + i) * d + c);
+#pragma unroll
+                    for (int e = 0; e < kKeysEach; ++e) {
+                        const float2 k = *(const float2*)(K + (kg + 8 * e) * kpitch + c);
+#pragma unroll
+                        for (int i = 0; i < kWarpRows; ++i) s[i][e] = fmaf(q[i].y, k.y, fmaf(q[i].x, k.x, s[i][e]));
                     }
                 }
-            }
-            __syncthreads();
-            if (4 * r4 >= rows) continue;              // sixteen lanes without rows
-            uint64_t s[4][4] = {};                     // even and odd elements apart
-#pragma unroll 2
-            for (int c = 0; c < d; c += 4) {
-                ulonglong2 q[4], k[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    q[i] = *(const ulonglong2*)(Q + (4 * r4 + i) * d + c);
-                    k[i] = *(const ulonglong2*)(K + (at + 16 * i) * kpitch + c);
-                }
+            __syncthreads();                           // the keys have been read
+            if (j + 1 < j_end) request(j + 1, ahead, false);
+            if (works) {
+                // two of the eight rows, the four lanes' sums of them
+                float h[4][kKeysEach], v[2][kKeysEach];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        fma2(s[i][e], q[i].x, k[e].x);
-                        fma2(s[i][e], q[i].y, k[e].y);
+                    for (int e = 0; e < kKeysEach; ++e) h[i][e] = (sp & 1 ? s[i + 4][e] : s[i][e]) + __shfl_xor_sync(0xffffffffu, sp & 1 ? s[i][e] : s[i + 4][e], 8);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < kKeysEach; ++e) v[i][e] = (sp & 2 ? h[i + 2][e] : h[i][e]) + __shfl_xor_sync(0xffffffffu, sp & 2 ? h[i][e] : h[i + 2][e], 16);
+                const bool edge = pos[1] < 0 || k0 + kBlockKeys - 1 > pos[0] || k0 < all_lo;
+                float top[2], f[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < kKeysEach; ++e) {
+                        const int key = k0 + kg + 8 * e;
+                        v[i][e] = edge && !(key <= pos[i] && (a.window <= 0 || pos[i] - key < a.window)) ? -INFINITY : v[i][e] * scale;
+                        top[i] = e ? fmaxf(top[i], v[i][e]) : v[i][e];
                     }
-            }
-            const unsigned half = 0xffffu << (lane & 16);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v[4], top = m[i];
+                for (int o = 1; o < 8; o <<= 1)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = k0 + at + 16 * e;
-                    const bool seen = key <= pos[i] && (a.window <= 0 || pos[i] - key < a.window);
-                    v[e] = seen ? (__uint_as_float((uint32_t)s[i][e]) + __uint_as_float((uint32_t)(s[i][e] >> 32))) * a.scale : -INFINITY;
-                    top = fmaxf(top, v[e]);
-                }
+                    for (int i = 0; i < 2; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
 #pragma unroll
-                for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(half, top, o));
-                const float f = m[i] == -INFINITY ? 0.f : expf(m[i] - top);
-                float sum = 0.f;
+                for (int i = 0; i < 2; ++i) {
+                    top[i] = fmaxf(top[i], m[i]);
+                    const float sub = top[i] == -INFINITY ? 0.f : top[i];
+                    f[i] = exp2_approx(m[i] - sub);
+                    m[i] = top[i];
+                    float sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = v[e] == -INFINITY ? 0.f : expf(v[e] - top);
-                    sum += v[e];
-                }
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(half, sum, o);
-                l[i] = l[i] * f + sum;
-                m[i] = top;
-                const uint64_t f2 = twice(f);
-                uint64_t none = 0;
-#pragma unroll
-                for (int k = 0; k < PAIRS; ++k) {
-                    uint64_t y = none;
-                    fma2(y, acc[i][k], f2);
-                    acc[i][k] = y;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) P[(4 * r4 + i) * kWeightPitch + at + 16 * e] = v[e];
-            }
-            __syncwarp(half);
-            for (int key = 0; key < kBlockKeys; key += 4) {
-                float x[4][4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) load4(P + (4 * r4 + i) * kWeightPitch + key, x[i]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int k = 0; k < PAIRS; ++k) {
-                        const uint64_t v = *(const uint64_t*)(V + (key + e) * dv + column[k]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) fma2(acc[i][k], v, twice(x[i][e]));
+                    for (int e = 0; e < kKeysEach; ++e) {
+                        v[i][e] = exp2_approx(v[i][e] - sub);
+                        sum += v[i][e];
+                        P[(row + r0 + i) * kWeightPitch + kg + 8 * e] = v[i][e];
                     }
+                    l[i] = l[i] * f[i] + sum;          // of this lane's keys
+                }
+                if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+                    for (int i = 0; i < kWarpRows; ++i) {
+                        const uint64_t f2 = twice(__shfl_sync(0xffffffffu, f[i & 1], (i >> 2 & 1) * 8 + (i >> 1 & 1) * 16));
+#pragma unroll
+                        for (int k = 0; k < PAIRS; ++k) {
+                            uint64_t y = 0;
+                            fma2(y, acc[i][k], f2);
+                            acc[i][k] = y;
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            if (kBulk && ok) ok = mbar_wait_warp(smem_u32(&sh.v_full), phase, &sh.gave_up);
+            phase ^= 1u;
+            if (works)
+#pragma unroll 1
+                for (int key = 4 * kh; key < kBlockKeys; key += 8) {
+                    float x[kWarpRows][4];
+#pragma unroll
+                    for (int i = 0; i < kWarpRows; ++i) load4(P + (row + i) * kWeightPitch + key, x[i]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int k = 0; k < PAIRS; ++k) {
+                            const uint64_t y = *(const uint64_t*)(V + (key + e) * dv + column[k]);
+#pragma unroll
+                            for (int i = 0; i < kWarpRows; ++i) fma2(acc[i][k], y, twice(x[i][e]));
+                        }
+                }
+            __syncthreads();                           // the values have been read
+            if (j + 1 < j_end) {
+                request(j + 1, ahead, true);
+                if (kBulk) ahead = find(j + 2);
             }
         }
-        __syncthreads();                               // the values make room for the sums
+        // both halves of the keys; the place of the values takes the rows of an item that is whole
         float* to = whole ? V : p.part + (long long)slot * p.tile * dv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (4 * r4 + i >= rows) break;
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int k = 0; k < PAIRS; ++k)
-                if (32 * k + 2 * at < dv) *(uint64_t*)(to + (4 * r4 + i) * dv + 32 * k + 2 * at) = acc[i][k];
-            if (at == 0) {
-                if (whole) P[4 * r4 + i] = l[i];
-                else *(float2*)(p.ml + ((long long)slot * p.tile + 4 * r4 + i) * 2) = make_float2(m[i], l[i]);
+            for (int o = 1; o < 8; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+            if (kg == 0 && row + r0 + i < rows) {
+                if (whole) P[row + r0 + i] = l[i];
+                else *(float2*)(p.ml + ((long long)slot * p.tile + row + r0 + i) * 2) = make_float2(m[i], l[i]);
             }
         }
+#pragma unroll
+        for (int i = 0; i < kWarpRows; ++i)
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) {
+                const uint64_t y = __shfl_xor_sync(0xffffffffu, acc[i][k], 16);
+                const float x0 = __uint_as_float((uint32_t)acc[i][k]) + __uint_as_float((uint32_t)y);
+                const float x1 = __uint_as_float((uint32_t)(acc[i][k] >> 32)) + __uint_as_float((uint32_t)(y >> 32));
+                if (kh == (i & 1) && row + i < rows && 32 * k + 2 * cl < dv) *(float2*)(to + (row + i) * dv + 32 * k + 2 * cl) = make_float2(x0, x1);
+            }
         if (whole) {
-            __syncthreads();
-            for (int r = tid >> 5; r < rows; r += kBlockThreads / 32) {
+            __syncwarp();
+            for (int i = row; i < min(row + kWarpRows, rows); ++i) {
                 float x[2][4];
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                    if (4 * lane + 128 * k < dv) load4(V + r * dv + 4 * lane + 128 * k, x[k]);
-                finish_row<T>(p, w, row0 + r, x, P[r]);
+                    if (4 * lane + 128 * k < dv) load4(V + i * dv + 4 * lane + 128 * k, x[k]);
+                finish_row<T>(p, w, row0 + i, x, P[i]);
             }
         }
     }
+    if (!ok) *(volatile int*)p.error_flag = 1;
 }
 
 // ---- cut items ---------------------------------------------------------------------------------------------------
@@ -458,7 +555,7 @@ int launch_block(Paged& p, size_t smem, cudaStream_t st)
     ZKDS_CUDA(cudaFuncSetAttribute(paged_block_kernel<T, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax));
     fp_launch(paged_block_kernel<T, PAIRS>, dim3((unsigned)p.grid), dim3(kBlockThreads), smem, st, p);
     const int rc = fp_launched();
-    return rc != ZKDS_OK ? rc : launch_combine<T>(p, 0, st);
+    return rc != ZKDS_OK ? rc : launch_combine<T>(p, 1, st);
 }
 
 template <typename T>
@@ -488,8 +585,10 @@ void choose(Paged& p)
     p.least = 2;
     if (p.a.max_tokens * p.group > kPlainRows) {
         p.tile = kBlockRows;
-        const int per_sm = (int)(220 * 1024 / BlockShape(p.a).smem);
-        p.grid = fp_sm_count() * (per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm);
+        p.block = kBlockKeys;
+        const BlockShape s(p.a);
+        const int per_sm = (int)(220 * 1024 / s.smem), most = s.pairs <= 3 ? 3 : 2;
+        p.grid = fp_sm_count() * (per_sm < 1 ? 1 : per_sm > most ? most : per_sm);
         return;
     }
     p.tile = kPlainRows;
