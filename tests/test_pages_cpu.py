@@ -373,3 +373,23 @@ def test_oracle_of_pages_is_the_window_of_a_whole_sequence():
     for h in range(2):
         p = fo.softmax_rows(q[:, h] @ k[:, 0].T * 0.5, fo.window_mask(20, 6))
         assert np.abs(got[:, h] - (p @ v[:, 0])[15:]).max() < 1e-12
+
+
+def test_calls_refuse_what_is_on_no_gpu(K):
+    """and hold on to nothing that they refused"""
+    import sys
+    t = {n: torch.zeros(*shape, dtype=dt) for n, shape, dt in (("q", (3, 4, 16), torch.float32), ("pages", (5, 16, 2, 16), torch.float32),
+         ("table", (1, 2), torch.int32), ("rows", (2,), torch.int32), ("lengths", (1,), torch.int32), ("logits", (2, 30), torch.float32), ("u", (2,), torch.float32))}
+    pages = (t["pages"], t["pages"], t["table"], t["rows"], t["lengths"])
+    kept = {n: sys.getrefcount(x) for n, x in t.items()}
+    for _ in range(3):
+        for call in (lambda: K.paged_attention(t["q"], *pages, t["q"], 0.1), lambda: K.write_pages(t["q"], t["q"], *pages), lambda: K.sample(t["logits"], t["u"]),
+                     lambda: K.copy_pages([t["pages"]], [0], [1]), lambda: K.sample([1.0], t["u"]), lambda: K.write_pages(t["q"], t["q"], *pages, layout="other"),
+                     lambda: K.copy_pages([t["pages"]], [0, 1], [2]), lambda: K.copy_pages([t["pages"]], [2 ** 40], [2]), lambda: K.copy_pages([3], [0], [1])):
+            with pytest.raises(ValueError):
+                call()
+        for call in (lambda: K.copy_pages([t["pages"]], [0.5], [1]), lambda: K.copy_pages(7, [0], [1])):
+            with pytest.raises(TypeError):
+                call()
+    assert K.copy_pages([], [], []) is None and K.copy_pages([t["pages"]], [], []) is None
+    assert {n: sys.getrefcount(x) for n, x in t.items()} == kept

@@ -730,3 +730,33 @@ def test_the_path_of_a_call_without_heads(K):
     import ctypes
     a = K.PagedAttentionArgs()
     assert K.paged_path(ctypes.byref(a)) == 0
+
+
+def test_calls_hold_on_to_nothing(K):
+    """no tensor, page list or result is held by a call that is over"""
+    import sys
+    s = pool("bfloat16", [2, 1], [30, 9], 16, 4, 2, 64, 64, fill=0.0)
+    out, k, cs, u = torch.empty_like(s["q"]), rnd((3, 2, 64), "bfloat16"), torch.zeros(40, 32, 2, device="cuda"), torch.zeros(3, device="cuda")
+    l, source = rnd((3, 50), "float32"), [0]
+    whole_k, whole_v = s["k"].contiguous(), s["v"].contiguous()
+    watched = [s["q"], s["k"], s["v"], s["table"], s["rows"], s["lengths"], out, k, cs, u, l, whole_k, whole_v, source, torch.bfloat16, torch.float32, torch.int32]
+
+    def calls():
+        pages = s["k"], s["v"], s["table"], s["rows"], s["lengths"]
+        K.paged_attention(s["q"], *pages, out, 0.1, gate=s["q"])
+        K.write_pages(k, k, *pages, q=s["q"], q_out=out, cos_sin=cs)
+        K.copy_pages([whole_k, whole_v], source, [1])
+        K.sample(l, u, temperature=u, top_k=3)
+        for bad in (lambda: K.paged_attention(s["q"], *pages, s["q"], 0.1), lambda: K.write_pages(k, k, *pages, q=s["q"]), lambda: K.copy_pages([whole_k, l], source, [90]),
+                    lambda: K.sample(l, u, out=u)):
+            with pytest.raises(ValueError):
+                bad()
+    calls()
+    before, held = [sys.getrefcount(x) for x in watched], torch.cuda.memory_allocated()
+    for _ in range(20):
+        calls()
+    after = [sys.getrefcount(x) for x in watched]
+    # dtypes are referred to by whatever else is alive
+    assert after[:-3] == before[:-3] and all(abs(a - b) < 20 for a, b in zip(after[-3:], before[-3:]))
+    assert torch.cuda.memory_allocated() == held
+    K.device_status(sync=True)

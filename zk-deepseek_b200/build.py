@@ -4,6 +4,7 @@
 
     libint64gemm.so   the int64 fixed-point kernels of the integer model
     libfloatops.so    the kernels of the floating-point decoder designs
+    float_calls.so    a Python module beside it: argument structures from tensors (built with either name)
 
 nvcc cross-compiles without a GPU.  The libraries link the CUDA runtime statically and resolve the driver entry
 points they need (tensor-map encoding) at run time, so they load on a machine without a GPU as well.  A library is
@@ -15,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -28,8 +30,9 @@ LIBRARIES = {
     "libfloatops.so": (["float_capi.cu", "float_ops.cu", "float_gemm.cu", "float_gemm_f32.cu", "float_gemm_tc.cu", "float_attention.cu",
                         "float_grouped.cu", "float_paged.cu", "float_paged_tc.cu", "float_pages.cu", "float_recurrent.cu", "float_sample.cu", "float_scan_tc.cu"],
                        ["common.cuh", "float_common.cuh", "float_paged.cuh", "tcgen05.cuh", "zkds_float.h"]),
+    "float_calls.so": (["float_calls.c"], ["zkds_float.h"]),
 }
-INT_LIBRARY, FLOAT_LIBRARY = "libint64gemm.so", "libfloatops.so"
+INT_LIBRARY, FLOAT_LIBRARY, FLOAT_CALLS = "libint64gemm.so", "libfloatops.so", "float_calls.so"
 OUT = os.path.join(HERE, INT_LIBRARY)
 
 
@@ -52,6 +55,14 @@ def _compile(library, verbose):
     out = os.path.join(HERE, library)
     tag = ".%d.partial" % os.getpid()
     flags = FLAGS + (["-Xptxas", "-v"] if verbose else [])
+    if LIBRARIES[library][0][0].endswith(".c"):         # a Python module: no kernels, and the interpreter's headers
+        res = subprocess.run([shutil.which("gcc") or "cc", "-O2", "-Wall", "-shared", "-fPIC", "-I", INCLUDE, "-I", sysconfig.get_paths()["include"],
+                              "-o", out + tag] + [os.path.join(CSRC, s) for s in LIBRARIES[library][0]], capture_output=True, text=True)
+        if res.returncode:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("the C compiler failed building " + library)
+        os.replace(out + tag, out)
+        return out
     objs, jobs, failed = [], [], False
     for src in LIBRARIES[library][0]:                  # the translation units compile side by side
         obj = os.path.join(HERE, src + tag + ".o")
@@ -83,6 +94,8 @@ def _compile(library, verbose):
 
 def build(force=False, verbose=False, library=INT_LIBRARY):
     out = os.path.join(HERE, library)
+    if library == FLOAT_LIBRARY:
+        build(force, verbose, FLOAT_CALLS)
     if not force and not _stale(library):
         return out
     with open(out + ".lock.partial", "w") as lock:     # one process compiles, the others wait for it

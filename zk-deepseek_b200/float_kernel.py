@@ -1,14 +1,19 @@
 """ctypes bindings of libfloatops.so, the kernels of the floating-point decoder designs (include/zkds_float.h).
 
 Tensors go in as torch CUDA tensors; every call is launched on torch's current stream and its status is checked.
-There is no CPU or PyTorch fallback: a missing library raises at import, a failed launch raises `FloatOpsError`.
+There is no CPU or PyTorch fallback: a missing library raises at import, a failed launch raises `FloatOpsError`.  The calls over pages
+and of sampling get their structures from the module float_calls, which looks the tensors over in C.
 """
 import ctypes
-import math
 import os
 import threading
 
 import torch
+
+try:
+    from . import float_calls as _calls
+except ImportError:  # pragma: no cover - this directory first on sys.path
+    import float_calls as _calls
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 F32, BF16 = 0, 1
@@ -142,12 +147,14 @@ _scan = _sig("zkfp_scan", [ctypes.POINTER(ScanArgs), _vp])
 _scan_scratch = _sig("zkfp_scan_scratch", [ctypes.POINTER(ScanArgs)], _ll)
 scan_path = _sig("zkfp_scan_path", [ctypes.POINTER(ScanArgs)])
 _gated_norm = _sig("zkfp_gated_norm", [ctypes.POINTER(GatedNormArgs), _vp])
-_paged = _sig("zkfp_paged_attention", [ctypes.POINTER(PagedAttentionArgs), _vp])
+_paged = _sig("zkfp_paged_attention", [_vp, _vp])              # structures of these calls come as bytes
 _paged_scratch = _sig("zkfp_paged_scratch", [ctypes.POINTER(PagedAttentionArgs)], _ll)
 paged_path = _sig("zkfp_paged_path", [ctypes.POINTER(PagedAttentionArgs)])
-_write_pages = _sig("zkfp_write_pages", [ctypes.POINTER(WritePagesArgs), _vp])
-_copy_pages = _sig("zkfp_copy_pages", [ctypes.POINTER(PageBuffer), _i, ctypes.POINTER(_i), ctypes.POINTER(_i), _ll, _vp])
-_sample = _sig("zkfp_sample", [ctypes.POINTER(SampleArgs), _vp])
+_write_pages = _sig("zkfp_write_pages", [_vp, _vp])
+_copy_pages = _sig("zkfp_copy_pages", [_vp, _i, _vp, _vp, _ll, _vp])
+_sample = _sig("zkfp_sample", [_vp, _vp])
+_calls.setup(torch.Tensor, torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.empty, torch.cuda.current_device,
+             ctypes.cast(_paged_scratch, _vp).value)
 _embed = _sig("zkfp_embed", [_vp, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _f, _i, _vp])
 _add_norm = _sig("zkfp_add_norm", [_vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _ll, _d, _i, _vp])
 _norm_rows = _sig("zkfp_norm_rows", [_vp, _ll, _vp, _vp, _vp, _ll, _ll, _ll, _d, _i, _vp])
@@ -330,80 +337,6 @@ def gated_norm(args, *tensors):
 # among them).  The device checks what they hold; `device_status` raises for what did not fit.  Pages may be shared by sequences
 # that read them; one that takes new rows is one sequence's.
 
-def _refuse(what, why):
-    raise ValueError("%s: %s" % (what, why))
-
-
-def _tensor(what, name, t, dtype, dims, device, shape=None):
-    """the tensor's address; refuses what is not on the device, or not of this type and shape"""
-    if not isinstance(t, torch.Tensor) or t.dim() != dims:
-        _refuse(what, "%s is no tensor of %d dimensions" % (name, dims))
-    if t.dtype is not dtype:
-        _refuse(what, "%s is %s, not %s" % (name, t.dtype, dtype))
-    if t.get_device() != device:
-        _refuse(what, "%s is on %s, the call goes to cuda:%d" % (name, t.device, device))
-    if shape is not None and t.shape != shape:
-        _refuse(what, "%s is %s, not %s" % (name, list(t.shape), list(shape)))
-    return t.data_ptr()
-
-
-def _device(what, name, t):
-    """the current device, which the call goes to"""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _refuse(what, "%s is no tensor on a GPU" % name)
-    return torch.cuda.current_device()
-
-
-def _heads(what, name, t, dtype, dims, device, shape=None):
-    """address and strides of a tensor of heads: the elements of a head adjacent, everything on 16-byte pieces"""
-    at = _tensor(what, name, t, dtype, dims, device, shape)
-    strides = t.stride()
-    bits = at >> 1                             # 16-byte pieces are eight elements of bfloat16 (and two of float32's)
-    for s in strides[:-1]:
-        bits |= s
-    if bits & 7 or strides[-1] != 1:
-        n = t.shape                            # a dimension of one element has no stride of its own
-        if at & 15 or (n[-1] > 1 and strides[-1] != 1) or any(s & 7 and k > 1 for s, k in zip(strides[:-1], n)):
-            _refuse(what, "%s has strides %s: heads must be contiguous, all else multiples of 8 elements" % (name, list(strides)))
-        strides = [s if k > 1 else 0 for s, k in zip(strides, n)]
-    return at, strides[:-1]
-
-
-def _apart(what, name, t, strides):
-    """refuses a result whose heads lie on one another (a tensor that was expanded)"""
-    if 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, t.shape)):
-        _refuse(what, "the heads of %s lie on one another" % name)
-
-
-def _pool(what, k, v, table, rows, lengths):
-    """device, addresses and strides of the pages, addresses of the rest, row pitch of the table, shapes"""
-    dev = _device(what, "k_pages", k)
-    dt = k.dtype
-    if dt is not torch.bfloat16 and dt is not torch.float32:
-        _refuse(what, "pages hold float32 or bfloat16")
-    kp, ks = _heads(what, "k_pages", k, dt, 4, dev)
-    vp, vs = _heads(what, "v_pages", v, dt, 4, dev)
-    shape, vshape = k.shape, v.shape
-    if shape[:3] != vshape[:3]:
-        _refuse(what, "pages of keys are %s, of values %s" % (list(shape), list(vshape)))
-    pages, page, kv, d = shape
-    if not 8 <= page <= 1024 or page & (page - 1):
-        _refuse(what, "pages of %d positions" % page)
-    dv = vshape[3]
-    if d & 7 or dv & 7 or not d or not dv:
-        _refuse(what, "head sizes %d and %d are no multiples of 8" % (d, dv))
-    tp = _tensor(what, "table", table, torch.int32, 2, dev)
-    batch, cols = table.shape
-    rp, lp = _tensor(what, "rows", rows, torch.int32, 1, dev, (batch + 1,)), _tensor(what, "lengths", lengths, torch.int32, 1, dev, (batch,))
-    if not batch or not cols or not pages or not kv:
-        _refuse(what, "no sequences, no columns, no pages or no heads")
-    ld, step = table.stride()
-    ld = ld if batch > 1 else cols
-    if (cols > 1 and step != 1) or ld < cols or rows.stride(0) != 1 or (batch > 1 and lengths.stride(0) != 1):
-        _refuse(what, "table, rows and lengths must be contiguous along their last dimension")
-    return dev, dt, kp, ks, vp, vs, tp, rp, lp, ld, batch, cols, pages, page, kv, d, dv
-
-
 def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, window=0, max_tokens=None, gate=None, out_scale=1.0):
     """Softmax attention of new tokens over pages.
 
@@ -413,26 +346,10 @@ def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, windo
     max_tokens: most rows that a sequence brings (default: all), which chooses the kernel.  gate [tokens, heads, dv]: out is
     multiplied by sigmoid(gate) * out_scale.  Head sizes up to 256, up to 1024 sequences; scale is not negative; out lies on no
     input."""
-    what = "paged_attention"
-    dev, dt, kp, ks, vp, vs, tp, rp, lp, ld, batch, cols, pages, page, kv, d, dv = _pool(what, k_pages, v_pages, table, rows, lengths)
-    qp, qs = _heads(what, "q", q, dt, 3, dev)
-    tokens, heads, size = q.shape
-    if not heads or heads % kv or d != size:
-        _refuse(what, "%d query heads of %d over %d key heads of %d" % (heads, size, kv, d))
-    shape = (tokens, heads, dv)
-    op, os = _heads(what, "out", out, dt, 3, dev, shape)
-    _apart(what, "out", out, os)
-    gp, gs = _heads(what, "gate", gate, dt, 3, dev, shape) if gate is not None else (None, (0, 0))
-    if max_tokens is None:
-        max_tokens = tokens
-    if window < 0 or max_tokens < 0 or not 0 <= scale < 3e38:
-        _refuse(what, "a negative window, bound or scale")
-    if tokens and op in (qp, gp, kp, vp):
-        _refuse(what, "out lies on an input")
-    if tokens:
-        a = PagedAttentionArgs(qp, kp, vp, op, gp, tp, rp, lp, None, *qs, *ks, *vs, *os, *gs, tokens, pages, cols, ld, batch, max_tokens, heads,
-                               kv, d, dv, page, min(window, 0x7fffffff), code(dt), scale, out_scale)
-        _with_scratch(_paged, _paged_scratch, a, what, q.device, (q, k_pages, v_pages, table, rows, lengths, out, gate))
+    made = _calls.paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, window, max_tokens, gate, out_scale)
+    if made is not None:
+        a, scratch = made
+        _call(_paged, (a,), "paged_attention", q, k_pages, v_pages, table, rows, lengths, out, gate, scratch)
     return out
 
 
@@ -443,82 +360,20 @@ def write_pages(k, v, k_pages, v_pages, table, rows, lengths, q=None, q_out=None
     cos_sin [positions, pairs, 2] float32 (`float_model.rotary_table`): the first 2 * pairs elements of a head turn, (2i, 2i + 1)
     with layout "pairs", (i, i + pairs) with "half"; None: nothing does.  A row at a position without angles keeps its own, a row
     without a place in the pages is not written."""
-    what = "write_pages"
-    dev, dt, kp, ks, vp, vs, tp, rp, lp, ld, batch, cols, pages, page, kv, d, dv = _pool(what, k_pages, v_pages, table, rows, lengths)
-    if layout not in ("pairs", "half") or (q is None) != (q_out is None):
-        _refuse(what, "layout is 'pairs' or 'half', q and q_out come together")
-    ka, kt = _heads(what, "k", k, dt, 3, dev)
-    tokens = k.shape[0]
-    if k.shape != (tokens, kv, d):
-        _refuse(what, "k is %s for pages of %d heads of %d" % (list(k.shape), kv, d))
-    va, vt = _heads(what, "v", v, dt, 3, dev, (tokens, kv, dv))
-    heads, qa, qs, oa, os = 0, None, (0, 0), None, (0, 0)
-    if q is not None:
-        qa, qs = _heads(what, "q", q, dt, 3, dev)
-        heads = q.shape[1]
-        if not heads or q.shape != (tokens, heads, d):
-            _refuse(what, "q is %s beside %d keys of %d" % (list(q.shape), tokens, d))
-        oa, os = _heads(what, "q_out", q_out, dt, 3, dev, q.shape)
-        _apart(what, "q_out", q_out, os)
-    _apart(what, "k_pages", k_pages, ks)
-    _apart(what, "v_pages", v_pages, vs)
-    ca, positions, pairs = None, 0, 0
-    if cos_sin is not None:
-        ca = _tensor(what, "cos_sin", cos_sin, torch.float32, 3, dev)
-        positions, pairs, two = cos_sin.shape
-        if two != 2 or not cos_sin.is_contiguous() or 2 * pairs > d:
-            _refuse(what, "cos_sin %s is no contiguous [positions, pairs, 2] for heads of %d" % (list(cos_sin.shape), d))
-    if tokens:
-        a = WritePagesArgs(qa, ka, va, oa, kp, vp, ca, tp, rp, lp, *qs, *kt, *vt, *os, *ks, *vs, tokens, pages, cols, ld, batch, positions, heads,
-                           kv, d, dv, page, pairs, int(layout == "half"), code(dt))
-        _call(_write_pages, (ctypes.byref(a),), what, q, k, v, q_out, k_pages, v_pages, cos_sin, table, rows, lengths)
+    if layout not in ("pairs", "half"):
+        raise ValueError("write_pages: layout is 'pairs' or 'half'")
+    a = _calls.write_pages(k, v, k_pages, v_pages, table, rows, lengths, q, q_out, cos_sin, layout == "half")
+    if a is not None:
+        _call(_write_pages, (a,), "write_pages", q, k, v, q_out, k_pages, v_pages, cos_sin, table, rows, lengths)
 
 
 def copy_pages(buffers, source, target, positions=None):
     """Copies page source[i] over page target[i] in every buffer [pages, page, ...], or the first `positions` positions of it.  All
     copies happen at once: no page may be a target twice, or both a source and a target.  source and target: page numbers on the
     host."""
-    what = "copy_pages"
-    n = len(source)
-    if n != len(target):
-        _refuse(what, "%d sources, %d targets" % (n, len(target)))
-    if not buffers or not n:
-        return
-    dev = _device(what, "a buffer", buffers[0])
-    layout, words = None, []                   # four words of a PageBuffer each; layers are mostly alike
-    for i, t in enumerate(buffers):
-        if not isinstance(t, torch.Tensor) or t.get_device() != dev:
-            _refuse(what, "buffer %d is no tensor on cuda:%d" % (i, dev))
-        this = t.shape, t.stride(), t.dtype
-        if this != layout:
-            layout, (stride, some, pages) = this, _page_layout(what, i, t, n, source, target, positions)
-        at = t.data_ptr()
-        if at & 15:
-            _refuse(what, "buffer %d does not lie on 16-byte pieces" % i)
-        words += (at, stride, some, pages)
-    list_ = ctypes.cast((_ll * len(words))(*words), ctypes.POINTER(PageBuffer))
-    _call(_copy_pages, (list_, len(buffers), (_i * n)(*source), (_i * n)(*target), n), what, *buffers)
-
-
-def _page_layout(what, i, t, n, source, target, positions):
-    """bytes between pages, bytes of one that are copied, pages"""
-    if t.dim() < 2:
-        _refuse(what, "buffer %d is no [pages, page, ...] tensor" % i)
-    pages, lines = t.shape[:2]
-    if positions is not None and not 0 <= positions <= lines:
-        _refuse(what, "%d positions of pages of %d" % (positions, lines))
-    if pages <= max(max(source), max(target)) or min(min(source), min(target)) < 0:
-        _refuse(what, "pages that buffer %d of %d does not have" % (i, pages))
-    if t.numel() == 0:
-        return 0, 0, pages
-    if not t[0].is_contiguous():
-        _refuse(what, "pages of buffer %d are not contiguous: strides %s" % (i, list(t.stride())))
-    whole = t[0].numel() * t.element_size()
-    some = whole if positions is None else whole // lines * positions
-    stride = t.stride(0) * t.element_size() if pages > 1 else whole
-    if (stride | some) & 15 or stride < whole:
-        _refuse(what, "pages of buffer %d, or the part of them that is copied, do not lie on 16-byte pieces of their own" % i)
-    return stride, some, pages
+    made = _calls.copy_pages(buffers, source, target, positions)
+    if made is not None:
+        _call(_copy_pages, made, "copy_pages", *buffers)
 
 
 def sample(logits, random, out=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -529,43 +384,7 @@ def sample(logits, random, out=None, temperature=1.0, top_k=0, top_p=1.0, min_p=
     the order of their indices on [0, 1), as wide as they are likely, and random names the one.  temperature 0 takes the first of
     the largest.  Each of the four is a number or a tensor [rows] (float32; top_k int32).  Up to 262144 tokens a row.  A row of nothing but -infinity and
     NaN gives -1."""
-    what = "sample"
-    dev = _device(what, "logits", logits)
-    dt = logits.dtype
-    if dt is not torch.bfloat16 and dt is not torch.float32:
-        _refuse(what, "logits are float32 or bfloat16")
-    at = _tensor(what, "logits", logits, dt, 2, dev)
-    (rows, vocab), (ld, step) = logits.shape, logits.stride()
-    if rows == 1:
-        ld = vocab
-    if not vocab or (vocab > 1 and step != 1) or ld < vocab:
-        _refuse(what, "logits %s with strides %s" % (list(logits.shape), list(logits.stride())))
-    shape = (rows,)
-
-    def per_row(name, t, dtype):
-        at = _tensor(what, name, t, dtype, 1, dev, shape)
-        if rows > 1 and t.stride(0) != 1:
-            _refuse(what, "%s is not contiguous" % name)
-        return at
-
-    if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    f32, at_u, at_out = torch.float32, per_row("random", random, torch.float32), per_row("out", out, torch.int64)
-    pointers, values, held = [], [], [logits, random, out]
-    for name, x, dtype in (("temperature", temperature, f32), ("top_k", top_k, torch.int32), ("top_p", top_p, f32), ("min_p", min_p, f32)):
-        if isinstance(x, torch.Tensor):
-            pointers.append(per_row(name, x, dtype))
-            values.append(0)
-            held.append(x)
-        else:
-            if not x >= 0:
-                _refuse(what, "%s is %r" % (name, x))
-            pointers.append(None)
-            values.append(x)
-    temperature, top_k, top_p, min_p = values
-    if top_k != int(top_k):
-        _refuse(what, "top_k is %r" % (top_k,))
-    if rows:
-        a = SampleArgs(at, at_u, at_out, *pointers, ld, rows, vocab, code(dt), temperature, min(int(top_k), 0x7fffffff), top_p, min_p)
-        _call(_sample, (ctypes.byref(a),), what, *held)
+    a, out = _calls.sample(logits, random, out, temperature, top_k, top_p, min_p)
+    if a is not None:
+        _call(_sample, (a,), "sample", logits, random, out, temperature, top_k, top_p, min_p)
     return out
