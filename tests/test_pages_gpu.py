@@ -760,3 +760,12 @@ def test_calls_hold_on_to_nothing(K):
     assert after[:-3] == before[:-3] and all(abs(a - b) < 20 for a, b in zip(after[-3:], before[-3:]))
     assert torch.cuda.memory_allocated() == held
     K.device_status(sync=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", list(range(1, 10)))
+def test_every_number_of_few_rows(K, dtype, new):
+    """three to 27 rows a key head, beside sequences with fewer, over stretches of keys that end in every way"""
+    s = pool(dtype, [new, 1, new, max(new - 1, 0)], [new, 16 * new + 1, 400 + new, 129], 8, 6, 2, 40, 136 if new == 3 else 24)
+    check(K, s, dtype, window=0 if new % 2 else 37, max_tokens=new)
+    check(K, s, dtype, scale=1.0, window=100, max_tokens=1)

@@ -1,4 +1,4 @@
-// Attention of new tokens over pages: the kernels of CUDA cores (float32, and sizes that the tensor cores do not take) and
+// Attention of new tokens over pages: the kernels of CUDA cores (float32, and what the tensor cores do not take) and
 // the one that merges what the CTAs of a cut item leave.  How the work is shared is in float_paged.cuh.
 #include "float_paged.cuh"
 #include "tcgen05.cuh"
@@ -7,9 +7,16 @@ namespace zkds {
 
 namespace {
 
-// ---- CUDA cores, few rows ----------------------------------------------------------------------------------------
-// Tiles of 16 rows over blocks of 64 keys, all in shared memory, sums of a row in registers: a thread holds eight columns of
-// up to four rows.
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- CUDA cores, few rows of bfloat16 ------------------------------------------------------------------------------
+// For what the tensor cores do not take (heads beyond 128, tensors that were expanded): tiles of 16 rows over blocks of 64 keys, all in shared
+// memory, sums of a row in registers: a thread holds eight columns of up to four rows.
 constexpr int kPlainRows = 16, kPlainKeys = 64, kPlainThreads = 128, kPlainMost = 256;
 
 template <typename T>
@@ -172,6 +179,264 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
     }
 }
 
+// ---- CUDA cores, few rows of float32 -------------------------------------------------------------------------------
+// Up to R rows (4 or 8) per key head, so that the bytes of keys and values are the bound.  A warp works by itself, on every fourth stretch of 16
+// keys, which it asks for line by line; as in the kernel below, the four lanes that share rows and keys deal the head out among themselves in pairs of
+// elements and hand each other their sums, weights pass through shared memory, the next stretch's keys are on their way under the softmax and the second
+// product and its values under the next scores.  The warps' sums meet at the end of the item.
+// One new token of 1, 16, 64 sequences of up to 1024 positions, 16 heads of 128 over 4: 12, 14, 20 us (tiles of eight rows instead of four 14, 17, 25;
+// the kernel above, all warps on one block, 27, 29, 56).  Eight sequences with 6 and 8 tokens each, 24 and 32 rows: 19 and 24 us, the kernel below 22
+// and 24, so that 24 rows is where that one begins.
+constexpr int kFewRows = 24, kFewWarps = 4, kFewKeys = 16, kFewBlock = kFewWarps * kFewKeys, kFewThreads = kFewWarps * 32, kFewPitch = kFewKeys + 4;
+
+template <int R>
+struct FewShared {
+    uint64_t full[kFewWarps][2];                       // keys, values
+    uint64_t q_full;
+    float m[kFewWarps][R], l[kFewWarps][R];
+    __align__(16) float weights[kFewWarps][R][kFewPitch];
+    int gave_up;
+};
+
+template <int R>
+size_t few_bytes(const zkfp_paged_attention_args& a)
+{
+    return plan_bytes(a.batch) + sizeof(float) * ((size_t)kFewBlock * (a.d + 4 + a.dv) + (size_t)R * a.d) + sizeof(FewShared<R>);
+}
+
+template <int R, int PAIRS>
+__global__ void __launch_bounds__(kFewThreads, PAIRS <= 4 ? 3 : 2)
+paged_few_kernel(const __grid_constant__ Paged p)
+{
+    chain_enter();
+    extern __shared__ __align__(16) uint8_t sm[];
+    const zkfp_paged_attention_args& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = a.d, dv = a.dv, kpitch = d + 4, batch = (int)a.batch;
+    constexpr int kEach = R / 4;                       // rows of a lane behind the scores
+    const Plan plan(sm, batch);
+    float* ring = (float*)(sm + (((size_t)(batch + 1) * 8 + (size_t)batch * 12 + 15) & ~(size_t)15));
+    float* K = ring + warp * kFewKeys * (kpitch + dv);                                                         // [key][kpitch]; at the end [row][dv]
+    float* V = K + kFewKeys * kpitch;                                                                          // [key][dv]
+    float* Q = ring + kFewBlock * (kpitch + dv);                                                               // [row][d]
+    FewShared<R>& sh = *(FewShared<R>*)(Q + R * d);
+    if (tid == 0) {
+        for (int i = 0; i < kFewWarps; ++i) {
+            mbar_init(smem_u32(&sh.full[i][0]), kFewKeys);
+            mbar_init(smem_u32(&sh.full[i][1]), kFewKeys);
+        }
+        mbar_init(smem_u32(&sh.q_full), R);
+        sh.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    make_plan(p, plan);
+    const long long units = plan.before[batch];
+    const int ctas = sharing(p, units), cta = blockIdx.x;
+    if (tid == 0) no_cut(p, cta);
+    if (cta >= ctas || units == 0) return;
+    const long long u1 = range_begin(units, cta + 1, ctas);
+    long long u = range_begin(units, cta, ctas);
+    // scores: keys kg + 8 e, pairs sp, sp + 4, ... of the head; then rows r0 and on.  Values: column pairs cl + 16 k, keys 8 i + 4 kh + 0 .. 3.
+    const int kg = lane & 7, sp = lane >> 3, r0 = R / 2 * (sp & 1) + kEach * (sp >> 1), cl = lane & 15, kh = lane >> 4;
+    const int line_of = lane & (kFewKeys - 1);
+    const bool values = lane >= kFewKeys;              // which lines this lane asks for
+    const float scale = a.scale * 1.4426950408889634f;
+    int column[PAIRS];                                 // behind the last one: that one again, without a branch, and not stored
+#pragma unroll
+    for (int k = 0; k < PAIRS; ++k) column[k] = min(32 * k + 2 * cl, dv - 2);
+    uint32_t phase = 0, q_phase = 0;
+    bool ok = true;
+    Walk w;
+    for (w.locate(p, plan, u); u < u1; w.next(p, plan)) {
+        const int taken = (int)min((long long)w.left(p), u1 - u), j_begin = w.begin(p), j_end = w.end(p, taken);
+        const long long end = u + w.left(p);
+        u += taken;
+        if (j_begin == j_end) continue;
+        const bool whole = j_begin == 0 && j_end == w.count;
+        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, units, ctas, w, end);
+        const int slot = 2 * cta + (j_begin == 0 ? 1 : 0), row0 = w.t * R, rows = min(R, w.n * p.group - row0);
+        const float* from = values ? (const float*)a.v + w.kv * a.v_head : (const float*)a.k + w.kv * a.k_head;
+        const long long page_step = values ? a.v_page : a.k_page, line_step = values ? a.v_pos : a.k_pos;
+        float* to = values ? V + line_of * dv : K + line_of * kpitch;
+        const int size = values ? dv : d;
+        const uint32_t bar = smem_u32(&sh.full[warp][values]);
+        // the position of this lane's line of block j, its page, looked up a stretch ahead and looked at when it is needed, and the request
+        auto key_of = [&](int j) { return (w.first + j) * kFewBlock + warp * kFewKeys + line_of; };
+        auto find = [&](int j) { return j < j_end && key_of(j) < w.len ? a.table[w.b * a.table_ld + (key_of(j) >> p.shift)] : 0; };
+        auto request = [&](int j, int page) {
+            const int k = key_of(j);
+            const bool there = k < w.len && page >= 0 && page < a.pages;
+            if (k < w.len && !there) *(volatile int*)p.error_flag = 1;
+            if (there) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // zeros that the line held
+                mbar_expect_tx(bar, size * 4);
+                bulk_load(smem_u32(to), from + page * page_step + (k & (a.page - 1)) * line_step, size * 4, bar);
+            } else {
+                for (int c = 0; c < size; c += 4) *(float4*)(to + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+                mbar_arrive(bar);
+            }
+        };
+        request(j_begin, find(j_begin));
+        int ahead = find(j_begin + 1);
+        if (tid < R) {
+            // rows behind the last hold what they held, and nothing reads their results
+            const int t = by_group(p, row0 + tid), h = w.kv * p.group + row0 + tid - t * p.group;
+            mbar_expect_tx(smem_u32(&sh.q_full), tid < rows ? d * 4 : 0);
+            if (tid < rows) bulk_load(smem_u32(Q + tid * d), (const float*)a.q + (long long)(w.row0 + t) * a.q_tok + h * a.q_head, d * 4, smem_u32(&sh.q_full));
+        }
+        __syncwarp();
+        int pos[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) pos[i] = r0 + i < rows ? w.len - w.n + by_group(p, row0 + r0 + i) : -1;
+        const int all_lo = first_seen(p, pos[kEach - 1]);
+        float m[kEach], l[kEach];
+        uint64_t acc[R][PAIRS];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) acc[i][k] = 0;
+        if (ok) ok = mbar_wait_warp(smem_u32(&sh.q_full), q_phase, &sh.gave_up);
+        q_phase ^= 1u;
+        for (int j = j_begin; j < j_end; ++j) {
+            const int k0 = (w.first + j) * kFewBlock + warp * kFewKeys;
+            float s[R][2] = {};
+            if (ok) ok = mbar_wait_warp(smem_u32(&sh.full[warp][0]), phase, &sh.gave_up);
+#pragma unroll 2
+            for (int c = 2 * sp; c < d; c += 8) {
+                const float2 ka = *(const float2*)(K + kg * kpitch + c), kb = *(const float2*)(K + (kg + 8) * kpitch + c);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const float2 q = *(const float2*)(Q + i * d + c);
+                    s[i][0] = fmaf(q.y, ka.y, fmaf(q.x, ka.x, s[i][0]));
+                    s[i][1] = fmaf(q.y, kb.y, fmaf(q.x, kb.x, s[i][1]));
+                }
+            }
+            __syncwarp();                              // the keys have been read
+            if (j + 1 < j_end && !values) request(j + 1, ahead);
+            __syncwarp();
+            float h[R / 2][2], v[kEach][2], top[kEach], f[kEach];
+#pragma unroll
+            for (int i = 0; i < R / 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) h[i][e] = (sp & 1 ? s[i + R / 2][e] : s[i][e]) + __shfl_xor_sync(0xffffffffu, sp & 1 ? s[i][e] : s[i + R / 2][e], 8);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) v[i][e] = (sp & 2 ? h[i + kEach][e] : h[i][e]) + __shfl_xor_sync(0xffffffffu, sp & 2 ? h[i][e] : h[i + kEach][e], 16);
+            const bool edge = pos[kEach - 1] < 0 || k0 + kFewKeys - 1 > pos[0] || k0 < all_lo;
+            float changed = 0.f;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = k0 + kg + 8 * e;
+                    v[i][e] = edge && !(key <= pos[i] && (a.window <= 0 || pos[i] - key < a.window)) ? -INFINITY : v[i][e] * scale;
+                }
+                top[i] = fmaxf(v[i][0], v[i][1]);
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+                top[i] = fmaxf(top[i], m[i]);
+                const float sub = top[i] == -INFINITY ? 0.f : top[i];
+                f[i] = exp2_approx(m[i] - sub);
+                changed += f[i] != 1.f;
+                m[i] = top[i];
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    v[i][e] = exp2_approx(v[i][e] - sub);
+                    sum += v[i][e];
+                    sh.weights[warp][r0 + i][kg + 8 * e] = v[i][e];
+                }
+                l[i] = l[i] * f[i] + sum;              // of this lane's keys
+            }
+            if (__any_sync(0xffffffffu, changed != 0.f)) {
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const uint64_t f2 = twice(__shfl_sync(0xffffffffu, f[i % kEach], 8 * (i / (R / 2)) + 16 * (i % (R / 2) / kEach)));
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) {
+                        uint64_t y = 0;
+                        fma2(y, acc[i][k], f2);
+                        acc[i][k] = y;
+                    }
+                }
+            }
+            __syncwarp();
+            if (ok) ok = mbar_wait_warp(smem_u32(&sh.full[warp][1]), phase, &sh.gave_up);
+            phase ^= 1u;
+#pragma unroll
+            for (int key = 0; key < kFewKeys; key += 8) {
+                float x[R][4];
+#pragma unroll
+                for (int i = 0; i < R; ++i) load4(&sh.weights[warp][i][key + 4 * kh], x[i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) {
+                        const uint64_t y = *(const uint64_t*)(V + (key + 4 * kh + e) * dv + column[k]);
+#pragma unroll
+                        for (int i = 0; i < R; ++i) fma2(acc[i][k], y, twice(x[i][e]));
+                    }
+            }
+            __syncwarp();                              // the values have been read, and the weights
+            if (j + 1 < j_end && values) request(j + 1, ahead);
+            __syncwarp();
+            ahead = find(j + 2);
+        }
+        // the warps' sums, each in the place of its keys
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+            if (kg == 0) {
+                sh.m[warp][r0 + i] = m[i];
+                sh.l[warp][r0 + i] = l[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) {
+                const uint64_t y = __shfl_xor_sync(0xffffffffu, acc[i][k], 16);
+                const float x0 = __uint_as_float((uint32_t)acc[i][k]) + __uint_as_float((uint32_t)y);
+                const float x1 = __uint_as_float((uint32_t)(acc[i][k] >> 32)) + __uint_as_float((uint32_t)(y >> 32));
+                if (kh == (i & 1) && 32 * k + 2 * cl < dv) *(float2*)(K + i * dv + 32 * k + 2 * cl) = make_float2(x0, x1);
+            }
+        __syncthreads();
+        for (int i = warp; i < rows; i += kFewWarps) {
+            float top = -INFINITY, sum = 0.f, x[2][4] = {};
+#pragma unroll
+            for (int o = 0; o < kFewWarps; ++o) top = fmaxf(top, sh.m[o][i]);
+#pragma unroll
+            for (int o = 0; o < kFewWarps; ++o) {
+                if (sh.m[o][i] == -INFINITY) continue;
+                const float g = exp2_approx(sh.m[o][i] - top);
+                sum = fmaf(g, sh.l[o][i], sum);
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (4 * lane + 128 * k < dv) {
+                        float y[4];
+                        load4(ring + o * kFewKeys * (kpitch + dv) + i * dv + 4 * lane + 128 * k, y);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) x[k][q] = fmaf(g, y[q], x[k][q]);
+                    }
+            }
+            if (whole) {
+                finish_row<float>(p, w, row0 + i, x, sum);
+                continue;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (4 * lane + 128 * k < dv) store4(p.part + ((long long)slot * R + i) * dv + 4 * lane + 128 * k, x[k]);
+            if (lane == 0) *(float2*)(p.ml + ((long long)slot * R + i) * 2) = make_float2(top, sum);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");                   // the places are loaded into again
+        __syncthreads();
+    }
+    if (!ok) *(volatile int*)p.error_flag = 1;
+}
+
 // ---- CUDA cores, more rows -----------------------------------------------------------------------------------------
 // Tiles of 32 rows over blocks of 48 keys.  What bounds it next to multiply-adds is what shared memory can hand to the registers, 128 bytes a
 // cycle, so a thread multiplies eight rows by six keys (eight apart), fourteen loads of 8 bytes for 96 products, and the head is dealt out in
@@ -201,13 +466,6 @@ struct BlockShape {
                sizeof(BlockShared);
     }
 };
-
-__device__ __forceinline__ float exp2_approx(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 template <typename T, int PAIRS>
 __global__ void __launch_bounds__(kBlockThreads, PAIRS <= 3 ? 3 : 2)
@@ -521,12 +779,11 @@ paged_combine_kernel(const __grid_constant__ Paged p, int base2)
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
-template <typename T>
-int plain_grid(const zkfp_paged_attention_args& a)
+// CTAs that fit the GPU at once, `most` per SM
+int grid_of(size_t smem, int most)
 {
-    const size_t smem = PlainShape<T>(a).smem;
     const int per_sm = (int)(220 * 1024 / smem);
-    return fp_sm_count() * (per_sm < 1 ? 1 : per_sm > 6 ? 6 : per_sm);
+    return fp_sm_count() * (per_sm < 1 ? 1 : per_sm > most ? most : per_sm);
 }
 
 template <typename T>
@@ -538,15 +795,31 @@ int launch_combine(const Paged& p, int base2, cudaStream_t st)
     return fp_launched();
 }
 
-template <typename T>
 int launch_plain(Paged& p, cudaStream_t st)
 {
-    const PlainShape<T> s(p.a);
+    const PlainShape<bf16> s(p.a);
     if (s.smem > (size_t)kSharedMax) return ZKDS_ERR_UNSUPPORTED;
-    ZKDS_CUDA(cudaFuncSetAttribute(paged_plain_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax));
-    fp_launch(paged_plain_kernel<T>, dim3((unsigned)p.grid), dim3(kPlainThreads), s.smem, st, p, s.kpitch);
+    ZKDS_CUDA(cudaFuncSetAttribute(paged_plain_kernel<bf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax));
+    fp_launch(paged_plain_kernel<bf16>, dim3((unsigned)p.grid), dim3(kPlainThreads), s.smem, st, p, s.kpitch);
     const int rc = fp_launched();
-    return rc != ZKDS_OK ? rc : launch_combine<T>(p, 0, st);
+    return rc != ZKDS_OK ? rc : launch_combine<bf16>(p, 0, st);
+}
+
+template <int R, int PAIRS>
+int launch_few(Paged& p, cudaStream_t st)
+{
+    const size_t smem = few_bytes<R>(p.a);
+    if (smem > (size_t)kSharedMax) return ZKDS_ERR_UNSUPPORTED;
+    ZKDS_CUDA(cudaFuncSetAttribute(paged_few_kernel<R, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax));
+    fp_launch(paged_few_kernel<R, PAIRS>, dim3((unsigned)p.grid), dim3(kFewThreads), smem, st, p);
+    const int rc = fp_launched();
+    return rc != ZKDS_OK ? rc : launch_combine<float>(p, 1, st);
+}
+
+template <int R>
+int launch_few(Paged& p, cudaStream_t st)
+{
+    return p.a.dv <= 64 ? launch_few<R, 2>(p, st) : p.a.dv <= 128 ? launch_few<R, 4>(p, st) : launch_few<R, 8>(p, st);
 }
 
 template <typename T, int PAIRS>
@@ -561,7 +834,9 @@ int launch_block(Paged& p, size_t smem, cudaStream_t st)
 template <typename T>
 int launch_cores(Paged& p, cudaStream_t st)
 {
-    if (p.tile == kPlainRows) return launch_plain<T>(p, st);
+    if (p.tile == 4) return launch_few<4>(p, st);
+    if (p.tile == 8) return launch_few<8>(p, st);
+    if (p.tile == kPlainRows) return launch_plain(p, st);
     const BlockShape s(p.a);
     if (s.smem > (size_t)kSharedMax) return ZKDS_ERR_UNSUPPORTED;
     switch (s.pairs) {
@@ -580,19 +855,24 @@ void choose(Paged& p)
     const int path = zkfp_paged_path(&p.a);
     if (path == 2) return paged_stream_shape(p);
     if (path == 1) return paged_tile_shape(p);
-    p.block = kPlainKeys;
+    const long long rows = p.a.max_tokens * p.group;
     p.over = 1;
     p.least = 2;
-    if (p.a.max_tokens * p.group > kPlainRows) {
+    if (p.a.dtype != ZKFP_BF16 && rows <= kFewRows) {
+        p.tile = rows <= 4 ? 4 : 8;
+        p.block = kFewBlock;
+        p.over = 2;
+        p.grid = grid_of(rows <= 4 ? few_bytes<4>(p.a) : few_bytes<8>(p.a), p.a.dv <= 128 ? 3 : 2);
+    } else if (rows <= kPlainRows) {
+        p.tile = kPlainRows;
+        p.block = kPlainKeys;
+        p.grid = grid_of(PlainShape<bf16>(p.a).smem, 6);
+    } else {
+        const BlockShape s(p.a);
         p.tile = kBlockRows;
         p.block = kBlockKeys;
-        const BlockShape s(p.a);
-        const int per_sm = (int)(220 * 1024 / s.smem), most = s.pairs <= 3 ? 3 : 2;
-        p.grid = fp_sm_count() * (per_sm < 1 ? 1 : per_sm > most ? most : per_sm);
-        return;
+        p.grid = grid_of(s.smem, s.pairs <= 3 ? 3 : 2);
     }
-    p.tile = kPlainRows;
-    p.grid = p.a.dtype == ZKFP_BF16 ? plain_grid<bf16>(p.a) : plain_grid<float>(p.a);
 }
 
 bool paged_ok(const zkfp_paged_attention_args* a)
