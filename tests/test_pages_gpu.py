@@ -769,3 +769,16 @@ def test_every_number_of_few_rows(K, dtype, new):
     s = pool(dtype, [new, 1, new, max(new - 1, 0)], [new, 16 * new + 1, 400 + new, 129], 8, 6, 2, 40, 136 if new == 3 else 24)
     check(K, s, dtype, window=0 if new % 2 else 37, max_tokens=new)
     check(K, s, dtype, scale=1.0, window=100, max_tokens=1)
+
+
+def test_tensors_that_require_gradients_are_read_all_the_same(K):
+    s = pool("bfloat16", [2, 1], [30, 9], 16, 4, 2, 64, 64, fill=0.0)
+    want = attend_quietly(K, s, "bfloat16")
+    s["q"] = torch.nn.Parameter(s["q"])
+    with torch.no_grad():
+        assert torch.equal(attend_quietly(K, s, "bfloat16"), want)
+    l, u = rnd((3, 50), "float32"), torch.full((3,), 0.4, device="cuda")
+    assert torch.equal(K.sample(torch.nn.Parameter(l), u), K.sample(l, u))
+    half = torch.arange(96, device="cuda", dtype=torch.float16).reshape(3, 2, 16)                # a type that no other call takes
+    K.copy_pages([half], [0], [2])
+    assert torch.equal(half[2], half[0])

@@ -12,6 +12,7 @@ compiled when it is missing or older than one of its sources; callers on a fresh
 load.
 """
 import fcntl
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -55,8 +56,9 @@ def _compile(library, verbose):
     out = os.path.join(HERE, library)
     tag = ".%d.partial" % os.getpid()
     flags = FLAGS + (["-Xptxas", "-v"] if verbose else [])
-    if LIBRARIES[library][0][0].endswith(".c"):         # a Python module: no kernels, and the interpreter's headers
+    if LIBRARIES[library][0][0].endswith(".c"):         # a Python module: no kernels; the interpreter's headers, and DLPack's
         res = subprocess.run([shutil.which("gcc") or "cc", "-O2", "-Wall", "-shared", "-fPIC", "-I", INCLUDE, "-I", sysconfig.get_paths()["include"],
+                              "-I", os.path.join(os.path.dirname(importlib.util.find_spec("torch").origin), "include"),
                               "-o", out + tag] + [os.path.join(CSRC, s) for s in LIBRARIES[library][0]], capture_output=True, text=True)
         if res.returncode:
             sys.stderr.write(res.stdout + res.stderr)

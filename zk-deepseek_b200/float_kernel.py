@@ -154,7 +154,7 @@ _write_pages = _sig("zkfp_write_pages", [_vp, _vp])
 _copy_pages = _sig("zkfp_copy_pages", [_vp, _i, _vp, _vp, _ll, _vp])
 _sample = _sig("zkfp_sample", [_vp, _vp])
 _calls.setup(torch.Tensor, torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.empty, torch.cuda.current_device,
-             ctypes.cast(_paged_scratch, _vp).value)
+             ctypes.cast(_paged_scratch, _vp).value, getattr(torch.Tensor, "__dlpack_c_exchange_api__", None))
 _embed = _sig("zkfp_embed", [_vp, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _f, _i, _vp])
 _add_norm = _sig("zkfp_add_norm", [_vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _ll, _d, _i, _vp])
 _norm_rows = _sig("zkfp_norm_rows", [_vp, _ll, _vp, _vp, _vp, _ll, _ll, _ll, _d, _i, _vp])
