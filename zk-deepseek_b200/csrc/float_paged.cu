@@ -49,11 +49,12 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
     float *L = M + kPlainRows, *F = L + kPlainRows;
     make_plan(p, plan);
     const long long units = plan.before[batch];
-    const int ctas = sharing(p, units), cta = blockIdx.x;
+    const Share share(p, units);
+    const int cta = blockIdx.x;
     if (tid == 0) no_cut(p, cta);
-    if (cta >= ctas || units == 0) return;
-    const long long u1 = range_begin(units, cta + 1, ctas);
-    long long u = range_begin(units, cta, ctas);
+    if (cta >= share.ctas || units == 0) return;
+    const long long u1 = share.begin(cta + 1);
+    long long u = share.begin(cta);
     Walk w;
     for (w.locate(p, plan, u); u < u1; w.next(p, plan)) {
         const int taken = (int)min((long long)w.left(p), u1 - u), j_begin = w.begin(p), j_end = w.end(p, taken);
@@ -61,7 +62,7 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
         u += taken;
         if (j_begin == j_end) continue;
         const bool whole = j_begin == 0 && j_end == w.count;
-        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, units, ctas, w, end);
+        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, share, w, end);
         const int slot = 2 * cta + (j_begin == 0 ? 1 : 0), row0 = w.t * kPlainRows, rows = min(kPlainRows, w.n * p.group - row0);
         __syncthreads();
         for (int i = tid; i < kPlainRows * vd; i += kPlainThreads) {
@@ -230,11 +231,12 @@ paged_few_kernel(const __grid_constant__ Paged p)
     }
     make_plan(p, plan);
     const long long units = plan.before[batch];
-    const int ctas = sharing(p, units), cta = blockIdx.x;
+    const Share share(p, units);
+    const int cta = blockIdx.x;
     if (tid == 0) no_cut(p, cta);
-    if (cta >= ctas || units == 0) return;
-    const long long u1 = range_begin(units, cta + 1, ctas);
-    long long u = range_begin(units, cta, ctas);
+    if (cta >= share.ctas || units == 0) return;
+    const long long u1 = share.begin(cta + 1);
+    long long u = share.begin(cta);
     // scores: keys kg + 8 e, pairs sp, sp + 4, ... of the head; then rows r0 and on.  Values: column pairs cl + 16 k, keys 8 i + 4 kh + 0 .. 3.
     const int kg = lane & 7, sp = lane >> 3, r0 = R / 2 * (sp & 1) + kEach * (sp >> 1), cl = lane & 15, kh = lane >> 4;
     const int line_of = lane & (kFewKeys - 1);
@@ -252,7 +254,7 @@ paged_few_kernel(const __grid_constant__ Paged p)
         u += taken;
         if (j_begin == j_end) continue;
         const bool whole = j_begin == 0 && j_end == w.count;
-        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, units, ctas, w, end);
+        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, share, w, end);
         const int slot = 2 * cta + (j_begin == 0 ? 1 : 0), row0 = w.t * R, rows = min(R, w.n * p.group - row0);
         const float* from = values ? (const float*)a.v + w.kv * a.v_head : (const float*)a.k + w.kv * a.k_head;
         const long long page_step = values ? a.v_page : a.k_page, line_step = values ? a.v_pos : a.k_pos;
@@ -491,11 +493,12 @@ paged_block_kernel(const __grid_constant__ Paged p)
     }
     make_plan(p, plan);
     const long long units = plan.before[batch];
-    const int ctas = sharing(p, units), cta = blockIdx.x;
+    const Share share(p, units);
+    const int cta = blockIdx.x;
     if (tid == 0) no_cut(p, cta);
-    if (cta >= ctas || units == 0) return;
-    const long long u1 = range_begin(units, cta + 1, ctas);
-    long long u = range_begin(units, cta, ctas);
+    if (cta >= share.ctas || units == 0) return;
+    const long long u1 = share.begin(cta + 1);
+    long long u = share.begin(cta);
     // scores: keys kg + 8 e, pairs sp, sp + 4, ... of the head; then rows r0 and r0 + 1 of the warp's.  Values: column pairs cl + 16 k, keys 8 i + 4 kh + 0 .. 3.
     const int kg = lane & 7, sp = lane >> 3, r0 = 4 * (sp & 1) + 2 * (sp >> 1), cl = lane & 15, kh = lane >> 4;
     const float scale = a.scale * 1.4426950408889634f;
@@ -508,7 +511,7 @@ paged_block_kernel(const __grid_constant__ Paged p)
         u += taken;
         if (j_begin == j_end) continue;
         const bool whole = j_begin == 0 && j_end == w.count;
-        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, units, ctas, w, end);
+        if (tid == 0 && j_begin == 0 && !whole) write_cut(p, cta, share, w, end);
         const int slot = 2 * cta + (j_begin == 0 ? 1 : 0), row0 = w.t * kBlockRows, rows = min(kBlockRows, w.n * p.group - row0);
         const T *kb = (const T*)a.k + w.kv * a.k_head, *vb = (const T*)a.v + w.kv * a.v_head;
         // A thread asks for one line of a block, keys or values; its page is looked up a block ahead, and looked at when it is needed.
@@ -848,16 +851,14 @@ int launch_cores(Paged& p, cudaStream_t st)
 }
 
 // grid and tile of the kernel that a call takes
-void choose(Paged& p)
+void choose_kernel(Paged& p)
 {
-    p.shift = page_shift(p.a.page);
-    set_group(p, p.a.heads / p.a.kv_heads);
     const int path = zkfp_paged_path(&p.a);
     if (path == 2) return paged_stream_shape(p);
     if (path == 1) return paged_tile_shape(p);
     const long long rows = p.a.max_tokens * p.group;
     p.over = 1;
-    p.least = 2;
+    p.least = 1;
     if (p.a.dtype != ZKFP_BF16 && rows <= kFewRows) {
         p.tile = rows <= 4 ? 4 : 8;
         p.block = kFewBlock;
@@ -873,6 +874,17 @@ void choose(Paged& p)
         p.block = kBlockKeys;
         p.grid = grid_of(s.smem, s.pairs <= 3 ? 3 : 2);
     }
+}
+
+void choose(Paged& p)
+{
+    p.shift = page_shift(p.a.page);
+    p.group = p.a.heads / p.a.kv_heads;
+    choose_kernel(p);
+    p.by_groups.set(p.group);
+    p.by_tiles.set(p.tile);
+    p.by_blocks.set(p.block);
+    p.by_heads.set(p.a.kv_heads);
 }
 
 bool paged_ok(const zkfp_paged_attention_args* a)

@@ -33,11 +33,25 @@ __device__ __forceinline__ int sequence_of_row(const int* rows, int batch, long 
 // leaves its sums, and paged_combine_kernel merges them in the order of the keys.  Results depend on lengths alone, not on timing.
 constexpr int kPagedBatch = 1024;
 
+// A division whose divisor the host knows, of 0 <= x < 2^31: the high bits of a product.  (The multiplier is 2^shift / divisor rounded up, its error
+// times x below 2^shift.  What starts a launch is a chain of such steps, each of a CTA's few: with divisions one sequence took 13.2 us, now 12.8, 64 87.3, now 84.5.)
+struct Ratio {
+    uint32_t mul;
+    int shift;
+    void set(int divisor)
+    {
+        int s = 0;
+        while ((1 << s) < divisor) ++s;
+        shift = 31 + s;
+        mul = (uint32_t)(((1ull << shift) + divisor - 1) / divisor);
+    }
+    __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * mul) >> shift); }
+};
+
 struct Paged {
     zkfp_paged_attention_args a;
-    int shift, group, tile, block, grid, over, least;
-    uint32_t group_mul;              // a division by `group`: the high bits of a product
-    int group_shift;
+    int shift, group, tile, block, grid, over, least;          // least: 2 to its power
+    Ratio by_groups, by_tiles, by_blocks, by_heads;
     float* part;                     // [2 * grid][tile][dv] weighted sums; first the item that began in front of a CTA's
     float* ml;                       // [2 * grid][tile][2] maximum, sum        range, then the one that ends behind it
     int* cut;                        // [grid][8] the item that begins in a CTA's range and ends behind it
@@ -58,16 +72,7 @@ struct Plan {
 };
 inline size_t plan_bytes(long long batch) { return ((size_t)(batch + 1) * 8 + (size_t)batch * 12 + 15) & ~(size_t)15; }
 
-// x / group for x < 2^30 (the multiplier is 2^shift / group rounded up, its error times x below 2^shift)
-inline void set_group(Paged& p, int group)
-{
-    int s = 0;
-    while ((1 << s) < group) ++s;
-    p.group = group;
-    p.group_shift = 30 + s;
-    p.group_mul = (uint32_t)(((1ull << p.group_shift) + group - 1) / group);
-}
-__device__ __forceinline__ int by_group(const Paged& p, int x) { return (int)(((uint64_t)(uint32_t)x * p.group_mul) >> p.group_shift); }
+__device__ __forceinline__ int by_group(const Paged& p, int x) { return p.by_groups(x); }
 
 // the first position that a row at position i (which may be negative) sees
 __device__ __forceinline__ int first_seen(const Paged& p, int i) { return p.a.window > 0 && i >= p.a.window ? i - p.a.window + 1 : 0; }
@@ -78,14 +83,14 @@ __device__ __forceinline__ void tile_blocks(const Paged& p, int n, int len, int 
     const int last_row = min((t + 1) * p.tile, n * p.group) - 1;
     const int i0 = len - n + by_group(p, t * p.tile), i1 = len - n + by_group(p, last_row);
     if (i1 < 0) { first = 0; count = 1; return; }
-    first = first_seen(p, i0) / p.block;
-    count = i1 / p.block - first + 1;
+    first = p.by_blocks(first_seen(p, i0));
+    count = p.by_blocks(i1) - first + 1;
 }
 
 __device__ __forceinline__ int tiles_of(const Paged& p, int n)
 {
     const int rows = n * p.group;
-    return rows <= p.tile ? (rows > 0 ? 1 : 0) : (rows + p.tile - 1) / p.tile;
+    return p.by_tiles(rows + p.tile - 1);
 }
 
 __device__ __forceinline__ long long warp_sum64(long long v)
@@ -158,17 +163,26 @@ __device__ __forceinline__ void make_plan(const Paged& p, const Plan& s)
     __syncthreads();
 }
 
-// CTAs that share the units
-__device__ __forceinline__ int sharing(const Paged& p, long long units)
-{
-    const long long most = units / p.least;
-    return most < 1 ? 1 : most < p.grid ? (int)most : p.grid;
-}
-__device__ __forceinline__ long long range_begin(long long units, int cta, int ctas)
-{
-    if (units < 0x200000) return (uint32_t)units * (uint32_t)cta / (uint32_t)ctas;      // ctas < 2048
-    return units * cta / ctas;
-}
+// CTAs that share the units, how many each, and how many CTAs one more
+struct Share {
+    int ctas, more;
+    long long each;
+    __device__ __forceinline__ Share(const Paged& p, long long units)
+    {
+        const long long most = units >> p.least;
+        ctas = most < 1 ? 1 : most < p.grid ? (int)most : p.grid;
+        each = units < 0x80000000ll ? (uint32_t)units / (uint32_t)ctas : units / ctas;
+        more = (int)(units - each * ctas);
+    }
+    __device__ __forceinline__ long long begin(int cta) const { return cta * each + min(cta, more); }
+    // the first CTA whose range begins at unit u or behind it
+    __device__ __forceinline__ int behind(long long u) const
+    {
+        const long long longer = more * (each + 1);
+        const long long by = u <= longer ? each + 1 : each, in = (u <= longer ? u : u - longer) + by - 1;
+        return (u <= longer ? 0 : more) + (in < 0x80000000ll ? (int)((uint32_t)in / (uint32_t)by) : (int)(in / by));
+    }
+};
 
 // one item and the part of it that starts at unit u; whole warps walk, every warp by itself
 struct Walk {
@@ -192,8 +206,8 @@ struct Walk {
         b = lo;
         sequence(p, s);
         const long long mine = s.before[b + 1] - s.before[b], in = u - s.before[b];
-        const long long per = mine < 0x80000000ll ? (uint32_t)mine / (uint32_t)p.a.kv_heads : mine / p.a.kv_heads;
-        kv = (int)(in < 0x80000000ll && per < 0x80000000ll ? (uint32_t)in / (uint32_t)per : in / per);
+        const long long per = mine < 0x80000000ll ? p.by_heads((int)mine) : mine / p.a.kv_heads;
+        kv = p.a.kv_heads == 1 ? 0 : (int)(mine < 0x80000000ll ? (uint32_t)in / (uint32_t)per : in / per);
         long long rest = in - kv * per;
         const int lane = threadIdx.x & 31;
         for (int t0 = 0;; t0 += 32) {                  // ends: rest < per, the sum of all tiles
@@ -242,13 +256,10 @@ struct Walk {
 // What paged_combine_kernel has to know of the item whose first block CTA `cta` takes and whose last one it does not: in how many
 // parts it was taken, 0 for none.  `end`: the unit behind the item's last.  One thread writes it, of every CTA of the grid.
 __device__ __forceinline__ void no_cut(const Paged& p, int cta) { p.cut[cta * 8] = 0; }
-__device__ __forceinline__ void write_cut(const Paged& p, int cta, long long units, int ctas, const Walk& w, long long end)
+__device__ __forceinline__ void write_cut(const Paged& p, int cta, const Share& share, const Walk& w, long long end)
 {
-    // the first CTA whose range begins behind it
-    const long long behind = end >= units ? ctas : units < 0x100000 ? ((uint32_t)end * (uint32_t)ctas + (uint32_t)units - 1) / (uint32_t)units
-                                                                    : (end * ctas + units - 1) / units;
     int4* to = (int4*)(p.cut + cta * 8);
-    to[0] = make_int4((int)behind - cta, w.b, w.kv, w.t);
+    to[0] = make_int4(share.behind(end) - cta, w.b, w.kv, w.t);
     to[1] = make_int4(w.row0, w.n, w.len, 0);
 }
 

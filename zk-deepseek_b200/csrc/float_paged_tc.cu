@@ -56,7 +56,7 @@ constexpr int kStretchSeg = kStretch * 128;            // bytes of 16 keys x 64 
 constexpr int kStreamStages = 4;
 // An item by itself costs about as much as 6 blocks of 64 keys, or 2 tiles of 128 (64 sequences up to 8192, microseconds, at 2, 3, 4, 5, 6: 127,
 // 110, 95, 91, 88; a chunk beside decoding sequences at 2, 3, 4: 116, 117, 119; a prompt 170, 171, 175).
-constexpr int kStreamOver = 6, kStreamLeast = 4, kTileOver = 2, kTileLeast = 2;
+constexpr int kStreamOver = 6, kStreamLeast = 2, kTileOver = 2, kTileLeast = 1;
 
 struct StreamShape {
     int segk, segv, box, stages;
@@ -152,13 +152,14 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     }
     make_plan(p, plan);
     const long long units = plan.before[batch];
-    const int ctas = sharing(p, units), cta = blockIdx.x;
-    if (cta >= ctas || units == 0) return;
-    const long long u1 = range_begin(units, cta + 1, ctas);
+    const Share share(p, units);
+    const int cta = blockIdx.x;
+    if (cta >= share.ctas || units == 0) return;
+    const long long u1 = share.begin(cta + 1);
     const uint32_t one = elect_one(), my_bars = smem_u32(bars + warp * stages);
     uint8_t* my_ring = ring + warp * stages * kStage;
     Cursor at;
-    at.u = range_begin(units, cta, ctas);
+    at.u = share.begin(cta);
     at.w.locate(p, plan, at.u);
     bool more = at.part(p, plan, u1), loads = more, ok = true;
     Cursor in = at;                                            // the loads, as far ahead as the ring holds
@@ -221,7 +222,7 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     for (; more; more = at.next(p, plan, u1)) {
         const Walk& w = at.w;
         const int row0 = w.t * p.tile, rows = min(p.tile, w.n * p.group - row0), halves = rows > 8 ? 2 : 1;
-        if (threadIdx.x == 0 && at.begins && !at.whole) write_cut(p, cta, units, ctas, w, at.item_end);
+        if (threadIdx.x == 0 && at.begins && !at.whole) write_cut(p, cta, share, w, at.item_end);
         // queries: rows r and r + 8, elements cq, cq + 1 and eight further on of every 16
         uint32_t q[SEGK * 4][4];
         int pos[2] = {-1, -1};
@@ -556,16 +557,17 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tc_fence_after();
     const uint32_t tmem = s.tmem;
     const long long units = plan.before[a.batch];
-    const int ctas = sharing(p, units), cta = blockIdx.x;
-    const bool works = cta < ctas && units > 0;
+    const Share share(p, units);
+    const int cta = blockIdx.x;
+    const bool works = cta < share.ctas && units > 0;
 
     if (warp == 0) {
         const uint32_t one = elect_one();
         int ks = 0, vs = 0;
         uint32_t kp = 0, vp = 0, qp = 0;
         bool ok = true;
-        long long u = works ? range_begin(units, cta, ctas) : 0;
-        const long long u1 = works ? range_begin(units, cta + 1, ctas) : 0;
+        long long u = works ? share.begin(cta) : 0;
+        const long long u1 = works ? share.begin(cta + 1) : 0;
         Walk w;
         if (works) w.locate(p, plan, u);
         if (one) no_cut(p, cta);
@@ -586,7 +588,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const int taken = (int)min((long long)w.left(p), u1 - u);
             part = part_of(t, w, taken);
             if (part.begin == part.end) break;                 // units of an item that others take
-            if (one && part.begins && !part.whole) write_cut(p, cta, units, ctas, w, u + w.left(p));
+            if (one && part.begins && !part.whole) write_cut(p, cta, share, w, u + w.left(p));
             if (!(ok = publish())) break;
             if (!(ok = mbar_wait_warp(smem_u32(&s.q_empty), qp ^ 1u, abort_flag))) break;
             qp ^= 1u;
