@@ -447,9 +447,9 @@ paged_few_kernel(const __grid_constant__ Paged p)
 // eight rows; only keys and values need all of them to meet.  They have one place each: the next block's keys are on their way under the
 // softmax and the second product of this one, its values under the next scores.  Rows of keys are shifted by one 16-byte piece against each other,
 // which meets no bank twice.
-// Chunks of 100 tokens of three sequences, 16 heads of 72 over 4, the last 300 of up to 777 positions: 38 us, 6 of them to the first scores, 5 for the cut
-// items.  128 tokens of four sequences up to 1024, heads of 128: 96.  (Blocks of 64 keys 44 and 92, of 32 keys 40 and 109; four rows by two
-// keys a thread 42 and 116.)
+// Chunks of 100 tokens of three sequences, 16 heads of 72 over 4, the last 300 of up to 777 positions: 35 us, 5 of them to the first scores, 5 for the cut
+// items.  128 tokens of four sequences up to 1024, heads of 128: 88.  (When these took 38 and 96: blocks of 64 keys 44 and 92, of 32 keys 40 and 109,
+// four rows by two keys a thread 42 and 116.)
 constexpr int kBlockRows = 32, kBlockKeys = 48, kKeysEach = kBlockKeys / 8, kBlockThreads = 128, kWarpRows = 8, kWeightPitch = kBlockKeys + 4;
 
 struct BlockShared {

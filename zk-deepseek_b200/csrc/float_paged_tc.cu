@@ -55,7 +55,8 @@ constexpr int kStreamWarps = 4, kStretch = 16, kStreamRows = 16, kStreamKeys = k
 constexpr int kStretchSeg = kStretch * 128;            // bytes of 16 keys x 64 columns
 constexpr int kStreamStages = 4;
 // An item by itself costs about as much as 6 blocks of 64 keys, or 2 tiles of 128 (64 sequences up to 8192, microseconds, at 2, 3, 4, 5, 6: 127,
-// 110, 95, 91, 88; a chunk beside decoding sequences at 2, 3, 4: 116, 117, 119; a prompt 170, 171, 175).
+// 110, 95, 91, 88; a chunk beside decoding sequences at 2, 3, 4: 116, 117, 119; a prompt 170, 171, 175; today 84, 103 and 167).  No CTA takes less than
+// 4 blocks, or 2 tiles.
 constexpr int kStreamOver = 6, kStreamLeast = 2, kTileOver = 2, kTileLeast = 1;
 
 struct StreamShape {
