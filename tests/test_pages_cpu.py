@@ -393,3 +393,25 @@ def test_calls_refuse_what_is_on_no_gpu(K):
                 call()
     assert K.copy_pages([], [], []) is None and K.copy_pages([t["pages"]], [], []) is None
     assert {n: sys.getrefcount(x) for n, x in t.items()} == kept
+
+
+def test_a_copy_that_fails_changes_nothing():
+    def fails(*args, **kw):
+        raise RuntimeError("no copy")
+    c = make()
+    a = c.acquire()
+    c.extend(a, 0, 11)
+    write(c, a, 0, range(11))
+    b = c.fork(a)
+    before = [list(h) for h in c.held], list(c.lengths), c.free_pages(), c.free_slots()
+    c.copy = fails
+    for act in (lambda: c.extend_all([a, b], 11, 9), lambda: c.extend(b, 11, 1), lambda: c.fork(a), lambda: c.compact() or fails()):
+        with pytest.raises(RuntimeError):
+            act()
+        assert ([list(h) for h in c.held], list(c.lengths), c.free_pages(), c.free_slots()) == before
+        consistent(c)
+    c.copy = copy
+    c.extend_all([a, b], 11, 9)
+    write(c, a, 11, range(9))
+    assert read(c, a) == list(range(11)) + list(range(9)) and read(c, b)[:11] == list(range(11))
+    consistent(c)

@@ -105,7 +105,8 @@ class PagedCache:
         self.extend_all([slot], start, n)
 
     def extend_all(self, slots, start, n):
-        """the step about to run writes positions start .. start + n - 1 of these slots; nothing changes where it does not fit"""
+        """the step about to run writes positions start .. start + n - 1 of these slots; nothing changes where it does not fit or a copy
+        fails"""
         if len(set(slots)) != len(slots):
             raise ValueError("a slot twice in one step")
         for s in slots:
@@ -127,17 +128,19 @@ class PagedCache:
         more = -(-(start + n) // self.page) - -(-start // self.page)
         if len(copies) + more * len(slots) > len(self._spare):
             raise CacheFull("%d pages are free, the step takes %d" % (len(self._spare), len(copies) + more * len(slots)))
-        source, target = [], []
-        for s in copies:
-            source.append(self.held[s][last])
-            target.append(self._take())
-            self.held[s][last] = target[-1]
+        source, target = [self.held[s][last] for s in copies], [self._take() for _ in copies]
+        if source:
+            try:
+                self.copy(self._pools(), source, target, positions=inside)
+            except Exception:
+                self._give(target)
+                raise
+            for s, p in zip(copies, target):
+                self.held[s][last] = p
+            self._give(source)
         for s in slots:
             self.held[s].extend(self._take() for _ in range(more))
             self.lengths[s] = start + n
-        if source:
-            self.copy(self._pools(), source, target, positions=inside)
-            self._give(source)
         if source or more:
             self.version += 1
 
@@ -160,9 +163,13 @@ class PagedCache:
         self.held[new], self.lengths[new] = list(self.held[slot]), self.lengths[slot]
         for p in self.held[new]:
             self.counts[p] += 1
-        if self.lengths[slot]:
-            copy_states(self.copy, self.states, slot, new)
         self.version += 1
+        if self.lengths[slot]:
+            try:
+                copy_states(self.copy, self.states, slot, new)
+            except Exception:
+                self.release(new)
+                raise
         return new
 
     def compact(self):

@@ -76,8 +76,12 @@ class SequenceCache:
             from paged_cache import _copy_pages, copy_states
         new, n = self.acquire(), self.lengths[slot]
         if n:
-            _copy_pages([b for b in self.buffers if b is not None], [slot], [new], positions=n)
-            copy_states(_copy_pages, self.states, slot, new)
+            try:
+                _copy_pages([b for b in self.buffers if b is not None], [slot], [new], positions=n)
+                copy_states(_copy_pages, self.states, slot, new)
+            except Exception:
+                self.release(new)
+                raise
         self.lengths[new] = n
         return new
 
