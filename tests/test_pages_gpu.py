@@ -782,3 +782,11 @@ def test_tensors_that_require_gradients_are_read_all_the_same(K):
     half = torch.arange(96, device="cuda", dtype=torch.float16).reshape(3, 2, 16)                # a type that no other call takes
     K.copy_pages([half], [0], [2])
     assert torch.equal(half[2], half[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_bound_on_rows_of_any_size(K, dtype):
+    """and one that is too low, for tiles of rows that several CTAs take parts of"""
+    s = pool(dtype, [90, 3], [2000, 700], 32, 16, 2, 64, 48, fill=0.0)
+    for bound in (0, 1, 7, 90, 2 ** 31, 2 ** 62, 2 ** 70):
+        check(K, s, dtype, max_tokens=bound)

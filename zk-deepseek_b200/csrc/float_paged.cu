@@ -209,7 +209,6 @@ template <int R, int PAIRS>
 __global__ void __launch_bounds__(kFewThreads, PAIRS <= 4 ? 3 : 2)
 paged_few_kernel(const __grid_constant__ Paged p)
 {
-    chain_enter();
     extern __shared__ __align__(16) uint8_t sm[];
     const zkfp_paged_attention_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = a.d, dv = a.dv, kpitch = d + 4, batch = (int)a.batch;
@@ -229,6 +228,7 @@ paged_few_kernel(const __grid_constant__ Paged p)
         sh.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    chain_enter();                                     // barriers touch nobody else
     make_plan(p, plan);
     const long long units = plan.before[batch];
     const Share share(p, units);
@@ -473,7 +473,6 @@ template <typename T, int PAIRS>
 __global__ void __launch_bounds__(kBlockThreads, PAIRS <= 3 ? 3 : 2)
 paged_block_kernel(const __grid_constant__ Paged p)
 {
-    chain_enter();
     extern __shared__ __align__(16) uint8_t sm[];
     const zkfp_paged_attention_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = a.d, dv = a.dv, kpitch = d + 4, batch = (int)a.batch;
@@ -491,6 +490,7 @@ paged_block_kernel(const __grid_constant__ Paged p)
         sh.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    chain_enter();                                     // barriers touch nobody else
     make_plan(p, plan);
     const long long units = plan.before[batch];
     const Share share(p, units);
@@ -725,7 +725,12 @@ paged_block_kernel(const __grid_constant__ Paged p)
 // ---- cut items ---------------------------------------------------------------------------------------------------
 // Block x merges the item that CTA x began and did not end, a warp per row.  Maxima are in units of log2 where base2.  Lanes take the
 // parts' maxima and sums, 32 at a time, then all of them the columns of four parts at a time (eight: a prompt of 4096 173 instead of 169 us).
-template <typename T, int K>
+// Of large tiles a warp takes several rows, the next one's maxima and first two parts on their way under the one at work: blocks cost as
+// much as the rows do (chunks of 100, 40 and 33 tokens with a block per four rows 24.3, 24.3 and 26.9 us, with 24 blocks 20.1, 18.4 and 25.0, with 12
+// 22.8, 18.4 and 30.0).
+constexpr int kMergeBlocks = 24;                       // per item of a large tile
+
+template <typename T, int K, bool LARGE>
 __global__ void __launch_bounds__(128)
 paged_combine_kernel(const __grid_constant__ Paged p, int base2)
 {
@@ -738,47 +743,81 @@ paged_combine_kernel(const __grid_constant__ Paged p, int base2)
     w.b = what.y; w.kv = what.z; w.t = what.w;
     w.row0 = where.x; w.n = where.y; w.len = where.z;
     const int row0 = w.t * p.tile, rows = min(p.tile, w.n * p.group - row0);
-    const int r = blockIdx.y * 4 + (threadIdx.x >> 5);
+    int r = blockIdx.y * 4 + (threadIdx.x >> 5);
     if (r >= rows) return;
     // the first part lies in the second place of its CTA, the others in the first of theirs
-    auto place = [&](int i) { return (2ll * (c + i) + (i == 0)) * p.tile + r; };
-    float x[K][4] = {}, m = -INFINITY, l = 0.f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        const int n = min(parts - i0, 32);
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < n) ml = *(const float2*)(p.ml + place(i0 + lane) * 2);
-        const float m_new = fmaxf(m, warp_max(ml.x)), m_sub = m_new == -INFINITY ? 0.f : m_new;
-        // a part without a key that the row sees has no say, whatever its sums are
-        const float f = ml.x == -INFINITY ? 0.f : base2 ? exp2f(ml.x - m_sub) : expf(ml.x - m_sub);
-        const float old = m == -INFINITY ? 0.f : base2 ? exp2f(m - m_sub) : expf(m - m_sub);
-        l = l * old + (ml.x == -INFINITY ? 0.f : f * ml.y);
-        m = m_new;
-        const unsigned some = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
-        if (i0)
+    auto place = [&](int i, int row) { return (2ll * (c + i) + (i == 0)) * p.tile + row; };
+    auto maxima = [&](int i0, int row) {
+        return i0 + lane < parts ? *(const float2*)(p.ml + place(i0 + lane, row) * 2) : make_float2(-INFINITY, 0.f);
+    };
+    auto columns = [&](int i, int row, float (&y)[K][4]) {
 #pragma unroll
-            for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k)
+            if (4 * lane + 128 * k < dv) load4(p.part + place(i, row) * dv + 4 * lane + 128 * k, y[k]);
+    };
+    constexpr int kAhead = LARGE ? 2 : 0;
+    float2 ml = maxima(0, r);
+    float ahead[2][K][4] = {};
 #pragma unroll
-                for (int q = 0; q < 4; ++q) x[k][q] *= old;
-        for (int i = 0; i < n; i += 4) {
-            float y[4][K][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    if (i + e < n && (some >> (i + e) & 1) && 4 * lane + 128 * k < dv) load4(p.part + place(i0 + i + e) * dv + 4 * lane + 128 * k, y[e][k]);
-                    else y[e][k][0] = y[e][k][1] = y[e][k][2] = y[e][k][3] = 0.f;
-                }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float g = __shfl_sync(0xffffffffu, f, (i + e) & 31);
+    for (int e = 0; e < kAhead; ++e)
+        if (e < parts) columns(e, r, ahead[e]);
+    for (;;) {
+        float x[K][4] = {}, m = -INFINITY, l = 0.f;
+        const int next = r + 4 * gridDim.y;
+        for (int i0 = 0; i0 < parts; i0 += 32) {
+            const int n = min(parts - i0, 32);
+            if (i0) ml = maxima(i0, r);
+            const float m_new = fmaxf(m, warp_max(ml.x)), m_sub = m_new == -INFINITY ? 0.f : m_new;
+            // a part without a key that the row sees has no say, whatever its sums are
+            const float f = ml.x == -INFINITY ? 0.f : base2 ? exp2f(ml.x - m_sub) : expf(ml.x - m_sub);
+            const float old = m == -INFINITY ? 0.f : base2 ? exp2f(m - m_sub) : expf(m - m_sub);
+            l = l * old + (ml.x == -INFINITY ? 0.f : f * ml.y);
+            m = m_new;
+            const unsigned some = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+            if (i0)
 #pragma unroll
                 for (int k = 0; k < K; ++k)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) x[k][q] = fmaf(g, y[e][k][q], x[k][q]);
+                    for (int q = 0; q < 4; ++q) x[k][q] *= old;
+            else {
+#pragma unroll
+                for (int e = 0; e < kAhead; ++e) {
+                    const float g = __shfl_sync(0xffffffffu, f, e);
+#pragma unroll
+                    for (int k = 0; k < K; ++k)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) x[k][q] = some >> e & 1 ? fmaf(g, ahead[e][k][q], x[k][q]) : x[k][q];
+                }
+                if (LARGE && next < rows) {
+                    if (parts <= 32) ml = maxima(0, next);
+#pragma unroll
+                    for (int e = 0; e < kAhead; ++e)
+                        if (e < parts) columns(e, next, ahead[e]);
+                }
+            }
+            for (int i = i0 ? 0 : kAhead; i < n; i += 4) {
+                float y[4][K][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        if (i + e < n && (some >> (i + e) & 1) && 4 * lane + 128 * k < dv) load4(p.part + place(i0 + i + e, r) * dv + 4 * lane + 128 * k, y[e][k]);
+                        else y[e][k][0] = y[e][k][1] = y[e][k][2] = y[e][k][3] = 0.f;
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float g = __shfl_sync(0xffffffffu, f, (i + e) & 31);
+#pragma unroll
+                    for (int k = 0; k < K; ++k)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) x[k][q] = fmaf(g, y[e][k][q], x[k][q]);
+                }
             }
         }
+        finish_row<T>(p, w, row0 + r, x, warp_sum(l));
+        if (!LARGE || (r = next) >= rows) return;
+        if (parts > 32) ml = maxima(0, r);
     }
-    finish_row<T>(p, w, row0 + r, x, warp_sum(l));
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
@@ -792,9 +831,15 @@ int grid_of(size_t smem, int most)
 template <typename T>
 int launch_combine(const Paged& p, int base2, cudaStream_t st)
 {
+    const long long bound = p.a.max_tokens * p.group < p.tile ? p.a.max_tokens * p.group : p.tile, most = (bound + 3) / 4;
+    if (p.tile > 4 * kMergeBlocks) {
+        const dim3 grid((unsigned)p.grid, (unsigned)(most < 1 ? 1 : most > kMergeBlocks ? kMergeBlocks : most));
+        fp_launch(paged_combine_kernel<T, 1, true>, grid, dim3(128), 0, st, p, base2);          // dv <= 128
+        return fp_launched();
+    }
     const dim3 grid((unsigned)p.grid, (unsigned)(p.tile + 3) / 4);
-    if (p.a.dv <= 128) fp_launch(paged_combine_kernel<T, 1>, grid, dim3(128), 0, st, p, base2);
-    else fp_launch(paged_combine_kernel<T, 2>, grid, dim3(128), 0, st, p, base2);
+    if (p.a.dv <= 128) fp_launch(paged_combine_kernel<T, 1, false>, grid, dim3(128), 0, st, p, base2);
+    else fp_launch(paged_combine_kernel<T, 2, false>, grid, dim3(128), 0, st, p, base2);
     return fp_launched();
 }
 
@@ -876,8 +921,15 @@ void choose_kernel(Paged& p)
     }
 }
 
+// (so that products with it stay in range)
+void bound_tokens(zkfp_paged_attention_args& a)
+{
+    if (a.max_tokens > 1 << 30) a.max_tokens = 1 << 30;
+}
+
 void choose(Paged& p)
 {
+    bound_tokens(p.a);
     p.shift = page_shift(p.a.page);
     p.group = p.a.heads / p.a.kv_heads;
     choose_kernel(p);
@@ -913,8 +965,10 @@ extern "C" {
 int zkfp_paged_path(const zkfp_paged_attention_args* a)
 {
     if (!a || a->heads <= 0 || a->kv_heads <= 0 || a->heads < a->kv_heads || a->d <= 0 || a->dv <= 0 || a->batch <= 0) return 0;
-    if (paged_stream_takes(*a)) return 2;
-    return paged_tile_takes(*a) ? 1 : 0;
+    zkfp_paged_attention_args b = *a;
+    bound_tokens(b);
+    if (paged_stream_takes(b)) return 2;
+    return paged_tile_takes(b) ? 1 : 0;
 }
 
 long long zkfp_paged_scratch(const zkfp_paged_attention_args* a)

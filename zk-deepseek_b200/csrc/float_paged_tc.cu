@@ -133,7 +133,6 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     const __grid_constant__ Paged p, int box, int stages)
 {
     extern __shared__ uint8_t raw[];
-    chain_enter();
     const zkfp_paged_attention_args& a = p.a;
     constexpr uint32_t kLoad = (SEGK + SEGV) * kStretchSeg, kStage = kLoad > SEGV * 4096 ? kLoad : SEGV * 4096;      // also room for 16 rows of sums
     constexpr int kPitch = SEGV * 64;
@@ -148,10 +147,11 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     volatile int* abort_flag = gave_up;
     if (threadIdx.x == 0) {
         *gave_up = 0;
-        no_cut(p, blockIdx.x);
         for (int i = 0; i < kStreamWarps * stages; ++i) mbar_init(smem_u32(bars + i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    chain_enter();                                     // barriers touch nobody else
+    if (threadIdx.x == 0) no_cut(p, blockIdx.x);
     make_plan(p, plan);
     const long long units = plan.before[batch];
     const Share share(p, units);
@@ -519,7 +519,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                   const __grid_constant__ TileParams t)
 {
     extern __shared__ __align__(1024) uint8_t raw[];
-    chain_enter();
     const Paged& p = t.p;
     const zkfp_paged_attention_args& a = p.a;
     uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
@@ -552,6 +551,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
+    chain_enter();                                     // barriers touch nobody else
     if (warp == 1) tmem_alloc(smem_u32(&s.tmem), 512);
     make_plan(p, plan);
     tc_fence_before();
@@ -775,6 +775,24 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const bool any = first_tile <= last_tile, writes = quarter * 32 < rows, whole = part.whole;
             const int tok = part.token0 + in_seq, b = part.b, kv = part.kv, head = kv * p.group + part.row0[g] + row - in_seq * p.group;
             const long long slot = (2ll * cta + (part.begins ? 1 : 0)) * p.tile + g * t.rows + row;
+            // 32 bytes of every row pass through shared memory, so that a store meets 16 rows and not 32: lanes 2 r and 2 r + 1 take the
+            // halves of rows r and r + 16.  Gates come one step ahead, the first under the last products.
+            const int piece = lane & 1;
+            long long to[2], gate_at[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int who = (lane >> 1) + 16 * k;
+                const long long tk = __shfl_sync(0xffffffffu, tok, who), hd = __shfl_sync(0xffffffffu, head, who);
+                to[k] = quarter * 32 + who >= rows ? -1 : whole ? tk * a.o_tok + hd * a.o_head : (slot - lane + who) * a.dv;
+                gate_at[k] = tk * a.gate_tok + hd * a.gate_head;
+            }
+            const bool gated = whole && a.gate;
+            uint4 gate[2];
+            auto ask = [&](int col) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) gate[k] = gated && to[k] >= 0 && col < o_end ? *(const uint4*)((const bf16*)a.gate + gate_at[k] + col) : make_uint4(0, 0, 0, 0);
+            };
+            ask(o_begin + 8 * piece);
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s.part_empty[at]));
             at ^= 1;
@@ -790,18 +808,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     pair_sync();
                     l += s.most[3][g][half ^ 1][row];
                 }
-                // 32 bytes of every row pass through shared memory, so that a store meets 16 rows and not 32: lanes 2 r and 2 r + 1 take the
-                // halves of rows r and r + 16
                 uint8_t* stage = s.stage[warp - 2];
-                const int piece = lane & 1;
-                long long to[2], gate_at[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int who = (lane >> 1) + 16 * k;
-                    const long long tk = __shfl_sync(0xffffffffu, tok, who), hd = __shfl_sync(0xffffffffu, head, who);
-                    to[k] = quarter * 32 + who >= rows ? -1 : whole ? tk * a.o_tok + hd * a.o_head : (slot - lane + who) * a.dv;
-                    gate_at[k] = tk * a.gate_tok + hd * a.gate_head;
-                }
                 auto at_stage = [&](int r, int i) { return (uint4*)(stage + r * 32 + ((i ^ (r >> 2)) & 1) * 16); };
                 if (whole) {
                     const uint64_t r2 = twice(pos >= 0 ? 1.0f / l : 0.f);
@@ -818,8 +825,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         const int col = c + 8 * piece;
                         if (a.gate) {
 #pragma unroll
-                            for (int k = 0; k < 2; ++k)
-                                *at_stage((lane >> 1) + 16 * k, piece) = to[k] >= 0 && col < o_end ? *(const uint4*)((const bf16*)a.gate + gate_at[k] + col) : make_uint4(0, 0, 0, 0);
+                            for (int k = 0; k < 2; ++k) *at_stage((lane >> 1) + 16 * k, piece) = gate[k];
+                            ask(col + 16);
                             __syncwarp();
                         }
                         if (blank && pos < 0)
