@@ -943,7 +943,7 @@ bool paged_ok(const zkfp_paged_attention_args* a)
 {
     return a && a->q && a->k && a->v && a->out && a->table && a->rows && a->lengths && a->tokens >= 0 && a->pages > 0 && a->table_cols > 0 &&
            a->table_ld >= a->table_cols && a->batch > 0 && a->max_tokens >= 0 && a->kv_heads > 0 && a->heads > 0 &&
-           a->heads % a->kv_heads == 0 && a->scale >= 0.f && a->scale < 3e38f && a->window >= 0 && !((uintptr_t)a->scratch & 15) && a->d > 0 && a->dv > 0 && !(a->d & 7) && !(a->dv & 7) && page_shift(a->page) >= 0 && (unsigned)a->dtype <= 1 &&
+           a->heads % a->kv_heads == 0 && a->scale >= 0.f && a->scale < 3e38f && a->window >= 0 && !((uintptr_t)a->scratch & 31) && a->d > 0 && a->dv > 0 && !(a->d & 7) && !(a->dv & 7) && page_shift(a->page) >= 0 && (unsigned)a->dtype <= 1 &&
            !((a->q_tok | a->q_head | a->k_page | a->k_pos | a->k_head | a->v_page | a->v_pos | a->v_head | a->o_tok | a->o_head | a->gate_tok |
               a->gate_head) & 7) &&
            !(((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out | (uintptr_t)a->gate) & 15);

@@ -775,15 +775,15 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const bool any = first_tile <= last_tile, writes = quarter * 32 < rows, whole = part.whole;
             const int tok = part.token0 + in_seq, b = part.b, kv = part.kv, head = kv * p.group + part.row0[g] + row - in_seq * p.group;
             const long long slot = (2ll * cta + (part.begins ? 1 : 0)) * p.tile + g * t.rows + row;
-            // 32 bytes of every row pass through shared memory, so that a store meets 16 rows and not 32: lanes 2 r and 2 r + 1 take the
-            // halves of rows r and r + 16.  Gates come one step ahead, the first under the last products.
+            // Of an item that is whole, 32 bytes of every row pass through shared memory, so that a store meets 16 rows and not 32: lanes 2 r and
+            // 2 r + 1 take the halves of rows r and r + 16; sums of a part go out 32 bytes a row and store.  Gates come one step ahead, the first under the last products.
             const int piece = lane & 1;
             long long to[2], gate_at[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int who = (lane >> 1) + 16 * k;
                 const long long tk = __shfl_sync(0xffffffffu, tok, who), hd = __shfl_sync(0xffffffffu, head, who);
-                to[k] = quarter * 32 + who >= rows ? -1 : whole ? tk * a.o_tok + hd * a.o_head : (slot - lane + who) * a.dv;
+                to[k] = quarter * 32 + who >= rows ? -1 : tk * a.o_tok + hd * a.o_head;
                 gate_at[k] = tk * a.gate_tok + hd * a.gate_head;
             }
             const bool gated = whole && a.gate;
@@ -864,19 +864,17 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                                            o_begin, o_end);
                     }
                 } else {
-#pragma unroll 1
+                    float* mine = p.part + slot * a.dv;
+#pragma unroll 2
                     for (int c = o_begin; c < o_end; c += 8) {
                         int32_t y[8] = {};
                         if (any) {
                             tmem_ld8(tO + (uint32_t)c, y);
                             tmem_ld_wait();
                         }
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) *at_stage(lane, k) = *reinterpret_cast<uint4*>(&y[4 * k]);
-                        __syncwarp();
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            if (to[k] >= 0) *(uint4*)(p.part + to[k] + c + 4 * piece) = *at_stage((lane >> 1) + 16 * k, piece);
+                        if (row < rows)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(mine + c), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
+                                         "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
                         __syncwarp();
                     }
                     if (row < rows) p.ml[slot * 2 + half] = half ? l : m;
