@@ -11,7 +11,7 @@
 // holds (logits that are equal, or nearly), the key is found 8 bits at a time instead.
 //
 // Latency bounds it: a pass over the row for each limit and one for the draw, and the cluster's barriers between them.  One row of 129280 with top p
-// 20 to 23 us (8 without a limit), 64 rows of 32768 with top k 16, 256 rows of 129280 with limits of their own 191: 37 rows at a time, as many as
+// 20 to 27 us (8 without a limit), 64 rows of 32768 with top k 16, 256 rows of 129280 with limits of their own 191: 37 rows at a time, as many as
 // shared memory holds, for reading a row again from memory for every pass costs more (265).
 #include <cooperative_groups.h>
 
