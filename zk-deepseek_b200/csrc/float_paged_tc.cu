@@ -15,8 +15,8 @@
 //   warp 1      MMA issue
 //   warps 2-9   softmax, tile 0    warps 10-17 softmax, tile 1: two threads share a query row, half of the columns each
 // The running maximum only replaces the one in use when it has grown by more than 2^8, and then in front of the next tile, where the
-// output tile is rescaled in place: a tile's weights are made from the maximum in use, without looking for the new one first (what
-// outgrows even 32 bits that way does not come out finite, and is taken again).  Weights go to the second product in halves, so that it
+// output tile is rescaled in place: a tile's weights are made from the maximum in use, without looking for the new one first.  A row whose
+// scores outgrow that by more than 2^100 within one tile is marked by a sum that is NaN, and is taken again.  Weights go to the second product in halves, so that it
 // starts under the other half.  CTAs stay and take one part of an item after the other.  What bounds it is one tile's softmax under the other's
 // products: a prompt of 4096, 32 heads of 128 over 8, takes 167 us, 0.82 PFLOP/s, the tensor pipe active for 44 %, the exponentials' for as much.
 #include <cuda.h>
@@ -374,6 +374,7 @@ constexpr int kTile = 128;                     // query rows and keys per tile
 constexpr uint32_t kSeg = kTile * 128;         // bytes of 128 rows x 64 bfloat16
 constexpr int kTileThreads = 576, kTileMost = 128;
 constexpr int kMaxKeySlots = 8;
+constexpr float kMostGrown = 100.f;            // log2 of how far scores may be above the maximum in use
 
 struct TileParams {
     Paged p;
@@ -765,6 +766,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     if (masked) l += weigh<true>(tS, c0, c_lo, c_hi, scale2, sub, most);
                     else l += weigh<false>(tS, c0, 0, 0, scale2, sub, most);
                     s.most[j & 1][g][half][row] = most;
+                    // In front of the next tile, or where parts are merged, this one's sums are multiplied by 2^-(most - m).  Up to 2^100 neither that nor
+                    // the sums leave the range of 32 bits (128 weights a tile, 2^-126 the smallest number that is not flushed).
+                    if (most * t.scale_log2 - m > kMostGrown) l = __int_as_float(0x7fffffff);
                     tmem_st_wait();
                 }
                 tc_fence_before();
