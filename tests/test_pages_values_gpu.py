@@ -1,10 +1,11 @@
-"""Values that calls over pages meet rarely: scores that jump from one tile of keys to the next."""
+"""Values that calls over pages meet rarely: scores that jump from one tile of keys to the next, keys that are NaN or infinite where a
+row does see them."""
 import numpy as np
 import pytest
 import torch
 
 from oracle import float_oracle as fo
-from test_pages_gpu import HALF, K, attend, i32, limit, np64, pool, rnd  # noqa: F401 (K is a fixture)
+from test_pages_gpu import DTYPES, HALF, K, attend, check, i32, limit, np64, pool, rnd  # noqa: F401 (K is a fixture)
 
 pytestmark = pytest.mark.gpu
 LN2 = float(np.float32(np.log(2.0)))                   # with it as scale, scores count in powers of two
@@ -83,3 +84,61 @@ def test_scores_that_jump_under_a_gate(K):
     # either result is rounded once, and the sigmoid of bfloat16 results is good to more than they are
     assert (np.abs(got - want) <= 4 * HALF["bfloat16"] * np.abs(want) + 1e-30).all()
     K.device_status(sync=True)
+
+
+# ---- keys that are seen ------------------------------------------------------------------------------------------
+ENDS = [17, 33, 49, 65, 97, 129, 193, 257, 385, 641]   # the last position by itself in a warp's stretch, a block or a tile
+
+
+def spoil(s, lengths, value, element=slice(None)):
+    """the newest key of every sequence"""
+    for b, n in enumerate(lengths):
+        s["k"][s["host"][0][b][(n - 1) // 16], (n - 1) % 16, :, element] = value
+
+
+@pytest.mark.parametrize("d", [64, 136])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,heads,kv", [(1, 3, 3), (1, 4, 1), (3, 4, 2), (20, 6, 3)])
+@pytest.mark.parametrize("lengths", [[n] for n in ENDS] + [ENDS, ENDS[::-1] * 3, [385] * 7], ids=lambda x: "%dx%d" % (len(x), x[0]))
+def test_a_newest_key_that_is_nan(K, dtype, d, new, heads, kv, lengths):
+    """the rows that see it are NaN in every column, the others as if it were not there"""
+    s = pool(dtype, [new] * len(lengths), lengths, 16, heads, kv, d, d)
+    last = np.arange(1, len(lengths) + 1) * new - 1
+    want = np64(attend(K, s, dtype, d ** -0.5, max_tokens=new))
+    spoil(s, lengths, float("nan"))
+    got = np64(attend(K, s, dtype, d ** -0.5, max_tokens=new))
+    K.device_status(sync=True)
+    blind = np.ones(len(got), bool)
+    blind[last] = False
+    assert np.isnan(got[last]).all(), np.isnan(got[last]).mean()
+    assert np.isfinite(want).all() and np.isfinite(got[blind]).all()
+    if blind.any():
+        assert np.abs(got - want)[blind].max() <= 4 * HALF[dtype] * (np.abs(want).max() + 4.0) + (2e-5 if dtype == "float32" else 0)
+
+
+@pytest.mark.parametrize("d", [64, 136])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("new", [1, 20])
+def test_an_element_of_the_newest_key_that_is_not_finite(K, dtype, d, new, bad):
+    """+infinity as a score gives NaN, -infinity weighs nothing: what the formula says in 64 bits"""
+    s = pool(dtype, [new] * len(ENDS), ENDS, 16, 4, 2, d, d)
+    spoil(s, ENDS, bad, 3)
+    got = np64(attend(K, s, dtype, d ** -0.5, max_tokens=new))
+    K.device_status(sync=True)
+    table, rows, lengths = s["host"]
+    with np.errstate(invalid="ignore"):
+        want, size, score = fo.paged_attention(np64(s["q"]), np64(s["k"]), np64(s["v"]), table, rows, lengths, d ** -0.5)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and (bad != bad or not np.isnan(want).all())
+    fine = np.isfinite(want)
+    # scores of normal numbers: |q k| scale stays below 8 for all but the spoiled key
+    off = np.abs(got - want) - limit(dtype, size, np.full_like(score, 8.0), d, max(ENDS)) - HALF[dtype] * np.abs(want)
+    assert (off[fine] <= 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 20])
+def test_a_scale_of_zero_is_the_mean(K, dtype, new):
+    s = pool(dtype, [new] * 4, [17, 100, 385, 700], 16, 4, 2, 64, 64)
+    check(K, s, dtype, scale=0.0, max_tokens=new)
+    check(K, s, dtype, scale=0.0, window=33, max_tokens=new)

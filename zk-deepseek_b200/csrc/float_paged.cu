@@ -412,7 +412,10 @@ paged_few_kernel(const __grid_constant__ Paged p)
             for (int o = 0; o < kFewWarps; ++o) top = fmaxf(top, sh.m[o][i]);
 #pragma unroll
             for (int o = 0; o < kFewWarps; ++o) {
-                if (sh.m[o][i] == -INFINITY) continue;
+                if (sh.m[o][i] == -INFINITY) {
+                    sum += sh.l[o][i];                 // 0, or NaN where a visible score was
+                    continue;
+                }
                 const float g = exp2_approx(sh.m[o][i] - top);
                 sum = fmaf(g, sh.l[o][i], sum);
 #pragma unroll
@@ -768,10 +771,11 @@ paged_combine_kernel(const __grid_constant__ Paged p, int base2)
             const int n = min(parts - i0, 32);
             if (i0) ml = maxima(i0, r);
             const float m_new = fmaxf(m, warp_max(ml.x)), m_sub = m_new == -INFINITY ? 0.f : m_new;
-            // a part without a key that the row sees has no say, whatever its sums are
+            // A part without a score above -infinity has no say, whatever its sums are; its sum of weights is 0, or NaN where a visible score was,
+            // which makes the row NaN and has it taken again.
             const float f = ml.x == -INFINITY ? 0.f : base2 ? exp2f(ml.x - m_sub) : expf(ml.x - m_sub);
             const float old = m == -INFINITY ? 0.f : base2 ? exp2f(m - m_sub) : expf(m - m_sub);
-            l = l * old + (ml.x == -INFINITY ? 0.f : f * ml.y);
+            l = l * old + (ml.x == -INFINITY ? ml.y : f * ml.y);
             m = m_new;
             const unsigned some = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
             if (i0)

@@ -345,7 +345,10 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
             for (int i = 0; i < kStreamWarps; ++i) {
                 const float mi = M[i * kStreamRows + rr];
-                if (mi == -INFINITY) continue;
+                if (mi == -INFINITY) {
+                    sum += L[i * kStreamRows + rr];            // 0, or NaN where a visible score was
+                    continue;
+                }
                 const float g = exp2_approx(mi - top);
                 sum = fmaf(g, L[i * kStreamRows + rr], sum);
                 if (lane * 4 < kPitch) {
