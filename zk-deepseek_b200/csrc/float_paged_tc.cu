@@ -377,7 +377,10 @@ constexpr int kTile = 128;                     // query rows and keys per tile
 constexpr uint32_t kSeg = kTile * 128;         // bytes of 128 rows x 64 bfloat16
 constexpr int kTileThreads = 576, kTileMost = 128;
 constexpr int kMaxKeySlots = 8;
-constexpr float kMostGrown = 100.f;            // log2 of how far scores may be above the maximum in use
+// log2 of how far a tile's scores may be above the maximum in use, so that neither its sums (128 weights) nor the factor that brings them down
+// in front of the next tile, or where parts are merged, leave the range of 32 bits (factors below 2^-126 are flushed to zero).  Looked at where the
+// maximum is replaced and behind the last tile; behind every tile costs a prompt of 4096 3 %.
+constexpr float kMostGrown = 100.f;
 
 struct TileParams {
     Paged p;
@@ -756,7 +759,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                             for (int i = 0; i < 8; ++i) o[i] = __float_as_int(__int_as_float(o[i]) * f);
                             tmem_st8(tO + (uint32_t)c, o);
                         }
-                        l *= f;
+                        l = top - m > kMostGrown ? __int_as_float(0x7fffffff) : l * f;
                         m = m == -INFINITY ? m : fmaxf(m, top);
                     }
                     if (__any_sync(0xffffffffu, m == -INFINITY)) {      // rows that have not seen a key yet
@@ -769,9 +772,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     if (masked) l += weigh<true>(tS, c0, c_lo, c_hi, scale2, sub, most);
                     else l += weigh<false>(tS, c0, 0, 0, scale2, sub, most);
                     s.most[j & 1][g][half][row] = most;
-                    // In front of the next tile, or where parts are merged, this one's sums are multiplied by 2^-(most - m).  Up to 2^100 neither that nor
-                    // the sums leave the range of 32 bits (128 weights a tile, 2^-126 the smallest number that is not flushed).
-                    if (most * t.scale_log2 - m > kMostGrown) l = __int_as_float(0x7fffffff);
                     tmem_st_wait();
                 }
                 tc_fence_before();
@@ -811,6 +811,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
             if (writes) {
                 if (any) {                                // (without a tile nothing keeps the halves from the next part's place)
+                    if (s.most[last_tile & 1][g][half][row] * t.scale_log2 - m > kMostGrown) l = __int_as_float(0x7fffffff);
                     s.most[3][g][half][row] = l;
                     pair_sync();
                     l += s.most[3][g][half ^ 1][row];
