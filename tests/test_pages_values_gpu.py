@@ -1,5 +1,5 @@
 """Values that calls over pages meet rarely: scores that jump from one tile of keys to the next, keys that are NaN or infinite where a
-row does see them."""
+row does see them, infinities and NaN among heads that do not turn."""
 import numpy as np
 import pytest
 import torch
@@ -142,3 +142,69 @@ def test_a_scale_of_zero_is_the_mean(K, dtype, new):
     s = pool(dtype, [new] * 4, [17, 100, 385, 700], 16, 4, 2, 64, 64)
     check(K, s, dtype, scale=0.0, max_tokens=new)
     check(K, s, dtype, scale=0.0, window=33, max_tokens=new)
+
+
+# ---- heads that do not turn --------------------------------------------------------------------------------------
+def odd(shape, dtype, seed):
+    """normal numbers with infinities, zeros of both signs and NaN with bits of their own among them"""
+    x = rnd(shape, dtype, seed)
+    bits = x.view(torch.int16 if dtype == "bfloat16" else torch.int32)
+    shift = 0 if dtype == "bfloat16" else 16
+    g = torch.Generator().manual_seed(seed + 1)
+    kind = torch.randint(0, 12, shape, generator=g).cuda()
+    for i, b in enumerate((0x7f80, -0x80, 0x7fc0, 0x7fa5, -0x8000, 0)):
+        bits[kind == i] = b << shift
+    return x
+
+
+def same_bits(a, b):
+    t = torch.int16 if a.dtype == torch.bfloat16 else torch.int32
+    return torch.equal(a.contiguous().view(t), b.contiguous().view(t))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["pairs", "half"])
+@pytest.mark.parametrize("d,pairs", [(64, 16), (64, 5), (64, 32), (24, 3), (256, 40), (8, 0)])
+def test_what_does_not_turn_is_copied(K, dtype, layout, d, pairs):
+    new, lengths, page, heads, kv = [3, 0, 40], [9, 5, 33], 8, 5, 2
+    s = pool(dtype, new, lengths, page, heads, kv, d, 16, fill=0.0)
+    table, rows, _ = s["host"]
+    n = sum(new)
+    q, k, v = odd((n, heads, d), dtype, 3), odd((n, kv, d), dtype, 5), odd((n, kv, 16), dtype, 7)
+    place = [(b, lengths[b] - new[b] + t) for b in range(3) for t in range(new[b])]
+
+    def run(cos_sin):
+        s["k"].zero_()
+        s["v"].zero_()
+        out = torch.empty_like(q)
+        K.write_pages(k, v, s["k"], s["v"], s["table"], s["rows"], s["lengths"], q=q, q_out=out, cos_sin=cos_sin, layout=layout)
+        K.device_status(sync=True)
+        kept = [(r, table[b, i // page], i % page) for r, (b, i) in enumerate(place) if i >= 0]
+        r, p, l = (torch.tensor(x).cuda() for x in zip(*kept))
+        assert same_bits(s["v"][p, l], v[r])
+        return out, s["k"][p, l], k[r], np.array([i for _, i in place]), np.array([i for _, i in place if i >= 0])
+
+    out, got, want, pos, kpos = run(None)
+    assert same_bits(out, q) and same_bits(got, want)
+    if not pairs:
+        return
+    # angles for some of the positions only: the others keep their heads, and every head keeps its part behind the pairs
+    held = 20
+    angles = torch.outer(torch.arange(held).double(), 0.37 ** torch.arange(pairs).double())
+    cos_sin = torch.stack((angles.cos(), angles.sin()), -1).float().cuda()
+    out, got, want, pos, kpos = run(cos_sin)
+    assert same_bits(out[..., 2 * pairs:], q[..., 2 * pairs:]) and same_bits(got[..., 2 * pairs:], want[..., 2 * pairs:])
+    for x, y, i in ((out, q, pos), (got, want, kpos)):
+        plain = torch.from_numpy((i < 0) | (i >= held)).cuda()
+        assert same_bits(x[plain], y[plain]) and not plain.all()
+        # the others: NaN where the formula has it, else two products and their sum in 32 bits and one rounding
+        for r in np.nonzero(~plain.cpu().numpy())[0]:
+            for h in range(x.shape[1]):
+                with np.errstate(invalid="ignore"):
+                    w = fo.turned(np64(y[r, h]), np64(cos_sin[i[r]]), layout)[:2 * pairs]
+                g = np64(x[r, h])[:2 * pairs]
+                big = np.abs(np64(y[r, h])[np.isfinite(np64(y[r, h]))]).max()
+                assert np.array_equal(np.isnan(g), np.isnan(w))
+                fine = np.isfinite(w)
+                assert np.array_equal(g[~fine & ~np.isnan(w)], w[~fine & ~np.isnan(w)])
+                assert (np.abs(g[fine] - w[fine]) <= HALF[dtype] * np.abs(w[fine]) + 3 * 2.0 ** -24 * 2 * big).all()

@@ -57,12 +57,13 @@ bool moves_ok(const int* source, const int* target, long long moves, long long p
 
 // ---- heads into pages --------------------------------------------------------------------------------------------
 // A block takes one row and every gridDim.y-th group of its heads: queries, keys, then values.  A head is cut into units: eight elements of
-// adjacent pairs, two times eight of pairs half a rotation apart, or single pairs where those do not lie on 16-byte pieces; what does not
-// turn is copied.  A thread keeps its unit, and so its angles, from head to head, and has 64 bytes on their way at a time.
-// Every element is read and written by one thread, so q_out may be q.  Bytes bound it: two prompts of 4095 tokens, 128 + 2 x 16 heads of
-// 128, move 0.68 GB in 121 us (5.6 TB/s; one head at a time, angles loaded for each: 156).
+// adjacent pairs (which turn all or not at all, or some of them where the pairs end inside a unit), two times eight of pairs half a rotation apart, or
+// single pairs where those do not lie on 16-byte pieces; what does not turn is copied, bit by bit.  A thread keeps its unit, and so its angles, from head
+// to head, and has 64 bytes on their way at a time (single pairs: four of them).  Every element is read and written by one thread, so q_out may be q.
+// Bytes bound it: two prompts of 4095 tokens, 128 + 2 x 16 heads of 128, move 0.68 GB in 125 us (one head at a time, angles loaded for each: 156); in
+// halves, all or half of a head, 131 and 154, single pairs 391 (one at a time 485).  Units that choose pair by pair take 1 % longer, and are another kernel.
 constexpr int kWriteThreads = 256;
-enum { kAdjacent, kApart, kSingle };
+enum { kAdjacent, kAdjacentSome, kApart, kSingle };
 
 __device__ __forceinline__ void turn(float& a, float& b, float2 cs)
 {
@@ -74,43 +75,74 @@ __device__ __forceinline__ void turn(float& a, float& b, float2 cs)
 // eight elements as they lie in memory
 template <typename T>
 struct Eight {
-    uint4 v[sizeof(T) / 2];
+    static constexpr int N = sizeof(T) / 2;
+    uint4 v[N];
     __device__ __forceinline__ void load(const T* p)
     {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+        for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void store(T* p) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
     }
     __device__ __forceinline__ void get(float (&x)[8]) const { load8(reinterpret_cast<const T*>(v), x); }
+    __device__ __forceinline__ void put(const float (&x)[8]) { store8(reinterpret_cast<T*>(v), x); }
+    // the first `pairs` adjacent pairs
+    __device__ __forceinline__ void set(const float (&x)[8], int pairs)
+    {
+        Eight y;
+        y.put(x);
+        uint32_t *to = reinterpret_cast<uint32_t*>(v), *from = reinterpret_cast<uint32_t*>(y.v);
+#pragma unroll
+        for (int k = 0; k < 4 * N; ++k) to[k] = k / N < pairs ? from[k] : to[k];
+    }
 };
 
-// unit u of `heads` heads, from `src` to `dst`, heads `step` apart beginning with `first`
+// Unit u of `heads` heads, from `src` to `dst`, heads `step` apart beginning with `first`.  cs: null where nothing turns.
 template <typename T, int KIND>
 __device__ __forceinline__ void turn_heads(const T* src, long long src_head, T* dst, long long dst_head, int u, int pairs, const float2* cs, int first,
                                            int step, int heads)
 {
     if (KIND == kSingle) {
-        const bool turns = u < pairs;
-        const float2 t = turns && cs ? cs[u] : make_float2(1.f, 0.f);
-        for (int h = first; h < heads; h += step) {
-            const T* from = src + h * src_head;
-            T* to = dst + h * dst_head;
-            if (turns) {
-                float x = to_f32(from[u]), y = to_f32(from[u + pairs]);
-                turn(x, y, t);
-                to[u] = from_f32<T>(x);
-                to[u + pairs] = from_f32<T>(y);
-            } else {
-                to[u + pairs] = from[u + pairs];
-            }
+        constexpr int kAhead = 4;
+        const bool two = u < pairs, turns = two && cs;
+        const float2 t = turns ? cs[u] : make_float2(1.f, 0.f);
+        for (int h0 = first; h0 < heads; h0 += kAhead * step) {
+            T x[kAhead], y[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (h0 + i * step < heads) {
+                    const T* from = src + (h0 + i * step) * src_head + u;
+                    y[i] = from[pairs];
+                    if (two) x[i] = from[0];
+                }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (h0 + i * step < heads) {
+                    T* to = dst + (h0 + i * step) * dst_head + u;
+                    if (turns) {
+                        float a = to_f32(x[i]), b = to_f32(y[i]);
+                        turn(a, b, t);
+                        x[i] = from_f32<T>(a);
+                        y[i] = from_f32<T>(b);
+                    }
+                    if (two) to[0] = x[i];
+                    to[pairs] = y[i];
+                }
         }
         return;
     }
+    constexpr bool kNext = KIND != kApart;             // pairs are adjacent
     constexpr int V = KIND == kApart ? 2 : 1, N = KIND == kApart ? 8 : 4, kAhead = 8 / (int)sizeof(T) / V;
+    // pairs of this unit that turn; what does not is stored as it was loaded, bit by bit
+    const int turns = cs ? min(max(pairs - N * u, 0), N) : 0;
     float2 t[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) t[k] = cs && N * u + k < pairs ? cs[N * u + k] : make_float2(1.f, 0.f);
+    for (int k = 0; k < N; ++k) t[k] = k < turns ? cs[N * u + k] : make_float2(1.f, 0.f);
     // behind the pairs a unit of two is the second of its pieces alone
-    const bool both = KIND == kAdjacent || 8 * u < pairs;
+    const bool both = kNext || 8 * u < pairs;
     const int at[2] = {8 * u, 8 * u + pairs};
     for (int h0 = first; h0 < heads; h0 += kAhead * step) {
         Eight<T> raw[kAhead][V];
@@ -124,18 +156,24 @@ __device__ __forceinline__ void turn_heads(const T* src, long long src_head, T* 
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
             if (h0 + i * step < heads) {
-                float x[V][8];
+                if (kNext || turns) {
+                    float x[V][8];
 #pragma unroll
-                for (int v = 0; v < V; ++v) raw[i][v].get(x[v]);
-                if (both)
+                    for (int v = 0; v < V; ++v) raw[i][v].get(x[v]);
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
-                        if (KIND == kAdjacent) turn(x[0][2 * k & 7], x[0][(2 * k + 1) & 7], t[k]);
+                        if (kNext) turn(x[0][2 * k & 7], x[0][(2 * k + 1) & 7], t[k]);
                         else turn(x[0][k], x[V - 1][k], t[k]);
                     }
 #pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        if (kNext) raw[i][v].set(x[v], KIND == kAdjacentSome ? turns : turns == N ? 4 : 0);      // (a branch: 1 % longer)
+                        else raw[i][v].put(x[v]);
+                    }
+                }
+#pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (v == V - 1 || both) store8(dst + (h0 + i * step) * dst_head + at[v], x[v]);
+                    if (v == V - 1 || both) raw[i][v].store(dst + (h0 + i * step) * dst_head + at[v]);
             }
     }
 }
@@ -165,7 +203,7 @@ write_pages_kernel(const __grid_constant__ zkfp_write_pages_args a, int shift, i
     const bool turned = a.cos_sin && pos >= 0 && pos < a.positions;
     const float2* cs = (const float2*)a.cos_sin + (turned ? pos * a.pairs : 0);
     // a row without angles is copied, in the units of the others
-    const int pairs = turned || KIND != kAdjacent ? a.pairs : 0;
+    const int pairs = turned || KIND == kApart || KIND == kSingle ? a.pairs : 0;
     const int units = KIND == kSingle ? a.d - a.pairs : (KIND == kApart ? a.d - a.pairs : a.d) / 8;
     const int per = units < kWriteThreads ? kWriteThreads / units : 1, step = per * gridDim.y, head = blockIdx.y * per + (int)threadIdx.x / units;
     if ((int)threadIdx.x < per * units || units > kWriteThreads)
@@ -181,9 +219,9 @@ write_pages_kernel(const __grid_constant__ zkfp_write_pages_args a, int shift, i
     const int vecs = a.dv / 8;
     for (int i = blockIdx.y * kWriteThreads + threadIdx.x; i < a.kv_heads * vecs; i += kWriteThreads * gridDim.y) {
         const int g = i / vecs, c = (i - g * vecs) * 8;
-        float x[8];
-        load8((const T*)a.v + r * a.v_tok + g * a.v_head + c, x);
-        store8((T*)a.v_pages + page * a.v_page + line * a.v_pos + g * a.vp_head + c, x);
+        Eight<T> x;
+        x.load((const T*)a.v + r * a.v_tok + g * a.v_head + c);
+        x.store((T*)a.v_pages + page * a.v_page + line * a.v_pos + g * a.vp_head + c);
     }
 }
 
@@ -196,7 +234,8 @@ int write_pages(const zkfp_write_pages_args& a, int* flag, cudaStream_t st)
     gy = gy > most ? most : gy;
     const dim3 grid((unsigned)a.tokens, (unsigned)(gy < 1 ? 1 : gy)), block(kWriteThreads);
     const int shift = page_shift(a.page);
-    if (!a.half) fp_launch(write_pages_kernel<T, kAdjacent>, grid, block, 0, st, a, shift, flag);
+    if (!a.half && a.pairs & 3) fp_launch(write_pages_kernel<T, kAdjacentSome>, grid, block, 0, st, a, shift, flag);
+    else if (!a.half) fp_launch(write_pages_kernel<T, kAdjacent>, grid, block, 0, st, a, shift, flag);
     else if (a.pairs & 7) fp_launch(write_pages_kernel<T, kSingle>, grid, block, 0, st, a, shift, flag);
     else fp_launch(write_pages_kernel<T, kApart>, grid, block, 0, st, a, shift, flag);
     return fp_launched();
