@@ -1,5 +1,5 @@
 """Values that calls over pages meet rarely: scores that jump from one tile of keys to the next, keys that are NaN or infinite where a
-row does see them, infinities and NaN among heads that do not turn."""
+row does see them, what lies behind the end of a sequence, and infinities and NaN among heads that do not turn."""
 import numpy as np
 import pytest
 import torch
@@ -142,6 +142,36 @@ def test_a_scale_of_zero_is_the_mean(K, dtype, new):
     s = pool(dtype, [new] * 4, [17, 100, 385, 700], 16, 4, 2, 64, 64)
     check(K, s, dtype, scale=0.0, max_tokens=new)
     check(K, s, dtype, scale=0.0, window=33, max_tokens=new)
+
+
+# ---- behind the end ----------------------------------------------------------------------------------------------
+def test_stale_lines_cost_no_more_than_zeros(K):
+    """a chunk whose last pages hold NaN behind the end of the sequence takes as long as over a zeroed pool (within a factor of two; rows
+    that are all taken again one by one take many times as long)"""
+    best = {}
+    for fill in (0.0, float("nan"), 0.0, float("nan")):
+        s = pool("bfloat16", [256], [4001], 64, 16, 4, 128, 128, fill=fill)
+        out = torch.empty_like(s["q"])
+        call = lambda: K.paged_attention(s["q"], s["k"], s["v"], s["table"], s["rows"], s["lengths"], out, 128 ** -0.5, max_tokens=256)
+        for _ in range(3):
+            call()
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            call()
+            b.record()
+            b.synchronize()
+            best[fill == 0.0] = min(best.get(fill == 0.0, 1e9), a.elapsed_time(b))
+    assert best[False] <= 2 * best[True], best
+
+
+@pytest.mark.parametrize("length", [1, 5, 127, 128, 129, 250, 383, 4001])
+@pytest.mark.parametrize("page", [8, 64, 256])
+def test_stale_lines_of_any_kind(K, length, page):
+    """bfloat16 chunks: infinities and NaN behind the end, over pages smaller and larger than a tile"""
+    for fill in (float("nan"), float("inf"), -float("inf")):
+        s = pool("bfloat16", [33, 40], [length, 77], page, 2, 1, 72, 80, fill=fill)
+        check(K, s, "bfloat16", max_tokens=40)
 
 
 # ---- heads that do not turn --------------------------------------------------------------------------------------

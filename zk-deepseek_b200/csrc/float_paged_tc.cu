@@ -394,7 +394,7 @@ struct TileParams {
 // tile g takes part in, and the rows of g.
 struct Part {
     int begin, end, row0[2], rows[2], first[2], last[2];
-    int b, kv, token0, base;                   // sequence, key head, first token of the sequence, position of that
+    int b, kv, token0, base, len;              // sequence, key head, first token of the sequence, position of that, positions of the sequence
     int begins, whole;
 };
 
@@ -412,6 +412,7 @@ __device__ __forceinline__ Part part_of(const TileParams& t, const Walk& w, int 
     x.kv = w.kv;
     x.token0 = w.row0;
     x.base = w.len - w.n;
+    x.len = w.len;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
         x.row0[g] = w.t * t.p.tile + g * t.rows;
@@ -519,6 +520,16 @@ __device__ __forceinline__ float weigh(uint32_t tS, int c0, int c_lo, int c_hi, 
     unpair(add_pair(add[0], add[1]), e, f);
     top = fmaxf(most[0], most[1]);
     return e + f;
+}
+
+// Lines of a tile of values from `held` on, which the sequence does not hold: no value, whatever is there.  (A function of its own, out of the way of
+// the products: a prompt of 4096 182 us, with it in the loop 185.)
+__device__ __noinline__ void blank_lines(uint8_t* tile, int held, int segments)
+{
+    for (int c = 0; c < segments; ++c)
+        for (int i = held * 8 + (threadIdx.x & 31); i < kTile * 8; i += 32) *(uint4*)(tile + (uint32_t)c * kSeg + i * 16) = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
 }
 
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -642,7 +653,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t one = elect_one(), tm = uniform(tmem);
         const uint32_t idesc_s = idesc_bf16(kTile, kTile), idesc_o = idesc_bf16(kTile, (a.dv + 15) & ~15, true);
         uint32_t pp[2] = {0, 0}, op[2] = {0, 0}, kp = 0, vp = 0, qp = 0, phase = 0;
-        int ks = 0, vs = 0, at = 0, begin = 0, end = 0, first[2] = {0, 0}, last[2] = {0, 0};
+        int ks = 0, vs = 0, at = 0, begin = 0, end = 0, len = 0, first[2] = {0, 0}, last[2] = {0, 0};
         // the sums of query tile g over the keys that are there, and its scores with the tile of keys that follows
         auto values = [&](const int g, int j) {
             if (j == first[g]) {                               // the last part's sums have been read
@@ -691,6 +702,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (!wait_awake(smem_u32(&s.part_full[at]), phase, abort_flag)) break;
             begin = (int)uniform(s.part[at].begin);
             end = (int)uniform(s.part[at].end);
+            len = (int)uniform(s.part[at].len);
+            const bool ragged = end > len / kTile;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 first[g] = (int)uniform(s.part[at].first[g]);
@@ -707,6 +720,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (ok && begin + 1 == end) umma_commit(smem_u32(&s.q_empty), one);
             for (int j = begin; j < end && ok; ++j) {
                 if (!(ok = wait_awake(smem_u32(&s.v_full[vs]), vp, abort_flag))) break;
+                if (ragged && j + 1 == end) blank_lines(base + (sV - sQ) + (uint32_t)vs * bytesV, len & (kTile - 1), t.segv);
                 tc_fence_after();
                 if (j >= first[0] && j <= last[0]) ok = values(0, j);
                 if (ok && j + 1 < end) ok = scores(0, j + 1);
