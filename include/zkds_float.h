@@ -228,7 +228,7 @@ int zkfp_gated_norm(const zkfp_gated_norm_args* a, void* stream);
  * table_cols * page positions.  Rows rows[b] .. rows[b + 1] - 1 of a batch are the newest tokens of sequence b, which
  * holds lengths[b] positions with them: row rows[b] + t sits at position lengths[b] - (rows[b + 1] - rows[b]) + t.
  * All three are device data and are checked there: what lies outside the tensors is not read or written, and
- * zkfp_device_status() reports it.  Rows behind rows[batch] are left as they were.  A page that takes new rows is one sequence's. */
+ * zkfp_device_status() reports it (2).  Rows behind rows[batch] are left as they were.  A page that takes new rows is one sequence's. */
 
 /* Softmax attention of new tokens over pages: a row sees the positions up to its own (window > 0: the last `window` of
  * them); a row at a negative position sees none and gives zeros.  Keys and values that a row does not see have no part in
@@ -323,7 +323,7 @@ int zkfp_linear_path(const zkfp_linear_args* a);
 int zkfp_attention_path(const zkfp_attention_args* a);
 int zkfp_scan_path(const zkfp_scan_args* a);
 
-/* 5 if since the last call a finished kernel gave up a bounded wait, or met pages, rows or lengths that do not fit, else 0 */
+/* 5 if a finished kernel gave up a bounded wait since a call last said so; else 2 if, likewise, one met pages, rows or lengths that do not fit; else 0 */
 int zkfp_device_status(void);
 long long zkfp_launches(void);      /* kernels launched by this library so far */
 int zkfp_cuda_error(void);          /* cudaError_t behind the last status 3 of this thread */

@@ -1,5 +1,6 @@
 """Values that calls over pages meet rarely: scores that jump from one tile of keys to the next, keys that are NaN or infinite where a
-row does see them, what lies behind the end of a sequence, and infinities and NaN among heads that do not turn."""
+row does see them, what lies behind the end of a sequence, infinities and NaN among heads that do not turn, and the status of
+what does not fit."""
 import numpy as np
 import pytest
 import torch
@@ -238,3 +239,27 @@ def test_what_does_not_turn_is_copied(K, dtype, layout, d, pairs):
                 fine = np.isfinite(w)
                 assert np.array_equal(g[~fine & ~np.isnan(w)], w[~fine & ~np.isnan(w)])
                 assert (np.abs(g[fine] - w[fine]) <= HALF[dtype] * np.abs(w[fine]) + 3 * 2.0 ** -24 * 2 * big).all()
+
+
+# ---- the status --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,new,d", [("bfloat16", 1, 64), ("bfloat16", 40, 64), ("bfloat16", 1, 136), ("bfloat16", 40, 136), ("float32", 1, 64), ("float32", 40, 64)])
+def test_a_status_of_its_own_for_what_does_not_fit(K, dtype, new, d):
+    """pages outside the pool and rows outside the batch are no waits that ran out, whichever kernel meets them"""
+    s = pool(dtype, [new, new], [100, 90], 16, 4, 2, d, d, fill=0.0)
+    out, kv = torch.empty_like(s["q"]), torch.ones_like(s["q"][:, :2])
+    attention = lambda: K.paged_attention(s["q"], s["k"], s["v"], s["table"], s["rows"], s["lengths"], out, 0.1, max_tokens=new)
+    write = lambda: K.write_pages(kv, kv, s["k"], s["v"], s["table"], s["rows"], s["lengths"])
+    K.device_status(sync=True)
+    for name, at, value in (("table", (0, 6), -1), ("rows", (2,), 2 * new + 9)):
+        kept = s[name].clone()
+        s[name][at] = value
+        for call in (attention, write):
+            call()
+            torch.cuda.synchronize()
+            with pytest.raises(K.FloatOpsError, match="do not fit") as e:
+                K.device_status()
+            assert e.value.status == 2
+            K.device_status()                          # it is said once
+        s[name].copy_(kept)
+    attention()
+    K.device_status(sync=True)

@@ -46,7 +46,7 @@ int* fp_error_flag()
     if (!g_flag_host[dev]) {
         int* h = nullptr;
         if (cudaHostAlloc((void**)&h, 64, cudaHostAllocMapped) != cudaSuccess) return nullptr;
-        h[0] = 0;
+        h[0] = h[1] = 0;
         int* d = nullptr;
         if (cudaHostGetDevicePointer((void**)&d, h, 0) != cudaSuccess) return nullptr;
         g_flag_dev[dev] = d;
@@ -150,9 +150,12 @@ int zkfp_device_status(void)
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !g_flag_host[dev]) return ZKDS_OK;
     volatile int* h = g_flag_host[dev];
-    const int v = h[0];
-    h[0] = 0;
-    return v ? ZKDS_ERR_DEVICE : ZKDS_OK;
+    for (int i = 0; i < 2; ++i)
+        if (h[i]) {
+            h[i] = 0;
+            return i ? ZKDS_ERR_RANGE : ZKDS_ERR_DEVICE;
+        }
+    return ZKDS_OK;
 }
 
 long long zkfp_launches(void) { return g_launches.load(); }

@@ -15,7 +15,7 @@ constexpr int kSharedMax = 227 * 1024;  // dynamic shared memory a CTA may ask f
 
 int fp_sm_count();
 int fp_launched();                      // cudaGetLastError -> status, counts the launch
-int* fp_error_flag();                   // device view of the host-mapped word that bounded waits set
+int* fp_error_flag();                   // device view of two host-mapped words: set by bounded waits, and by pages, rows or lengths that do not fit
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }

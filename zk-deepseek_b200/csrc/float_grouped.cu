@@ -28,7 +28,7 @@ heads_post_kernel(const zkfp_heads_args a, const zkfp_page_table pages, int shif
         block = pages.table[b * pages.ld + (pos >> shift)];
         line = pos & (pages.page - 1);
         if (block < 0 || block >= pages.pages) {               // the same for the whole row
-            if (threadIdx.x % LANES == 0) *(volatile int*)error_flag = 1;
+            if (threadIdx.x % LANES == 0) *(volatile int*)(error_flag + 1) = 1;
             return;
         }
     } else {

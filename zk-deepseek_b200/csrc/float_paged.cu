@@ -82,7 +82,7 @@ paged_plain_kernel(const __grid_constant__ Paged p, int kpitch)
             for (int i = tid; i < kPlainKeys * (vd + vv); i += kPlainThreads) {
                 const int r = i / (vd + vv), c = i - r * (vd + vv);
                 const long long page = r < nk ? page_of(p, w.b, k0 + r) : -1;
-                if (r < nk && page < 0) *(volatile int*)p.error_flag = 1;
+                if (r < nk && page < 0) *(volatile int*)(p.error_flag + 1) = 1;
                 const long long line = (k0 + r) & (a.page - 1);
                 const T* src = c < vd ? (const T*)a.k + page * a.k_page + line * a.k_pos + w.kv * a.k_head + c * 8
                                       : (const T*)a.v + page * a.v_page + line * a.v_pos + w.kv * a.v_head + (c - vd) * 8;
@@ -267,7 +267,7 @@ paged_few_kernel(const __grid_constant__ Paged p)
         auto request = [&](int j, int page) {
             const int k = key_of(j);
             const bool there = k < w.len && page >= 0 && page < a.pages;
-            if (k < w.len && !there) *(volatile int*)p.error_flag = 1;
+            if (k < w.len && !there) *(volatile int*)(p.error_flag + 1) = 1;
             if (there) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // zeros that the line held
                 mbar_expect_tx(bar, size * 4);
@@ -532,7 +532,7 @@ paged_block_kernel(const __grid_constant__ Paged p)
                 if (tid >= kBlockKeys) return;
                 const int k = k0 + tid;
                 const bool there = k < w.len && page >= 0 && page < a.pages;
-                if (k < w.len && !there) *(volatile int*)p.error_flag = 1;
+                if (k < w.len && !there) *(volatile int*)(p.error_flag + 1) = 1;
                 const uint32_t bar = values ? smem_u32(&sh.v_full) : smem_u32(&sh.k_full);
                 if (there) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // zeros that the line held
@@ -546,7 +546,7 @@ paged_block_kernel(const __grid_constant__ Paged p)
                 for (int i = tid; i < kBlockKeys * (size / 4); i += kBlockThreads) {
                     const int n = i / (size / 4), c = 4 * (i - n * (size / 4)), k = k0 + n;
                     const long long at = k < w.len ? page_of(p, w.b, k) : -1;
-                    if (k < w.len && at < 0) *(volatile int*)p.error_flag = 1;
+                    if (k < w.len && at < 0) *(volatile int*)(p.error_flag + 1) = 1;
                     float x[4] = {};
                     if (at >= 0) load4(from + at * page_step + (k & (a.page - 1)) * line_step + c, x);
                     store4(to + n * pitch + c, x);

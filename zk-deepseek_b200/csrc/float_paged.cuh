@@ -55,7 +55,7 @@ struct Paged {
     float* part;                     // [2 * grid][tile][dv] weighted sums; first the item that began in front of a CTA's
     float* ml;                       // [2 * grid][tile][2] maximum, sum        range, then the one that ends behind it
     int* cut;                        // [grid][8] the item that begins in a CTA's range and ends behind it
-    int* error_flag;
+    int* error_flag;                 // two words, see fp_error_flag
 };
 
 // in dynamic shared memory: (batch + 1) units in front of each sequence, then its first row, rows and positions
@@ -116,7 +116,7 @@ __device__ __forceinline__ void make_plan(const Paged& p, const Plan& s)
             bool bad = len < 0 || len > capacity;
             len = len < 0 ? 0 : len > capacity ? (int)capacity : len;
             if (row0 < 0 || row1 < row0 || row1 > p.a.tokens) { n = 0; bad = true; }
-            if (bad) *(volatile int*)p.error_flag = 1;
+            if (bad) *(volatile int*)(p.error_flag + 1) = 1;
         }
         const int tiles = tiles_of(p, n);
         long long units = 0;

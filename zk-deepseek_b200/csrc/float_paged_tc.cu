@@ -198,7 +198,7 @@ paged_stream_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                         if (page >= 0) page_id2 = (int)page;
                         else bad = true;
                     }
-                    if (bad) *(volatile int*)p.error_flag = 1;
+                    if (bad) *(volatile int*)(p.error_flag + 1) = 1;
                 }
                 __syncwarp();
             }
@@ -627,7 +627,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (loads && at < w.len) {
                     const long long page = page_of(p, w.b, at);
                     if (page >= 0) mine = (int)page;
-                    else *(volatile int*)p.error_flag = 1;
+                    else *(volatile int*)(p.error_flag + 1) = 1;
                 }
                 __syncwarp();
                 const int line = (j * kTile) & (a.page - 1);

@@ -188,7 +188,7 @@ write_pages_kernel(const __grid_constant__ zkfp_write_pages_args a, int shift, i
     if (b < 0) return;
     const int row0 = a.rows[b], n = a.rows[b + 1] - row0;
     const bool bad = row0 < 0 || row0 + (long long)n > a.tokens;
-    if ((bad || a.lengths[b] < 0) && threadIdx.x == 0) *(volatile int*)error_flag = 1;
+    if ((bad || a.lengths[b] < 0) && threadIdx.x == 0) *(volatile int*)(error_flag + 1) = 1;
     if (bad || row0 > r) return;
     const long long pos = (long long)a.lengths[b] - n + (r - row0);
     long long page = -1;
@@ -196,7 +196,7 @@ write_pages_kernel(const __grid_constant__ zkfp_write_pages_args a, int shift, i
         if ((pos >> shift) < a.table_cols) page = a.table[b * a.table_ld + (pos >> shift)];
         if (page < 0 || page >= a.pages) {
             page = -1;
-            if (threadIdx.x == 0) *(volatile int*)error_flag = 1;
+            if (threadIdx.x == 0) *(volatile int*)(error_flag + 1) = 1;
         }
     }
     const long long line = pos & (a.page - 1);

@@ -171,7 +171,7 @@ class FloatOpsError(RuntimeError):
 
 def _check(status, what):
     if status:
-        text = {1: "bad argument", 3: "CUDA error %d" % lib.zkfp_cuda_error(), 5: "a bounded wait ran out, or pages, rows or lengths do not fit",
+        text = {1: "bad argument", 3: "CUDA error %d" % lib.zkfp_cuda_error(), 2: "pages, rows or lengths do not fit", 5: "a bounded wait ran out",
                 6: "unsupported shape"}.get(status, "status %d" % status)
         raise FloatOpsError("%s: %s" % (what, text), status)
 
@@ -187,7 +187,7 @@ def _stream():
 
 
 def device_status(sync=False):
-    """raises if a finished kernel gave up a bounded wait, or met pages, rows or lengths that do not fit"""
+    """raises if a finished kernel gave up a bounded wait (status 5), or met pages, rows or lengths that do not fit (2)"""
     if sync:
         torch.cuda.current_stream().synchronize()
     _check(lib.zkfp_device_status(), "device status")
