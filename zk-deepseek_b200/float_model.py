@@ -26,11 +26,11 @@ from torch import nn
 
 try:
     from . import float_kernel as K
-    from .paged_cache import PagedCache
+    from .paged_cache import PagedCache, check_pages
     from .sequence_cache import SequenceCache
 except ImportError:  # pragma: no cover - this directory first on sys.path
     import float_kernel as K
-    from paged_cache import PagedCache
+    from paged_cache import PagedCache, check_pages
     from sequence_cache import SequenceCache
 
 # a step with at most this many tokens per sequence takes the decode form of attention: over the latents themselves, or over
@@ -38,6 +38,8 @@ except ImportError:  # pragma: no cover - this directory first on sys.path
 ABSORB_MAX_TOKENS = 16
 # a step with more rows than this is run in portions (bounds the activations and the expanded keys and values)
 MAX_STEP_TOKENS = 8192
+# largest head that attention over pages takes
+PAGED_MOST = 256
 
 
 def _padded(t, shape, dtype, device):
@@ -630,8 +632,13 @@ class FloatTransformer(nn.Module):
     def load_weights(self, W, device):
         """W(name, shape) returns a checked tensor"""
         args = self.args
-        if args.page and any(isinstance(layer.mixer, LatentAttention) for layer in self.layers):
-            raise NotImplementedError("layers of design %s keep latents, which live in slots and not in pages" % args.design.name)
+        if args.page:                     # refused before anything is read
+            check_pages(args.page, args.pages)
+            if any(isinstance(layer.mixer, LatentAttention) for layer in self.layers):
+                raise NotImplementedError("layers of design %s keep latents, which live in slots and not in pages" % args.design.name)
+            widest = max([m.d for m in self.modules() if isinstance(m, KeyValuedAttention)] + [0])
+            if widest > PAGED_MOST:
+                raise NotImplementedError("heads of %d elements live in slots, heads of up to %d in pages" % (widest, PAGED_MOST))
 
         def tables(rot):
             key = rot.base, rot.dims, rot.scaling

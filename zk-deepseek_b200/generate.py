@@ -162,6 +162,8 @@ def main(argv=None):
         ap.error("give at least one prompt, none of them empty")
     if args.samples < 1 or args.top_k < 0 or args.temperature < 0 or not 0 <= args.min_p <= 1 or not 0 < args.top_p <= 1:
         ap.error("--samples from 1, --top-k and --temperature from 0, --min-p and --top-p up to 1")
+    if (args.sample or args.samples > 1) and reg.architecture_of(reg.float_config.read_config(args.model)) == reg.INTEGER_MODEL:
+        ap.error("--sample and --samples are for the floating-point designs")
     more = {"page": args.page} if args.page else {}
     model = reg.load(args.model, dtype=args.dtype, max_seq_len=args.max_seq_len, max_batch_size=len(prompts) * args.samples, **more)
     vocab = model.args.vocab_size

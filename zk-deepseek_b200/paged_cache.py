@@ -25,17 +25,22 @@ def _copy_pages(buffers, source, target, positions=None):
     K.copy_pages(buffers, source, target, positions=positions)
 
 
+def check_pages(page, pages=None):
+    if page not in (8, 16, 32, 64, 128, 256, 512, 1024):
+        raise ValueError("pages of %r positions: a power of two from 8 to 1024" % (page,))
+    if pages is not None and pages < 1:
+        raise ValueError("a pool of %d pages" % pages)
+
+
 class PagedCache:
     def __init__(self, pitches, owners, slots, capacity, dtype, device, states=(), page=64, pages=None, copy=_copy_pages):
         """pitches, owners, slots, states: as for `SequenceCache`; capacity: most positions of a sequence; page: positions of a
         page; pages: of the pool (default: enough for all slots at their capacity); copy: what copies pages"""
-        if page not in (8, 16, 32, 64, 128, 256, 512, 1024):
-            raise ValueError("pages of %r positions: a power of two from 8 to 1024" % (page,))
+        check_pages(page, pages)
         self.slots, self.capacity, self.page, self.copy = slots, capacity, page, copy
         self.columns = -(-capacity // page)
         self.pages = slots * self.columns if pages is None else pages
-        if self.pages < 1:
-            raise ValueError("a pool of %d pages" % self.pages)
+        check_pages(page, self.pages)
         self.owners = list(owners)
         self.buffers = [None if p is None else torch.zeros(self.pages, page, p, dtype=dtype, device=device) for p in pitches]
         for i, o in enumerate(self.owners):

@@ -113,7 +113,8 @@ def load_integer_model(model_dir, device="cuda", max_seq_len=None, max_batch_siz
 def load(model_dir, dtype="bfloat16", device="cuda", max_seq_len=4096, max_batch_size=1, page=0, pages=None):
     """The model of a checkpoint directory, ready to run on `device`.  dtype belongs to the floating-point designs;
     the integer model has one number format.  page: positions of a page, for a cache in a pool of `pages` pages that sequences
-    share (0: a slot of max_seq_len positions each); for designs whose layers keep keys and values or a state."""
+    share (0: a slot of max_seq_len positions each); for designs whose layers keep keys and values, in heads of up to
+    256, or a state."""
     cfg = float_config.read_config(model_dir)
     if architecture_of(cfg) == INTEGER_MODEL:
         if page:
