@@ -56,7 +56,7 @@ def _compile(library, verbose):
     out = os.path.join(HERE, library)
     tag = ".%d.partial" % os.getpid()
     flags = FLAGS + (["-Xptxas", "-v"] if verbose else [])
-    if LIBRARIES[library][0][0].endswith(".c"):         # a Python module: no kernels; the interpreter's headers, and DLPack's
+    if LIBRARIES[library][0][0].endswith(".c"):         # a Python module: no kernels; the interpreter's headers, and DLPack's where torch has them
         res = subprocess.run([shutil.which("gcc") or "cc", "-O2", "-Wall", "-shared", "-fPIC", "-I", INCLUDE, "-I", sysconfig.get_paths()["include"],
                               "-I", os.path.join(os.path.dirname(importlib.util.find_spec("torch").origin), "include"),
                               "-o", out + tag] + [os.path.join(CSRC, s) for s in LIBRARIES[library][0]], capture_output=True, text=True)

@@ -1,13 +1,23 @@
 /* Argument structures of the calls over pages and of sampling, from torch tensors: what Python needs a microsecond a tensor for.
  * Every function looks its tensors over (types, shapes, strides, device), raises ValueError for what does not belong together
  * and gives the bytes of the structure that the call takes; it launches nothing and keeps nothing.  Tensors are read through DLPack's C
- * exchange interface (a versioned one: 0.05 us a tensor), and where that declines (a tensor that requires gradients, say) through their Python
- * attributes (0.4 us); nothing here depends on how torch was built. */
+ * exchange interface (a versioned one: 0.05 us a tensor), and where that declines (a tensor that requires gradients, say), or torch's headers or
+ * torch itself do not have it, through their Python attributes (0.4 us); nothing here depends on how torch was built. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
-#include <ATen/dlpack.h>
 #include <stdarg.h>
 #include <string.h>
+#ifdef __has_include
+#if __has_include(<ATen/dlpack.h>)
+#include <ATen/dlpack.h>
+#endif
+#endif
+/* the interface came with version 1.3 of the header */
+#if defined(DLPACK_MAJOR_VERSION) && DLPACK_MAJOR_VERSION == 1 && DLPACK_MINOR_VERSION >= 3
+#define EXCHANGE 1
+#else
+#define EXCHANGE 0
+#endif
 
 #include "zkds_float.h"
 
@@ -17,7 +27,9 @@ enum { kDims = 8 };
 static PyObject *tensor_type, *bfloat16, *float32, *int32, *int64, *empty, *current_device, *empty_names;
 static PyObject *n_dtype, *n_shape, *n_stride, *n_data_ptr, *n_get_device, *n_element_size;
 static long long (*paged_scratch)(const zkfp_paged_attention_args*);
+#if EXCHANGE
 static DLPackDLTensorFromPyObjectNoSync exchange;
+#endif
 
 static int refuse(const char* what, const char* format, ...)
 {
@@ -52,6 +64,7 @@ static int is_tensor(PyObject* t) { return PyObject_TypeCheck(t, (PyTypeObject*)
 static int see(const char* what, const char* name, PyObject* t, Tensor* s)
 {
     if (!is_tensor(t)) return refuse(what, "%s is no tensor", name);
+#if EXCHANGE
     DLTensor d;
     if (exchange && exchange(t, &d)) PyErr_Clear();
     else if (exchange) {
@@ -69,6 +82,7 @@ static int see(const char* what, const char* name, PyObject* t, Tensor* s)
             return 0;
         }
     }
+#endif
     int rc = -1;
     s->element = 0;
     PyObject *dtype = PyObject_GetAttr(t, n_dtype), *shape = NULL, *stride = NULL, *at = NULL, *device = NULL;
@@ -485,9 +499,11 @@ static PyObject* setup(PyObject* self, PyObject* const* x, Py_ssize_t count)
     if (count != 9 || !PyType_Check(x[0])) return PyErr_Format(PyExc_TypeError, "setup: 9 arguments, a type first");
     const unsigned long long at = PyLong_AsUnsignedLongLong(x[7]);
     if (PyErr_Occurred()) return NULL;
+#if EXCHANGE
     const DLPackExchangeAPI* api = x[8] == Py_None ? NULL : (const DLPackExchangeAPI*)PyCapsule_GetPointer(x[8], "dlpack_exchange_api");
     if (PyErr_Occurred()) return NULL;
     exchange = api && api->header.version.major == DLPACK_MAJOR_VERSION ? api->dltensor_from_py_object_no_sync : NULL;
+#endif
     for (int i = 0; i < 7; ++i) Py_XSETREF(*to[i], Py_NewRef(x[i]));
     paged_scratch = (long long (*)(const zkfp_paged_attention_args*))(uintptr_t)at;
     Py_RETURN_NONE;
