@@ -47,7 +47,7 @@ class PagedCache:
             if o is not None and self.buffers[o] is None:
                 raise ValueError("layer %d reads the entries of layer %d, which stores none" % (i, o))
         self.states = [{n: torch.zeros((slots,) + tuple(shape), dtype=dt, device=device) for n, (shape, dt) in s.items()} for s in states]
-        self._free = list(range(slots - 1, -1, -1))
+        self._free, self._taken = list(range(slots - 1, -1, -1)), [False] * slots
         self.lengths = [0] * slots
         self.held = [[] for _ in range(slots)]         # page numbers of every slot
         self.counts = [0] * self.pages
@@ -78,7 +78,7 @@ class PagedCache:
 
     # -- slots and pages -------------------------------------------------------------------------------------------
     def _used(self, slot):
-        if not 0 <= slot < self.slots or slot in self._free:
+        if not 0 <= slot < self.slots or not self._taken[slot]:
             raise ValueError("slot %d is not in use" % slot)
 
     def _take(self):
@@ -96,13 +96,13 @@ class PagedCache:
         if not self._free:
             raise CacheFull("all %d cache slots are in use" % self.slots)
         slot = self._free.pop()
-        self.lengths[slot] = 0
+        self.lengths[slot], self._taken[slot] = 0, True
         return slot
 
     def release(self, slot):
         self._used(slot)
         self._give(self.held[slot])
-        self.held[slot], self.lengths[slot] = [], 0
+        self.held[slot], self.lengths[slot], self._taken[slot] = [], 0, False
         self._free.append(slot)
         self.version += 1
 
@@ -115,6 +115,7 @@ class PagedCache:
         if len(set(slots)) != len(slots):
             raise ValueError("a slot twice in one step")
         for s in slots:
+            self._used(s)
             if start != self.lengths[s]:
                 raise ValueError("slot %d holds %d positions, the step starts at %d" % (s, self.lengths[s], start))
         if start + n > self.capacity:
@@ -151,6 +152,7 @@ class PagedCache:
 
     def truncate(self, slot, length):
         """forget the positions from `length` on; a recurrent state can only be forgotten as a whole"""
+        self._used(slot)
         if not 0 <= length <= self.lengths[slot]:
             raise ValueError("slot %d holds %d positions" % (slot, self.lengths[slot]))
         if any(self.states) and length not in (0, self.lengths[slot]):
