@@ -245,7 +245,7 @@ typedef struct {
     float* scratch;        /* zkfp_paged_scratch() floats, this call's alone, aligned to 32 bytes */
     long long q_tok, q_head, k_page, k_pos, k_head, v_page, v_pos, v_head, o_tok, o_head, gate_tok, gate_head;   /* elements */
     long long tokens, pages, table_cols, table_ld, batch;
-    long long max_tokens;  /* most rows a sequence brings; chooses the kernel, no result depends on it */
+    long long max_tokens;  /* most rows a sequence brings; chooses the kernel, and so the order of sums; any number gives right results */
     int heads, kv_heads, d, dv, page, window, dtype;
     float scale, out_scale;
 } zkfp_paged_attention_args;

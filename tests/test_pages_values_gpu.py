@@ -1,6 +1,6 @@
 """Values that calls over pages meet rarely: scores that jump from one tile of keys to the next, keys that are NaN or infinite where a
-row does see them, what lies behind the end of a sequence, infinities and NaN among heads that do not turn, and the status of
-what does not fit."""
+row does see them, what lies behind the end of a sequence, infinities and NaN among heads that do not turn, the status of
+what does not fit, and the bound on rows that is left out."""
 import numpy as np
 import pytest
 import torch
@@ -263,3 +263,13 @@ def test_a_status_of_its_own_for_what_does_not_fit(K, dtype, new, d):
         s[name].copy_(kept)
     attention()
     K.device_status(sync=True)
+
+
+# ---- the bound on rows -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,bound", [([1] * 40, 1), ([1], 1), ([7], 7), ([1, 1, 5, 1], 5), ([0, 0, 2], 1), ([2] * 9, 10)])
+def test_a_bound_that_is_left_out(K, new, bound):
+    """one row for each of the others is taken off; sequences without rows, or with more than that, come out right all the same"""
+    s = pool("bfloat16", new, [100 + 3 * i for i in range(len(new))], 16, 16, 2, 64, 64)
+    made, _ = K._calls.paged_attention(s["q"], s["k"], s["v"], s["table"], s["rows"], s["lengths"], torch.empty_like(s["q"]), 0.1, 0, None, None, 1.0)
+    assert K.PagedAttentionArgs.from_buffer_copy(made).max_tokens == bound
+    check(K, s, "bfloat16")

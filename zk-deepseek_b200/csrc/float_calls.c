@@ -243,7 +243,7 @@ static PyObject* paged_attention(PyObject* self, PyObject* const* x, Py_ssize_t 
         return NULL;
     const double scale = PyFloat_AsDouble(x[7]), out_scale = PyFloat_AsDouble(x[11]);
     if (PyErr_Occurred() || whole(x[8], &window)) return NULL;
-    most = tokens;
+    most = tokens < p.batch ? 1 : tokens - p.batch + 1;        /* if the other sequences bring one row each; it only chooses the kernel */
     if (x[9] != Py_None && whole(x[9], &most)) return NULL;
     if (window < 0 || most < 0 || !(scale >= 0 && scale < 3e38)) {
         refuse(what, "a negative window, bound or scale");

@@ -343,7 +343,9 @@ def paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, windo
     q [tokens, heads, d], out [tokens, heads, dv] (strided views): the rows of every sequence behind one another, a row sees
     the positions up to its own, with window > 0 the last `window` of them.  A row at a negative position (a sequence
     with more rows than positions) sees none and gives zeros; rows behind the last sequence are left as they were.
-    max_tokens: most rows that a sequence brings (default: all), which chooses the kernel.  gate [tokens, heads, dv]: out is
+    max_tokens: most rows that a sequence brings, which chooses the kernel and changes no result but its rounding (default: what is left if
+    every other sequence brings one; a batch of short chunks is better off with its own: 64 sequences of two tokens up to 1000 take 31 us from memory with 2,
+    53 without).  gate [tokens, heads, dv]: out is
     multiplied by sigmoid(gate) * out_scale.  Head sizes up to 256, up to 1024 sequences; scale is not negative; out lies on no
     input."""
     made = _calls.paged_attention(q, k_pages, v_pages, table, rows, lengths, out, scale, window, max_tokens, gate, out_scale)
