@@ -40,6 +40,21 @@ def test_a_model_that_pages_do_not_take_is_refused_unread(float_libpath, tmp_pat
         unread.load(latent, device="cpu", page=16)
 
 
+def test_a_step_of_too_many_sequences_is_refused_unchanged(float_libpath):
+    """in front of the cache, which would have grown, and of the first layer's write"""
+    import torch
+    M = importlib.import_module(PKG + ".float_model")
+    cfg = fc.vifelix(40, 16, 1e-5, 3.0, [fc.parallel(2, 1, 24, 16, 64, 1, 8, 8, 8, [0.9], None)])
+    shapes = {k: v.shape for k, v in fc.make_weights(cfg, 3).items()}
+    args = config.parse_config(cfg, shapes)
+    args.page, args.max_batch_size = 16, 1100
+    model = M.FloatTransformer(args, torch.bfloat16)
+    model.cache = None                                 # whoever asks for it fails
+    for S in (1, 3):
+        with pytest.raises(ValueError, match="1024"):
+            model.step(torch.zeros(1025, S, dtype=torch.int64), 0, list(range(1025)))
+
+
 @pytest.mark.parametrize("more", [["--sample"], ["--samples", "2"], ["--sample", "--top-k", "3", "--samples", "2"]])
 def test_the_program_refuses_to_draw_integer_tokens_unread(tmp_path, monkeypatch, more):
     G, R = (importlib.import_module(PKG + "." + n) for n in ("generate", "registry"))

@@ -38,8 +38,8 @@ except ImportError:  # pragma: no cover - this directory first on sys.path
 ABSORB_MAX_TOKENS = 16
 # a step with more rows than this is run in portions (bounds the activations and the expanded keys and values)
 MAX_STEP_TOKENS = 8192
-# largest head that attention over pages takes
-PAGED_MOST = 256
+# largest head, and most sequences of a step, that attention over pages takes
+PAGED_MOST, PAGED_SEQUENCES = 256, 1024
 
 
 def _padded(t, shape, dtype, device):
@@ -742,6 +742,8 @@ class FloatTransformer(nn.Module):
         stream after every layer.
         """
         B, S = tokens.shape
+        if self.args.page and B > PAGED_SEQUENCES:
+            raise ValueError("a step of %d sequences; over pages, up to %d" % (B, PAGED_SEQUENCES))
         info = {}
         if S == 1 and not layer_probe and layers_out is None and (want is None or len(want)):
             logits = self._decode(tokens, start_pos, slots)
