@@ -34,7 +34,7 @@ __device__ __forceinline__ int sequence_of_row(const int* rows, int batch, long 
 constexpr int kPagedBatch = 1024;
 
 // A division whose divisor the host knows, of 0 <= x < 2^31: the high bits of a product.  (The multiplier is 2^shift / divisor rounded up, its error
-// times x below 2^shift.  What starts a launch is a chain of such steps, each of a CTA's few: with divisions one sequence took 13.2 us, now 12.8, 64 87.3, now 84.5.)
+// times x below 2^shift.  What starts a launch is a chain of such steps, each of a CTA's few: with divisions one sequence took 13.2 us, without 12.8, 64 87.3 and 84.5, by themselves.)
 struct Ratio {
     uint32_t mul;
     int shift;
@@ -272,7 +272,7 @@ __device__ __forceinline__ long long page_of(const Paged& p, int b, int j)
 
 // ---- a row by itself ---------------------------------------------------------------------------------------------
 // The tiles multiply weights of zero with whatever values stand at positions that a row does not see.  Where that
-// is an infinity or a NaN (another row's, or what an earlier owner left in a page), the row's sums are not finite, and the row is
+// is an infinity or a NaN (another row's), or where a visible score is NaN, the row's sums are not finite, and the row is
 // taken once more from the definition, visible positions alone.  A warp takes 32 keys at a time, a lane one key, then a lane every
 // 32nd column.  o[k]: column lane + 32 k.
 template <typename T>

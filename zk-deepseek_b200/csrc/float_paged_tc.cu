@@ -5,7 +5,8 @@
 // and their bytes are the bound.  A warp works by itself: it owns every fourth stretch of 16 keys, loads it by TMA into a ring of its
 // own and keeps maxima, sums and the weighted values of all 16 rows in registers (m16n8k16 products: queries are the
 // A operand and stay in registers, keys and values are read from the swizzled tiles by ldmatrix).  No warp waits for
-// another one before the item ends.  64 sequences up to 8192, 16 key heads of 128: 84 us, 5.6 TB/s; one sequence of 4095, 8 key heads: 12.8.
+// another one before the item ends.  Calls among others, the merge of cut items included: 64 sequences up to 8192, 16 key heads of 128, 88 us,
+// 5.4 TB/s; one sequence of 4095, 8 key heads, 13.2.
 //
 // paged_tile_kernel: more rows.  An item is two tiles of up to 128 rows over tiles of 128 keys: scores and outputs of both in tensor
 // memory, bfloat16 weights overwrite their scores and are the tensor-memory operand of the second product; while one tile is
@@ -16,9 +17,11 @@
 //   warps 2-9   softmax, tile 0    warps 10-17 softmax, tile 1: two threads share a query row, half of the columns each
 // The running maximum only replaces the one in use when it has grown by more than 2^8, and then in front of the next tile, where the
 // output tile is rescaled in place: a tile's weights are made from the maximum in use, without looking for the new one first.  A row whose
-// scores outgrow that by more than 2^100 within one tile is marked by a sum that is NaN, and is taken again.  Weights go to the second product in halves, so that it
+// scores outgrow that by more than 2^100 within one tile is marked by a sum that is NaN, and is taken again.  Values behind the end of the
+// sequence are blanked: what another owner left there would make rows not finite.  Weights go to the second product in halves, so that it
 // starts under the other half.  CTAs stay and take one part of an item after the other.  What bounds it is one tile's softmax under the other's
-// products: a prompt of 4096, 32 heads of 128 over 8, takes 167 us, 0.82 PFLOP/s, the tensor pipe active for 44 %, the exponentials' for as much.
+// products: a call for a prompt of 4096, 32 heads of 128 over 8, takes 182 us among others, 0.76 PFLOP/s, the tensor pipe active for 44 %, the
+// exponentials' for as much.
 #include <cuda.h>
 
 #include "float_paged.cuh"
@@ -56,7 +59,7 @@ constexpr int kStreamWarps = 4, kStretch = 16, kStreamRows = 16, kStreamKeys = k
 constexpr int kStretchSeg = kStretch * 128;            // bytes of 16 keys x 64 columns
 constexpr int kStreamStages = 4;
 // An item by itself costs about as much as 6 blocks of 64 keys, or 2 tiles of 128 (64 sequences up to 8192, microseconds, at 2, 3, 4, 5, 6: 127,
-// 110, 95, 91, 88; a chunk beside decoding sequences at 2, 3, 4: 116, 117, 119; a prompt 170, 171, 175; today 84, 103 and 167).  No CTA takes less than
+// 110, 95, 91, 88; a chunk beside decoding sequences at 2, 3, 4: 116, 117, 119; a prompt 170, 171, 175; today 84, 103 and 167; launches by themselves).  No CTA takes less than
 // 4 blocks, or 2 tiles.
 constexpr int kStreamOver = 6, kStreamLeast = 2, kTileOver = 2, kTileLeast = 1;
 
@@ -435,7 +438,7 @@ struct TileShared {
 };
 
 // ---- the scores of a row -----------------------------------------------------------------------------------------
-// A thread has a row: 128 scores in tensor memory, 32 at a time in registers, the next 32 on their way.
+// Two threads share a row, 64 of its scores in tensor memory each: 32 at a time go through registers.
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float d;
